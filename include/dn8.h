@@ -195,6 +195,138 @@ typedef struct dn8_zoom_args {
 } dn8_zoom_args;
 int dn8_zoom(const dn8_zoom_args* a, dn8_stream stream);
 
+/* ---- the context transformer behind the encoder ----------------------------------------------
+ * The operators of a transformer over a study's tokens (the windows' features, or the places of the
+ * last maps), forward and backward: the reference runs this part of its network (the context
+ * transformer and the attention head per finding, src/knee/models/baseline.py:395-700) in torch.
+ * Types: DN8_F32, DN8_F16, DN8_BF16. Strides are in elements; the last dimension is contiguous. A
+ * call with no rows writes nothing (but a sum over no rows, which is 0). Outputs must not overlap inputs except where it is said. */
+#define DN8_F32 0
+#define DN8_F16 1
+#define DN8_BF16 2
+
+/* Layer norm of `rows` rows of C elements: h = x + res (rounded to x's type and written to sum; h = x
+ * without res), mu = mean(h), r = 1 / sqrt(mean((h - mu)^2) + eps), y = (h - mu) r w + b. Statistics
+ * in fp32. y may be x or res itself where types and strides agree, and so may sum. */
+typedef struct dn8_layer_norm_args {
+    const void* x;          /* [rows][C] x_type */
+    const void* res;        /* x_type, or NULL */
+    const void* w;          /* [C] w_type, or NULL (1) */
+    const void* b;          /* [C] w_type, or NULL (0) */
+    void* y;                /* y_type: x_type, or 16 bits behind an fp32 x */
+    void* sum;              /* x_type; needed with res */
+    float* mean;            /* [rows] or NULL */
+    float* rstd;            /* [rows] or NULL */
+    int64_t rows, x_stride, res_stride, y_stride, sum_stride;   /* elements between rows */
+    int32_t C, x_type, y_type, w_type;
+    float eps;
+} dn8_layer_norm_args;
+int dn8_layer_norm(const dn8_layer_norm_args* a, dn8_stream stream);
+
+/* Its gradient: g = dy w, xh = (x - mean) rstd, dx = rstd (g - mean(g) - xh mean(g xh)) + dsum (rounded
+ * once), dw = sum dy xh, db = sum dy over the rows. x is what was normalised (the stored sum where
+ * there was a residual), mean / rstd the forward pass's. dx is the gradient of x and of res alike.
+ * Sums in a fixed order: the same bits every call. dx may be dy, x or dsum itself where types and
+ * strides agree. */
+typedef struct dn8_layer_norm_bwd_args {
+    const void* dy;         /* [rows][C] y_type */
+    const void* x;          /* x_type */
+    const void* w;          /* [C] w_type, or NULL (1) */
+    const void* dsum;       /* x_type: the gradient that reaches the sum past the norm, or NULL */
+    const float* mean;
+    const float* rstd;
+    void* dx;               /* x_type */
+    void* dw;               /* [C] w_type, or NULL */
+    void* db;               /* [C] w_type, or NULL */
+    void* work;             /* dn8_layer_norm_bwd_work(C) bytes; needed with dw or db */
+    int64_t rows, dy_stride, x_stride, dsum_stride, dx_stride;
+    int32_t C, x_type, y_type, w_type;
+} dn8_layer_norm_bwd_args;
+int dn8_layer_norm_bwd(const dn8_layer_norm_bwd_args* a, dn8_stream stream);
+int64_t dn8_layer_norm_bwd_work(int32_t C);
+
+/* Rotary positions with several axes. The first 2 P elements of a head are P = sum of sections pairs:
+ * (j, j + P), or (2 j, 2 j + 1) when interleaved. sections[x] consecutive pairs belong to axis x; pair j
+ * turns by pos[token][axis] f_j with f_j = base^(-j / P), or base^(-i / sections[x]) for the i-th pair
+ * of axis x when per_axis. (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin); inverse turns back (the
+ * backward pass). Elements behind the pairs are copied. Angles are reduced in 64 bits. q_out may be q
+ * itself and k_out k itself (same strides). P <= 128. */
+#define DN8_ROPE_AXES 4
+typedef struct dn8_rope_args {
+    const void* q;          /* [T][Hq][D] type */
+    const void* k;          /* [T][Hk][D], or NULL with Hk = 0 */
+    const int32_t* pos;     /* [T][n_axes] */
+    void* q_out;
+    void* k_out;
+    int64_t T, q_stride_t, q_stride_h, k_stride_t, k_stride_h, qo_stride_t, qo_stride_h, ko_stride_t, ko_stride_h;
+    int32_t Hq, Hk, D, type, n_axes;
+    int32_t sections[DN8_ROPE_AXES];
+    int32_t per_axis, interleaved, inverse;
+    double base;
+} dn8_rope_args;
+int dn8_rope(const dn8_rope_args* a, dn8_stream stream);
+
+/* Attention over packed sequences. Sequence b: query rows cu_q[b] .. cu_q[b+1] - 1, keys cu_k[b] ..
+ * cu_k[b] + nk - 1, nk = len_k[b] where given (a cache slot filled so far), else cu_k[b+1] - cu_k[b].
+ * Query i of nq stands at p = i + nk - nq and sees key j iff keep[j] (a byte per key row, not zero),
+ * j <= p + right, and (j >= p - left or j < sinks); left or right = -1: no limit on that side.
+ * out = softmax(scale q k) v over the visible keys, lse = log sum exp(scale q k) (natural). A query
+ * that sees nothing: out = 0, lse = -inf. What masked keys hold, and rows of no sequence, is never
+ * used; rows of no sequence are not written. Visible keys and values have to be finite. Query head h
+ * reads key head h / (Hq / Hk). Scores, softmax and sums in fp32; the weights are rounded to `type`
+ * for the second product.
+ * Offsets are checked on the device: a sequence that leaves [0, Tq] or [0, Tk], or a len_k outside its
+ * slot, counts as empty and sets err. D a multiple of 8 up to 128; pointers 16-byte aligned, strides
+ * multiples of 8 elements; type DN8_F16 or DN8_BF16. */
+typedef struct dn8_attention_args {
+    const void* q;          /* [Tq][Hq][D] */
+    const void* k;          /* [Tk][Hk][D] */
+    const void* v;          /* [Tk][Hk][D] */
+    void* out;              /* [Tq][Hq][D] */
+    float* lse;             /* [Tq][Hq], or NULL */
+    const int32_t* cu_q;    /* [B + 1] */
+    const int32_t* cu_k;    /* [B + 1] */
+    const int32_t* len_k;   /* [B], or NULL */
+    const uint8_t* keep;    /* [Tk], or NULL */
+    int32_t* err;           /* device error word (0 = none) or NULL */
+    void* work;             /* dn8_attention_work bytes (may be 0) */
+    int64_t Tq, Tk;
+    int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, o_stride_t, o_stride_h;
+    int32_t B, Hq, Hk, D, type, left, right, sinks;
+    float scale;
+} dn8_attention_args;
+int dn8_attention(const dn8_attention_args* a, dn8_stream stream);
+int64_t dn8_attention_work(const dn8_attention_args* a);    /* of the current device; -1: bad arguments */
+
+/* Its gradient, from the forward pass's inputs, out and lse: P = exp(scale q k - lse) on the visible
+ * pairs, delta = sum(dout out), dv = P^T dout, dS = P (dout v^T - delta) scale, dq = dS k, dk = dS^T q;
+ * dk and dv summed over the query heads of a group. Rows that see nothing, and keys that nobody sees,
+ * get zeros. No atomics: the same bits every call. P and dS are rounded to `type` for the products. */
+typedef struct dn8_attention_bwd_args {
+    const void* dout;       /* [Tq][Hq][D] */
+    const void* q;
+    const void* k;
+    const void* v;
+    const void* out;
+    const float* lse;       /* [Tq][Hq] */
+    void* dq;               /* [Tq][Hq][D] */
+    void* dk;               /* [Tk][Hk][D] */
+    void* dv;               /* [Tk][Hk][D] */
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    const int32_t* len_k;
+    const uint8_t* keep;
+    int32_t* err;
+    void* work;             /* dn8_attention_bwd_work bytes */
+    int64_t Tq, Tk;
+    int64_t do_stride_t, do_stride_h, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h,
+        o_stride_t, o_stride_h, dq_stride_t, dq_stride_h, dk_stride_t, dk_stride_h, dv_stride_t, dv_stride_h;
+    int32_t B, Hq, Hk, D, type, left, right, sinks;
+    float scale;
+} dn8_attention_bwd_args;
+int dn8_attention_bwd(const dn8_attention_bwd_args* a, dn8_stream stream);
+int64_t dn8_attention_bwd_work(const dn8_attention_bwd_args* a);
+
 /* ---- weight preparation (host memory to host memory, once per pack) ------------------------
  * The kernels read their weights with bulk copies straight into the tensor cores' shared-memory
  * operand layout; these functions permute the reference pack tables into that layout. */

@@ -10,7 +10,9 @@ LIB_PATH = Path(__file__).resolve().with_name("libdn8b200.so")
 IN_TREE = LIB_PATH
 DN8_OK, DN8_EINVAL, DN8_ECUDA, DN8_EDEVICE = 0, 1, 2, 3
 DN8_HEAD_SCRATCH_VIEWS = 4096
-P, I32 = ctypes.c_void_p, ctypes.c_int32
+DN8_F32, DN8_F16, DN8_BF16 = 0, 1, 2
+DN8_ROPE_AXES = 4
+P, I32, I64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 
 
 class Conv1Args(ctypes.Structure):
@@ -47,6 +49,46 @@ class ZoomArgs(ctypes.Structure):
                 ("ty", ctypes.c_double)]
 
 
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [("x", P), ("res", P), ("w", P), ("b", P), ("y", P), ("sum", P), ("mean", P), ("rstd", P),
+                ("rows", I64), ("x_stride", I64), ("res_stride", I64), ("y_stride", I64), ("sum_stride", I64),
+                ("C", I32), ("x_type", I32), ("y_type", I32), ("w_type", I32), ("eps", ctypes.c_float)]
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    _fields_ = [("dy", P), ("x", P), ("w", P), ("dsum", P), ("mean", P), ("rstd", P), ("dx", P), ("dw", P), ("db", P),
+                ("work", P), ("rows", I64), ("dy_stride", I64), ("x_stride", I64), ("dsum_stride", I64),
+                ("dx_stride", I64), ("C", I32), ("x_type", I32), ("y_type", I32), ("w_type", I32)]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [("q", P), ("k", P), ("pos", P), ("q_out", P), ("k_out", P), ("T", I64),
+                ("q_stride_t", I64), ("q_stride_h", I64), ("k_stride_t", I64), ("k_stride_h", I64),
+                ("qo_stride_t", I64), ("qo_stride_h", I64), ("ko_stride_t", I64), ("ko_stride_h", I64),
+                ("Hq", I32), ("Hk", I32), ("D", I32), ("type", I32), ("n_axes", I32), ("sections", I32 * DN8_ROPE_AXES),
+                ("per_axis", I32), ("interleaved", I32), ("inverse", I32), ("base", ctypes.c_double)]
+
+
+_MASK = [("B", I32), ("Hq", I32), ("Hk", I32), ("D", I32), ("type", I32), ("left", I32), ("right", I32),
+         ("sinks", I32), ("scale", ctypes.c_float)]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [("q", P), ("k", P), ("v", P), ("out", P), ("lse", P), ("cu_q", P), ("cu_k", P), ("len_k", P),
+                ("keep", P), ("err", P), ("work", P), ("Tq", I64), ("Tk", I64),
+                ("q_stride_t", I64), ("q_stride_h", I64), ("k_stride_t", I64), ("k_stride_h", I64),
+                ("v_stride_t", I64), ("v_stride_h", I64), ("o_stride_t", I64), ("o_stride_h", I64)] + _MASK
+
+
+class AttentionBwdArgs(ctypes.Structure):
+    _fields_ = [("dout", P), ("q", P), ("k", P), ("v", P), ("out", P), ("lse", P), ("dq", P), ("dk", P), ("dv", P),
+                ("cu_q", P), ("cu_k", P), ("len_k", P), ("keep", P), ("err", P), ("work", P), ("Tq", I64), ("Tk", I64),
+                ("do_stride_t", I64), ("do_stride_h", I64), ("q_stride_t", I64), ("q_stride_h", I64),
+                ("k_stride_t", I64), ("k_stride_h", I64), ("v_stride_t", I64), ("v_stride_h", I64),
+                ("o_stride_t", I64), ("o_stride_h", I64), ("dq_stride_t", I64), ("dq_stride_h", I64),
+                ("dk_stride_t", I64), ("dk_stride_h", I64), ("dv_stride_t", I64), ("dv_stride_h", I64)] + _MASK
+
+
 class Table(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("data", P), ("nbytes", ctypes.c_int64)]
 
@@ -77,6 +119,14 @@ EXPORTS = {
     "dn8_head": ([ctypes.POINTER(HeadArgs), P], ctypes.c_int),
     "dn8_head_noalloc": ([ctypes.POINTER(HeadArgs), P], ctypes.c_int),
     "dn8_zoom": ([ctypes.POINTER(ZoomArgs), P], ctypes.c_int),
+    "dn8_layer_norm": ([ctypes.POINTER(LayerNormArgs), P], ctypes.c_int),
+    "dn8_layer_norm_bwd": ([ctypes.POINTER(LayerNormBwdArgs), P], ctypes.c_int),
+    "dn8_layer_norm_bwd_work": ([I32], I64),
+    "dn8_rope": ([ctypes.POINTER(RopeArgs), P], ctypes.c_int),
+    "dn8_attention": ([ctypes.POINTER(AttentionArgs), P], ctypes.c_int),
+    "dn8_attention_work": ([ctypes.POINTER(AttentionArgs)], I64),
+    "dn8_attention_bwd": ([ctypes.POINTER(AttentionBwdArgs), P], ctypes.c_int),
+    "dn8_attention_bwd_work": ([ctypes.POINTER(AttentionBwdArgs)], I64),
     "dn8_prepare_stem_weights": ([P, P], ctypes.c_int),
     "dn8_prepare_conv1_weights": ([P, I32, P], ctypes.c_int),
     "dn8_prepare_trans_weights": ([P, I32, I32, P], ctypes.c_int),

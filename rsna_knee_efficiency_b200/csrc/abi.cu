@@ -222,6 +222,140 @@ int dn8_head_noalloc(const dn8_head_args* a, dn8_stream stream) {
     return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_head_noalloc launch");
 }
 
+// ---- the context transformer's operators ----
+
+static bool float_type(int t) { return t == DN8_F32 || t == DN8_F16 || t == DN8_BF16; }
+
+int dn8_layer_norm(const dn8_layer_norm_args* a, dn8_stream stream) {
+    if (a == nullptr) return fail(DN8_EINVAL, "dn8_layer_norm: null arguments");
+    if (a->rows < 0 || a->rows >= (1ll << 31) || a->C < 1 || !(a->eps >= 0.0f))
+        return fail(DN8_EINVAL, "dn8_layer_norm: bad geometry rows=%lld C=%d eps=%g", static_cast<long long>(a->rows), a->C,
+                    a->eps);
+    if (!float_type(a->x_type) || !float_type(a->y_type) || !float_type(a->w_type) ||
+        (a->x_type != a->y_type && a->x_type != DN8_F32))
+        return fail(DN8_EINVAL, "dn8_layer_norm: types x=%d y=%d w=%d (y of x's type, or 16 bits behind fp32)", a->x_type,
+                    a->y_type, a->w_type);
+    if (a->rows == 0) return DN8_OK;
+    if (a->x == nullptr || a->y == nullptr || (a->res != nullptr && a->sum == nullptr))
+        return fail(DN8_EINVAL, "dn8_layer_norm: x and y, and sum with res, must not be null");
+    cudaError_t e = dn8::launch_layer_norm(*a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_layer_norm launch");
+}
+
+int64_t dn8_layer_norm_bwd_work(int32_t C) { return C < 1 ? -1 : static_cast<int64_t>(dn8::layer_norm_bwd_work(C)); }
+
+int dn8_layer_norm_bwd(const dn8_layer_norm_bwd_args* a, dn8_stream stream) {
+    if (a == nullptr) return fail(DN8_EINVAL, "dn8_layer_norm_bwd: null arguments");
+    if (a->rows < 0 || a->rows >= (1ll << 31) || a->C < 1)
+        return fail(DN8_EINVAL, "dn8_layer_norm_bwd: bad geometry rows=%lld C=%d", static_cast<long long>(a->rows), a->C);
+    if (!float_type(a->x_type) || !float_type(a->y_type) || !float_type(a->w_type) ||
+        (a->x_type != a->y_type && a->x_type != DN8_F32))
+        return fail(DN8_EINVAL, "dn8_layer_norm_bwd: types x=%d y=%d w=%d (y of x's type, or 16 bits behind fp32)",
+                    a->x_type, a->y_type, a->w_type);
+    if ((a->dw != nullptr || a->db != nullptr) && a->work == nullptr)
+        return fail(DN8_EINVAL, "dn8_layer_norm_bwd: dw and db need the workspace");
+    if (a->rows > 0 && (a->dy == nullptr || a->x == nullptr || a->mean == nullptr || a->rstd == nullptr || a->dx == nullptr))
+        return fail(DN8_EINVAL, "dn8_layer_norm_bwd: dy, x, mean, rstd and dx must not be null");
+    cudaError_t e = dn8::launch_layer_norm_bwd(*a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_layer_norm_bwd launch");
+}
+
+int dn8_rope(const dn8_rope_args* a, dn8_stream stream) {
+    if (a == nullptr) return fail(DN8_EINVAL, "dn8_rope: null arguments");
+    long long pairs = 0;
+    if (a->n_axes < 1 || a->n_axes > DN8_ROPE_AXES)
+        return fail(DN8_EINVAL, "dn8_rope: %d axes (1 to %d)", a->n_axes, DN8_ROPE_AXES);
+    for (int x = 0; x < a->n_axes; ++x) {
+        if (a->sections[x] < 0) return fail(DN8_EINVAL, "dn8_rope: negative section");
+        pairs += a->sections[x];
+    }
+    if (a->T < 0 || a->T >= (1ll << 31) || a->Hq < 1 || a->Hk < 0 || a->Hq + static_cast<long long>(a->Hk) > 4096 ||
+        pairs < 1 || pairs > 128 || a->D > 4096 || 2 * pairs > a->D)
+        return fail(DN8_EINVAL, "dn8_rope: bad geometry T=%lld Hq=%d Hk=%d D=%d pairs=%lld", static_cast<long long>(a->T),
+                    a->Hq, a->Hk, a->D, pairs);
+    if (!float_type(a->type)) return fail(DN8_EINVAL, "dn8_rope: type %d", a->type);
+    if (!(a->base > 0.0) || !(a->base < 1e300)) return fail(DN8_EINVAL, "dn8_rope: base %g", a->base);
+    if (a->T == 0) return DN8_OK;
+    if (a->q == nullptr || a->q_out == nullptr || a->pos == nullptr || (a->Hk > 0 && (a->k == nullptr || a->k_out == nullptr)))
+        return fail(DN8_EINVAL, "dn8_rope: null pointers");
+    int sms = 0;
+    if (int s = current_sms(&sms)) return s;
+    cudaError_t e = dn8::launch_rope(*a, sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_rope launch");
+}
+
+}  // extern "C"
+
+// What both directions of attention have in common; `call` names the entry point in the message.
+template <typename A> static int check_attention(const A* a, const char* call) {
+    if (a == nullptr) return fail(DN8_EINVAL, "%s: null arguments", call);
+    if (a->B < 0 || a->Tq < 0 || a->Tk < 0 || a->Tq >= (1ll << 30) || a->Tk >= (1ll << 30) || a->Hk < 1 || a->Hk > 65535 ||
+        a->Hq < 1 || a->Hq > 65535 || a->Hq % a->Hk)
+        return fail(DN8_EINVAL, "%s: bad geometry B=%d Tq=%lld Tk=%lld Hq=%d Hk=%d", call, a->B,
+                    static_cast<long long>(a->Tq), static_cast<long long>(a->Tk), a->Hq, a->Hk);
+    if (a->Tq * (a->Hq / a->Hk) >= (1ll << 30)) return fail(DN8_EINVAL, "%s: Tq Hq / Hk exceeds 2^30", call);
+    if (a->D < 8 || a->D > 128 || a->D % 8) return fail(DN8_EINVAL, "%s: head size %d (a multiple of 8 up to 128)", call, a->D);
+    if (a->type != DN8_F16 && a->type != DN8_BF16) return fail(DN8_EINVAL, "%s: type %d (16 bits)", call, a->type);
+    if (a->left < -1 || a->right < -1 || a->sinks < 0 || a->left > (1 << 30) || a->right > (1 << 30))
+        return fail(DN8_EINVAL, "%s: window left=%d right=%d sinks=%d", call, a->left, a->right, a->sinks);
+    if (!(a->scale > -1e30f && a->scale < 1e30f)) return fail(DN8_EINVAL, "%s: scale %g", call, a->scale);
+    const int64_t strides[] = {a->q_stride_t, a->q_stride_h, a->k_stride_t, a->k_stride_h,
+                               a->v_stride_t, a->v_stride_h, a->o_stride_t, a->o_stride_h};
+    for (int64_t s : strides)
+        if (s < 0 || s % 8 || s >= (1ll << 38)) return fail(DN8_EINVAL, "%s: strides must be multiples of 8 elements", call);
+    if (a->Tq > 0 && a->B > 0 && (a->q == nullptr || a->out == nullptr || !aligned16(a->q) || !aligned16(a->out)))
+        return fail(DN8_EINVAL, "%s: pointers must be non-null and 16-byte aligned", call);
+    if (a->Tk > 0 && a->B > 0 && (a->k == nullptr || a->v == nullptr || !aligned16(a->k) || !aligned16(a->v)))
+        return fail(DN8_EINVAL, "%s: pointers must be non-null and 16-byte aligned", call);
+    if (a->B > 0 && (a->cu_q == nullptr || a->cu_k == nullptr)) return fail(DN8_EINVAL, "%s: cu_q and cu_k are needed", call);
+    return DN8_OK;
+}
+
+extern "C" {
+
+int64_t dn8_attention_work(const dn8_attention_args* a) {
+    if (check_attention(a, "dn8_attention_work")) return -1;
+    if (a->B == 0 || a->Tq == 0) return 0;
+    int sms = 0;
+    if (current_sms(&sms)) return -1;
+    return static_cast<int64_t>(dn8::attention_work(*a, sms));
+}
+
+int dn8_attention(const dn8_attention_args* a, dn8_stream stream) {
+    if (int s = check_attention(a, "dn8_attention")) return s;
+    if (a->B == 0 || a->Tq == 0) return DN8_OK;
+    int sms = 0;
+    if (int s = current_sms(&sms)) return s;
+    if (dn8::attention_work(*a, sms) > 0 && !(a->work != nullptr && aligned16(a->work)))
+        return fail(DN8_EINVAL, "dn8_attention: this call needs a 16-byte aligned workspace");
+    cudaError_t e = dn8::launch_attention(*a, sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_attention launch");
+}
+
+int64_t dn8_attention_bwd_work(const dn8_attention_bwd_args* a) {
+    if (check_attention(a, "dn8_attention_bwd_work")) return -1;
+    return a->B == 0 ? 0 : static_cast<int64_t>(dn8::attention_bwd_work(*a));
+}
+
+int dn8_attention_bwd(const dn8_attention_bwd_args* a, dn8_stream stream) {
+    if (int s = check_attention(a, "dn8_attention_bwd")) return s;
+    if (a->B == 0 || (a->Tq == 0 && a->Tk == 0)) return DN8_OK;
+    const int64_t strides[] = {a->do_stride_t, a->do_stride_h, a->dq_stride_t, a->dq_stride_h,
+                               a->dk_stride_t, a->dk_stride_h, a->dv_stride_t, a->dv_stride_h};
+    for (int64_t s : strides)
+        if (s < 0 || s % 8 || s >= (1ll << 38))
+            return fail(DN8_EINVAL, "dn8_attention_bwd: strides must be multiples of 8 elements");
+    if (a->Tq > 0 && (a->dout == nullptr || a->dq == nullptr || a->lse == nullptr || a->work == nullptr ||
+                      !aligned16(a->dout) || !aligned16(a->dq) || !aligned16(a->work)))
+        return fail(DN8_EINVAL, "dn8_attention_bwd: pointers must be non-null and 16-byte aligned");
+    if (a->Tk > 0 && (a->dk == nullptr || a->dv == nullptr || !aligned16(a->dk) || !aligned16(a->dv)))
+        return fail(DN8_EINVAL, "dn8_attention_bwd: pointers must be non-null and 16-byte aligned");
+    int sms = 0;
+    if (int s = current_sms(&sms)) return s;
+    cudaError_t e = dn8::launch_attention_bwd(*a, sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_attention_bwd launch");
+}
+
 int dn8_test_inject_wait_fault(int32_t fault, int64_t wait_limit_cycles) {
     if (fault < 0 || fault > 1 || wait_limit_cycles < 0 || (fault == 1 && wait_limit_cycles == 0))
         return fail(DN8_EINVAL, "dn8_test_inject_wait_fault: fault 0 or 1 (with a wait limit > 0)");

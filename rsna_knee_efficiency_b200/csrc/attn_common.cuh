@@ -1,0 +1,93 @@
+// attn_common.cuh -- what the attention kernels share: the sequences of a packed batch, the keys a
+// query sees, and the split of the work.
+//
+// Sequence b holds the query rows cu_q[b] .. cu_q[b+1] - 1 and the keys cu_k[b] .. cu_k[b] + nk - 1 with
+// nk = len_k[b] where given (a cache slot filled so far), else cu_k[b+1] - cu_k[b]. Query i of nq
+// stands at position p = i + nk - nq and sees key j iff keep[j], j <= p + right and (j >= p - left or
+// j < sinks); a negative left or right is no limit on that side.
+#pragma once
+#include "ctx_common.cuh"
+#include "dn8_kernels.h"
+
+namespace dn8 {
+
+constexpr int ATT_FAR = 1 << 30;              // "no limit": beyond every length (checked < 2^30)
+constexpr float ATT_LOG2E = 1.4426950408889634f, ATT_LN2 = 0.6931471805599453f;
+
+struct Sequence {
+    int b;             // sequence, or -1: none
+    int q0, nq;        // first query row, queries
+    int k0, nk;        // first key row, keys
+    int blk;           // which block of the sequence's rows (or keys)
+};
+
+// Rows [s, e) of a sequence inside [0, T), or an error and no rows: offsets come from device memory,
+// so the kernels check them before they become addresses.
+DN8_DEV int checked_len(int s, int e, int64_t T, int* err) {
+    if (s >= 0 && e >= s && e <= T) return e - s;
+    if (err != nullptr) atomicCAS(err, 0, ERR_SHAPE);
+    return 0;
+}
+template <typename A> DN8_DEV int keys_of(const A& a, int b) {
+    const int s = a.cu_k[b], full = checked_len(s, a.cu_k[b + 1], a.Tk, a.err);
+    if (a.len_k == nullptr) return full;
+    return checked_len(0, a.len_k[b], full, a.err);
+}
+
+// Block `unit` of the batch when every sequence is cut into ceil(len mul / per) blocks, len being its
+// queries (KEYS = false) or its keys. Called by one whole warp.
+template <bool KEYS, typename A> DN8_DEV Sequence find_block(const A& a, int unit, int mul, int per) {
+    const int lane = threadIdx.x & 31;
+    int run = 0;
+    Sequence s;
+    s.b = -1;
+    for (int base = 0; base < a.B; base += 32) {
+        const int b = base + lane;
+        int n = 0;
+        if (b < a.B) n = KEYS ? keys_of(a, b) : checked_len(a.cu_q[b], a.cu_q[b + 1], a.Tq, a.err);
+        const int mine = static_cast<int>((static_cast<int64_t>(n) * mul + per - 1) / per);
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, unit < run + incl);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            s.b = base + src;
+            s.blk = unit - run - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src));
+            break;
+        }
+        run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (s.b >= 0) {
+        s.q0 = a.cu_q[s.b];
+        s.nq = checked_len(s.q0, a.cu_q[s.b + 1], a.Tq, a.err);
+        s.k0 = a.cu_k[s.b];
+        s.nk = keys_of(a, s.b);
+    }
+    return s;
+}
+
+// Key tiles of TILE keys that queries at positions p0 .. p1 see some key of: the tiles of the first
+// tokens, then those of the window. tile(t) for t = 0 .. count - 1.
+struct KeyTiles {
+    int first;         // tiles 0 .. first - 1: first tokens
+    int start;         // then start, start + 1, ...
+    int count;
+    DN8_DEV int tile(int t) const { return t < first ? t : start + t - first; }
+};
+DN8_DEV KeyTiles key_tiles(int p0, int p1, int nk, int left, int right, int sinks, int tile) {
+    const int hi = min(nk - 1, p1 + right), lo = max(0, p0 - left);
+    KeyTiles k;
+    k.first = k.start = k.count = 0;
+    if (hi < 0) return k;
+    const int s = min(sinks, hi + 1);                          // first tokens that may be seen
+    k.start = lo / tile;
+    if (k.start > 0) k.first = min(k.start, (s + tile - 1) / tile);
+    k.count = k.first + max(0, hi / tile - k.start + 1);
+    return k;
+}
+
+}  // namespace dn8

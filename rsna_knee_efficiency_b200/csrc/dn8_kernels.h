@@ -64,6 +64,14 @@ int trans_chunk(int cout);
 cudaError_t launch_stem(const dn8_stem_args& a, int sms, cudaStream_t st);
 cudaError_t launch_head(const dn8_head_args& a, cudaStream_t st, bool pdl = false);
 cudaError_t launch_zoom(const dn8_zoom_args& a, int sms, cudaStream_t st);
+cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, cudaStream_t st);
+cudaError_t launch_layer_norm_bwd(const dn8_layer_norm_bwd_args& a, cudaStream_t st);
+size_t layer_norm_bwd_work(int C);
+cudaError_t launch_rope(const dn8_rope_args& a, int sms, cudaStream_t st);
+cudaError_t launch_attention(const dn8_attention_args& a, int sms, cudaStream_t st);
+size_t attention_work(const dn8_attention_args& a, int sms);
+cudaError_t launch_attention_bwd(const dn8_attention_bwd_args& a, int sms, cudaStream_t st);
+size_t attention_bwd_work(const dn8_attention_bwd_args& a);
 constexpr int DN8_MAX_DEVICES = 64;
 cudaError_t head_scratch_tickets(int32_t** out);
 

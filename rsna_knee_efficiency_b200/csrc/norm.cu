@@ -1,0 +1,427 @@
+// norm.cu -- layer norm over the rows of a matrix, forward and backward, with the residual sum in
+// front of it and the reduction of the weight's and the bias's gradient.
+//
+//   h = x + res (rounded to x's type: the stored sum is what the statistics, and later the backward
+//   pass, see), mu = sum h / C, var = sum (h - mu)^2 / C, r = 1 / sqrt(var + eps), y = (h - mu) r w + b
+//   g = dy w, xh = (h - mu) r, dx = r (g - mean(g) - xh mean(g xh)) + dsum, dw = sum dy xh, db = sum dy
+//
+// Both passes are bound by memory: a row is read once into registers (a team of 32, 128 or 512
+// threads per row, so that a thread holds at most 32 values), the variance is summed from the
+// registers as squares of differences (no cancellation of E[x^2] - mu^2), and written once.
+// Statistics and sums are fp32.
+#include "ctx_common.cuh"
+#include "dn8_kernels.h"
+
+namespace dn8 {
+
+// Sum of one value per thread over a team of TPR threads; every thread gets the same sum. `red`
+// holds a float per warp and is free for the next call after the second barrier.
+template <int TPR> DN8_DEV float team_sum(float v, float* red) {
+    v = warp_sum(v);
+    if (TPR == 32) return v;
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) s += red[w];
+    __syncthreads();
+    return s;
+}
+template <int TPR> DN8_DEV void team_sum2(float& a, float& b, float* red) {
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (TPR == 32) return;
+    const int warp = (threadIdx.x % TPR) >> 5;               // `red` is the team's
+    if ((threadIdx.x & 31) == 0) {
+        red[warp] = a;
+        red[TPR / 32 + warp] = b;
+    }
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) {
+        a += red[w];
+        b += red[TPR / 32 + w];
+    }
+    __syncthreads();
+}
+
+// One row per team; a block holds 128 / TPR teams (at least one).
+template <typename TX, typename TY, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) ln_kernel(const dn8_layer_norm_args a) {
+    constexpr int TEAMS = TPR < 128 ? 128 / TPR : 1;
+    __shared__ float red[TPR / 32];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + threadIdx.x / TPR;
+    if (row >= a.rows) return;                               // a whole team (TPR > 32: a whole block)
+    const int t = threadIdx.x % TPR, C = a.C;
+    const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
+    float h[NV][VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (t + k * TPR) * VEC;
+        if (c < C) load_f32(x + c, h[k]);
+    }
+    if (a.res != nullptr) {
+        const TX* res = static_cast<const TX*>(a.res) + row * a.res_stride;
+        TX* sum = static_cast<TX*>(a.sum) + row * a.sum_stride;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (t + k * TPR) * VEC;
+            if (c < C) {
+                float r[VEC];
+                load_f32(res + c, r);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) h[k][e] = to_f32(from_f32<TX>(h[k][e] + r[e]));
+                store_f32(sum + c, h[k]);
+            }
+        }
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+        if ((t + k * TPR) * VEC < C)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += h[k][e];
+    const float mu = team_sum<TPR>(s, red) / static_cast<float>(C);
+    float q = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+        if ((t + k * TPR) * VEC < C)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = h[k][e] - mu;
+                q = fmaf(d, d, q);
+            }
+    const float r = rsqrtf(team_sum<TPR>(q, red) / static_cast<float>(C) + a.eps);
+    TY* y = static_cast<TY*>(a.y) + row * a.y_stride;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (t + k * TPR) * VEC;
+        if (c < C) {
+            float w[VEC], b[VEC], o[VEC];
+            if (a.w != nullptr) load_param(a.w, a.w_type, c, w);
+            if (a.b != nullptr) load_param(a.b, a.w_type, c, b);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                o[e] = fmaf((h[k][e] - mu) * r, a.w != nullptr ? w[e] : 1.0f, a.b != nullptr ? b[e] : 0.0f);
+            store_f32(y + c, o);
+        }
+    }
+    if (t == 0) {
+        if (a.mean != nullptr) a.mean[row] = mu;
+        if (a.rstd != nullptr) a.rstd[row] = r;
+    }
+}
+
+// Rows longer than a team's registers hold: one block per row, the sum's row read again (from L2) for
+// the variance and for the output.
+template <typename TX, typename TY>
+__global__ void __launch_bounds__(512) ln_long_kernel(const dn8_layer_norm_args a) {
+    __shared__ float red[16];
+    const int64_t row = blockIdx.x;
+    const int C = a.C;
+    const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
+    TX* sum = a.res != nullptr ? static_cast<TX*>(a.sum) + row * a.sum_stride : nullptr;
+    const TX* res = a.res != nullptr ? static_cast<const TX*>(a.res) + row * a.res_stride : nullptr;
+    float s = 0.0f;
+    for (int c = threadIdx.x; c < C; c += 512) {
+        float v = to_f32(x[c]);
+        if (res != nullptr) {
+            const TX hv = from_f32<TX>(v + to_f32(res[c]));
+            sum[c] = hv;
+            v = to_f32(hv);
+        }
+        s += v;
+    }
+    const TX* h = res != nullptr ? sum : x;                  // a thread reads back its own columns
+    const float mu = team_sum<512>(s, red) / static_cast<float>(C);
+    float q = 0.0f;
+    for (int c = threadIdx.x; c < C; c += 512) {
+        const float d = to_f32(h[c]) - mu;
+        q = fmaf(d, d, q);
+    }
+    const float r = rsqrtf(team_sum<512>(q, red) / static_cast<float>(C) + a.eps);
+    TY* y = static_cast<TY*>(a.y) + row * a.y_stride;
+    for (int c = threadIdx.x; c < C; c += 512) {
+        float w[1] = {1.0f}, b[1] = {0.0f};
+        if (a.w != nullptr) load_param(a.w, a.w_type, c, w);
+        if (a.b != nullptr) load_param(a.b, a.w_type, c, b);
+        y[c] = from_f32<TY>(fmaf((to_f32(h[c]) - mu) * r, w[0], b[0]));
+    }
+    if (threadIdx.x == 0) {
+        if (a.mean != nullptr) a.mean[row] = mu;
+        if (a.rstd != nullptr) a.rstd[row] = r;
+    }
+}
+
+// Backward: persistent blocks of TEAMS teams; a thread keeps the same columns for every row, so the
+// sums of dy xh and dy over the block's rows stay in its registers. They are added over the teams in
+// shared memory and written as one row of the workspace [gridDim.x][2][C]; ln_cols_kernel adds the
+// rows in a fixed order (no atomics: the same bits every call).
+template <typename TX, typename TY, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) ln_bwd_kernel(const dn8_layer_norm_bwd_args a) {
+    constexpr int THREADS = TPR < 256 ? 256 : TPR;
+    constexpr int TEAMS = THREADS / TPR, CB = NV * VEC * TPR;      // columns a team covers
+    __shared__ float red[TEAMS][2 * TPR / 32];
+    __shared__ float part[TEAMS > 1 ? 2 * CB : 1];
+    griddep_launch_dependents();
+    const int team = threadIdx.x / TPR, t = threadIdx.x % TPR, C = a.C;
+    float dw[NV][VEC], db[NV][VEC], w[NV][VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (t + k * TPR) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            dw[k][e] = db[k][e] = 0.0f;
+            w[k][e] = 1.0f;
+        }
+        if (c < C && a.w != nullptr) load_param(a.w, a.w_type, c, w[k]);
+    }
+    const float inv_c = 1.0f / static_cast<float>(C);
+    // every team of a block makes the same number of steps (the barriers of team_sum2)
+    const int64_t step = static_cast<int64_t>(gridDim.x) * TEAMS;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * TEAMS; base < a.rows; base += step) {
+        const int64_t row = base + team;
+        const bool live = row < a.rows;
+        float dy[NV][VEC], xh[NV][VEC];
+        float s1 = 0.0f, s2 = 0.0f, r = 0.0f;
+        if (live) {
+            const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
+            const TY* g = static_cast<const TY*>(a.dy) + row * a.dy_stride;
+            const float mu = a.mean[row];
+            r = a.rstd[row];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = (t + k * TPR) * VEC;
+                if (c < C) {
+                    load_f32(x + c, xh[k]);
+                    load_f32(g + c, dy[k]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if ((t + k * TPR) * VEC < C)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        xh[k][e] = (xh[k][e] - mu) * r;
+                        const float gv = dy[k][e] * w[k][e];
+                        s1 += gv;
+                        s2 = fmaf(gv, xh[k][e], s2);
+                        dw[k][e] = fmaf(dy[k][e], xh[k][e], dw[k][e]);
+                        db[k][e] += dy[k][e];
+                    }
+        }
+        team_sum2<TPR>(s1, s2, red[team]);
+        if (!live) continue;
+        s1 *= inv_c;
+        s2 *= inv_c;
+        TX* dx = static_cast<TX*>(a.dx) + row * a.dx_stride;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (t + k * TPR) * VEC;
+            if (c < C) {
+                float o[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o[e] = r * (dy[k][e] * w[k][e] - s1 - xh[k][e] * s2);
+                if (a.dsum != nullptr) {
+                    float d[VEC];
+                    load_f32(static_cast<const TX*>(a.dsum) + row * a.dsum_stride + c, d);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) o[e] += d[e];
+                }
+                store_f32(dx + c, o);
+            }
+        }
+    }
+    if (a.work == nullptr) return;
+    float* ws = static_cast<float*>(a.work) + static_cast<size_t>(blockIdx.x) * 2 * C;
+    if (TEAMS > 1) {
+        // one team after the other adds its sums (a fixed order)
+        for (int m = 0; m < TEAMS; ++m) {
+            if (team == m)
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int c = (t + k * TPR) * VEC + e;
+                        part[c] = (m ? part[c] : 0.0f) + dw[k][e];
+                        part[CB + c] = (m ? part[CB + c] : 0.0f) + db[k][e];
+                    }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < C; c += THREADS) {
+            ws[c] = part[c];
+            ws[C + c] = part[CB + c];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int c = (t + k * TPR) * VEC + e;
+                if (c < C) {
+                    ws[c] = dw[k][e];
+                    ws[C + c] = db[k][e];
+                }
+            }
+    }
+}
+
+// Rows longer than a team's registers hold: dx by one block per row (dy and h read twice) ...
+template <typename TX, typename TY>
+__global__ void __launch_bounds__(512) ln_bwd_long_kernel(const dn8_layer_norm_bwd_args a) {
+    __shared__ float red[32];
+    const int64_t row = blockIdx.x;
+    const int C = a.C;
+    const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
+    const TY* dy = static_cast<const TY*>(a.dy) + row * a.dy_stride;
+    const float mu = a.mean[row], r = a.rstd[row];
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int c = threadIdx.x; c < C; c += 512) {
+        float w[1] = {1.0f};
+        if (a.w != nullptr) load_param(a.w, a.w_type, c, w);
+        const float g = to_f32(dy[c]) * w[0];
+        s1 += g;
+        s2 = fmaf(g, (to_f32(x[c]) - mu) * r, s2);
+    }
+    team_sum2<512>(s1, s2, red);
+    s1 /= static_cast<float>(C);
+    s2 /= static_cast<float>(C);
+    TX* dx = static_cast<TX*>(a.dx) + row * a.dx_stride;
+    for (int c = threadIdx.x; c < C; c += 512) {
+        float w[1] = {1.0f};
+        if (a.w != nullptr) load_param(a.w, a.w_type, c, w);
+        float o = r * (to_f32(dy[c]) * w[0] - s1 - (to_f32(x[c]) - mu) * r * s2);
+        if (a.dsum != nullptr) o += to_f32((static_cast<const TX*>(a.dsum) + row * a.dsum_stride)[c]);
+        dx[c] = from_f32<TX>(o);
+    }
+}
+// ... and the sums of a slab of rows (blockIdx.y of gridDim.y) by one thread per column. It runs before
+// ln_bwd_long_kernel, whose dx may be dy's or dsum's own memory.
+template <typename TX, typename TY>
+__global__ void __launch_bounds__(256) ln_bwd_long_cols_kernel(const dn8_layer_norm_bwd_args a) {
+    const int c = blockIdx.x * 256 + threadIdx.x, C = a.C;
+    if (c >= C) return;
+    const int64_t per = (a.rows + gridDim.y - 1) / gridDim.y;
+    const int64_t r0 = per * blockIdx.y, r1 = min(a.rows, r0 + per);
+    float dw = 0.0f, db = 0.0f;
+    for (int64_t row = r0; row < r1; ++row) {
+        const float dy = to_f32(static_cast<const TY*>(a.dy)[row * a.dy_stride + c]);
+        const float h = to_f32(static_cast<const TX*>(a.x)[row * a.x_stride + c]);
+        dw = fmaf(dy, (h - a.mean[row]) * a.rstd[row], dw);
+        db += dy;
+    }
+    float* ws = static_cast<float*>(a.work) + static_cast<size_t>(blockIdx.y) * 2 * C;
+    ws[c] = dw;
+    ws[C + c] = db;
+}
+
+// dw, db = the sum of the workspace's rows: 32 columns per block, 32 threads adding every 32nd row of
+// a column, then a fixed tree.
+__global__ void __launch_bounds__(1024) ln_cols_kernel(const float* work, int nrows, int C, void* dw, void* db, int type) {
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;                    // column of [2][C]
+    griddep_wait();
+    float s = 0.0f;
+    if (c < 2 * C)
+        for (int r = ty; r < nrows; r += 32) s += work[static_cast<size_t>(r) * 2 * C + c];
+    part[ty][lane] = s;
+    __syncthreads();
+    s = warp_sum(part[lane][ty]);                            // column ty of the block's 32
+    const int co = blockIdx.x * 32 + ty;
+    if (lane == 0 && co < 2 * C) {
+        void* dst = co < C ? dw : db;
+        const int k = co < C ? co : co - C;
+        if (dst == nullptr) return;
+        if (type == DN8_F32) static_cast<float*>(dst)[k] = s;
+        else if (type == DN8_F16) static_cast<__half*>(dst)[k] = __float2half_rn(s);
+        else static_cast<__nv_bfloat16*>(dst)[k] = __float2bfloat16_rn(s);
+    }
+}
+
+namespace {
+
+bool vec_ok(const void* p, int64_t stride, int size) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (stride * size) % 16 == 0;
+}
+int type_size(int type) { return type == DN8_F32 ? 4 : 2; }
+
+constexpr int LN_COLS_ROWS = 296;       // rows of the backward pass's workspace (two blocks per SM)
+
+// x's and y's types: equal, or fp32 in and 16 bits out
+template <typename F> cudaError_t with_types(int tx, int ty, F&& f) {
+    if (tx == ty) return with_type(tx, [&](auto t) { return f(t, t); });
+    if (tx != DN8_F32) return cudaErrorInvalidValue;
+    return ty == DN8_F16 ? f(float(), __half()) : f(float(), __nv_bfloat16());
+}
+
+template <typename TX, typename TY, int VEC, int NV>
+cudaError_t ln_go(const dn8_layer_norm_args& a, cudaStream_t st) {
+    const int per = VEC * NV;
+    const dim3 rows(static_cast<unsigned>(a.rows)), rows4(static_cast<unsigned>((a.rows + 3) / 4));
+    if (a.C <= 32 * per) return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, 32>, rows4, dim3(128), 0, st, a);
+    if (a.C <= 128 * per) return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, 128>, rows, dim3(128), 0, st, a);
+    if (a.C <= 512 * per) return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, 512>, rows, dim3(512), 0, st, a);
+    return launch_pdl(false, ln_long_kernel<TX, TY>, rows, dim3(512), 0, st, a);
+}
+
+template <typename TX, typename TY, int VEC, int NV>
+cudaError_t ln_bwd_go(const dn8_layer_norm_bwd_args& a, cudaStream_t st, int* nrows) {
+    const int per = VEC * NV;
+    const int teams = a.C <= 32 * per ? 8 : a.C <= 128 * per ? 2 : 1;
+    const int64_t want = (a.rows + teams - 1) / teams;
+    const int grid = static_cast<int>(want < LN_COLS_ROWS ? want : LN_COLS_ROWS);
+    *nrows = grid;
+    if (a.C <= 32 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 32>, dim3(grid), dim3(256), 0, st, a);
+    if (a.C <= 128 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 128>, dim3(grid), dim3(256), 0, st, a);
+    if (a.C <= 512 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 512>, dim3(grid), dim3(512), 0, st, a);
+    if (a.work != nullptr) {
+        const int slabs = static_cast<int>(a.rows < 32 ? 1 : a.rows / 32 < LN_COLS_ROWS ? a.rows / 32 : LN_COLS_ROWS);
+        *nrows = slabs;
+        cudaError_t e = launch_pdl(false, ln_bwd_long_cols_kernel<TX, TY>, dim3((a.C + 255) / 256, slabs), dim3(256), 0, st, a);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(false, ln_bwd_long_kernel<TX, TY>, dim3(static_cast<unsigned>(a.rows)), dim3(512), 0, st, a);
+}
+
+}  // namespace
+
+cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, cudaStream_t st) {
+    const int sx = type_size(a.x_type), sy = type_size(a.y_type);
+    const bool vec = a.C % 8 == 0 && vec_ok(a.w, 0, 4) && vec_ok(a.b, 0, 4) && vec_ok(a.x, a.x_stride, sx) &&
+                     vec_ok(a.y, a.y_stride, sy) &&
+                     (a.res == nullptr || (vec_ok(a.res, a.res_stride, sx) && vec_ok(a.sum, a.sum_stride, sx)));
+    return with_types(a.x_type, a.y_type, [&](auto tx, auto ty) {
+        using TX = decltype(tx);
+        using TY = decltype(ty);
+        // 16-byte loads where every row allows them, single elements otherwise
+        if (!vec) return ln_go<TX, TY, 1, 16>(a, st);
+        if (sizeof(TX) == 4) return ln_go<TX, TY, 4, 8>(a, st);
+        return ln_go<TX, TY, 8, 4>(a, st);
+    });
+}
+
+size_t layer_norm_bwd_work(int C) { return static_cast<size_t>(LN_COLS_ROWS) * 2 * C * sizeof(float); }
+
+cudaError_t launch_layer_norm_bwd(const dn8_layer_norm_bwd_args& args, cudaStream_t st) {
+    dn8_layer_norm_bwd_args a = args;
+    if (a.dw == nullptr && a.db == nullptr) a.work = nullptr;
+    const int sx = type_size(a.x_type), sy = type_size(a.y_type);
+    const bool vec = a.C % 8 == 0 && vec_ok(a.w, 0, 4) && vec_ok(a.x, a.x_stride, sx) && vec_ok(a.dy, a.dy_stride, sy) &&
+                     vec_ok(a.dx, a.dx_stride, sx) && (a.dsum == nullptr || vec_ok(a.dsum, a.dsum_stride, sx));
+    int nrows = 0;
+    cudaError_t e = a.rows == 0 ? cudaSuccess : with_types(a.x_type, a.y_type, [&](auto tx, auto ty) {
+        using TX = decltype(tx);
+        using TY = decltype(ty);
+        if (!vec) return ln_bwd_go<TX, TY, 1, 8>(a, st, &nrows);
+        if (sizeof(TX) == 4) return ln_bwd_go<TX, TY, 4, 4>(a, st, &nrows);
+        return ln_bwd_go<TX, TY, 8, 2>(a, st, &nrows);
+    });
+    if (e != cudaSuccess || a.work == nullptr) return e;
+    return launch_pdl(nrows > 0, ln_cols_kernel, dim3((2 * a.C + 31) / 32), dim3(1024), 0, st,
+                      static_cast<const float*>(a.work), nrows, a.C, a.dw, a.db, a.w_type);
+}
+
+}  // namespace dn8
