@@ -298,11 +298,16 @@ template <typename A> static int check_attention(const A* a, const char* call) {
     if (a->type != DN8_F16 && a->type != DN8_BF16) return fail(DN8_EINVAL, "%s: type %d (16 bits)", call, a->type);
     if (a->left < -1 || a->right < -1 || a->sinks < 0 || a->left > (1 << 30) || a->right > (1 << 30))
         return fail(DN8_EINVAL, "%s: window left=%d right=%d sinks=%d", call, a->left, a->right, a->sinks);
-    if (!(a->scale > -1e30f && a->scale < 1e30f)) return fail(DN8_EINVAL, "%s: scale %g", call, a->scale);
+    if (!(a->scale > 0.0f && a->scale < 1e30f)) return fail(DN8_EINVAL, "%s: scale %g must be positive", call, a->scale);
     const int64_t strides[] = {a->q_stride_t, a->q_stride_h, a->k_stride_t, a->k_stride_h,
                                a->v_stride_t, a->v_stride_h, a->o_stride_t, a->o_stride_h};
     for (int64_t s : strides)
         if (s < 0 || s % 8 || s >= (1ll << 38)) return fail(DN8_EINVAL, "%s: strides must be multiples of 8 elements", call);
+    // (a zero stride would let rows or heads share memory: tensor maps cannot say so)
+    if ((a->Tq > 1 && a->q_stride_t == 0) || (a->Hq > 1 && a->q_stride_h == 0) ||
+        (a->Tk > 1 && (a->k_stride_t == 0 || a->v_stride_t == 0)) ||
+        (a->Hk > 1 && (a->k_stride_h == 0 || a->v_stride_h == 0)))
+        return fail(DN8_EINVAL, "%s: rows or heads of q, k or v share memory (stride 0)", call);
     if (a->Tq > 0 && a->B > 0 && (a->q == nullptr || a->out == nullptr || !aligned16(a->q) || !aligned16(a->out)))
         return fail(DN8_EINVAL, "%s: pointers must be non-null and 16-byte aligned", call);
     if (a->Tk > 0 && a->B > 0 && (a->k == nullptr || a->v == nullptr || !aligned16(a->k) || !aligned16(a->v)))

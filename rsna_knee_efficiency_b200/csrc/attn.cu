@@ -1,6 +1,6 @@
 // attn.cu -- attention over packed sequences with a sliding window, first tokens that stay visible and
 // a key mask; grouped heads.
-#include "attn_common.cuh"
+#include "attn_umma.cuh"
 
 namespace dn8 {
 
@@ -39,19 +39,6 @@ template <> DN8_DEV void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-DN8_DEV uint32_t pack2(__half, float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    uint32_t u;
-    memcpy(&u, &h, 4);
-    return u;
-}
-DN8_DEV uint32_t pack2(__nv_bfloat16, float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    uint32_t u;
-    memcpy(&u, &h, 4);
-    return u;
-}
-
 // Where a share's partial results are kept: [row block][key head][share] of (16 rows x (maximum, sum)) and
 // 16 x DP outputs, relative to the row's maximum (in units of log2).
 struct RowsPlan {
@@ -349,9 +336,14 @@ template <typename T, int DP> cudaError_t rows_go(const dn8_attention_args& a, R
 
 }  // namespace
 
-size_t attention_work(const dn8_attention_args& a, int sms) { return rows_work(a, rows_plan(a, sms)); }
+// Few rows per sequence and key head: the row kernel, which packs the heads of a group and splits the
+// key axis. Otherwise 128-row tiles on the tensor cores (attn_tile.cu).
+static bool few_rows(const dn8_attention_args& a) { return a.Tq * (a.Hq / a.Hk) <= 32ll * a.B; }
+
+size_t attention_work(const dn8_attention_args& a, int sms) { return few_rows(a) ? rows_work(a, rows_plan(a, sms)) : 0; }
 
 cudaError_t launch_attention(const dn8_attention_args& a, int sms, cudaStream_t st) {
+    if (!few_rows(a)) return launch_attention_tile(a, st);
     const RowsPlan p = rows_plan(a, sms);
     if (a.type == DN8_F16) return head_pad(a.D) == 64 ? rows_go<__half, 64>(a, p, st) : rows_go<__half, 128>(a, p, st);
     return head_pad(a.D) == 64 ? rows_go<__nv_bfloat16, 64>(a, p, st) : rows_go<__nv_bfloat16, 128>(a, p, st);

@@ -1,0 +1,126 @@
+// attn_umma.cuh -- tcgen05 kind::f16 pieces of the attention kernels: tiles of 128 rows x 64 or 128
+// elements in shared memory (blocks of 64 elements = 128-byte rows, 128-byte swizzle, as TMA writes
+// them), fp32 accumulators and 16-bit left operands in TMEM.
+#pragma once
+#include "attn_common.cuh"
+
+namespace dn8 {
+
+constexpr int AT_TILE = 128;                       // rows of a query or key tile
+constexpr uint32_t AT_BLOCK = AT_TILE * 128;       // bytes of a block: 128 rows x 64 elements
+
+DN8_DEV void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)) : "memory");
+}
+// A tile of DP elements: one box of 64 elements x 1 head x 128 rows per block.
+template <int DP> DN8_DEV void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+#pragma unroll
+    for (int b = 0; b < DP / 64; ++b) tma_load_3d(dst + b * AT_BLOCK, map, bar, b * 64, head, row);
+}
+
+constexpr uint32_t LAYOUT_SW128 = 2;
+// Rows along M or N, the 64-element blocks along K: K step kk (16 elements).
+DN8_DEV uint64_t desc_rows(uint32_t tile, int kk) {
+    return sdesc(tile + (kk >> 2) * AT_BLOCK + (kk & 3) * 32, 16, 1024, LAYOUT_SW128);
+}
+// Rows along K (16 rows per step, kk), elements along N.
+DN8_DEV uint64_t desc_cols(uint32_t tile, int kk) { return sdesc(tile + kk * 2048, AT_BLOCK, 1024, LAYOUT_SW128); }
+
+// Instruction descriptor of kind::f16: D fp32, A and B of type T; `bcols`: B's rows are along K.
+template <typename T> DN8_DEV constexpr uint32_t idesc_f16(int M, int N, bool bcols) {
+    const uint32_t t = sizeof(T) == 2 && !__is_same(T, __half) ? 1u : 0u;        // 1: bf16, 0: fp16
+    return (1u << 4) | (t << 7) | (t << 10) | (static_cast<uint32_t>(bcols) << 16) |
+           (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+// Issued by a whole converged warp (one elected lane).
+DN8_DEV void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, e;\n\t.reg .b32 l;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "elect.sync l|e, 0xffffffff;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// A from TMEM: 16 elements of a row in 8 columns, elements 2c and 2c + 1 in column c.
+DN8_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, e;\n\t.reg .b32 l;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "elect.sync l|e, 0xffffffff;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// D[128 x 128] = A B^T over DP elements, both tiles in shared memory
+template <typename T, int DP> DN8_DEV void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+        umma_f16_ss(d, desc_rows(a, kk), desc_rows(b, kk), idesc_f16<T>(AT_TILE, AT_TILE, false), kk > 0);
+}
+// D[128 x DP] (+)= A B, A [128 x 128] in TMEM (64 columns), B a tile of 128 rows
+template <typename T, int DP> DN8_DEV void mma_values(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+#pragma unroll
+    for (int kk = 0; kk < AT_TILE / 16; ++kk)
+        umma_f16_ts(d, a + 8 * kk, desc_cols(b, kk), idesc_f16<T>(AT_TILE, DP, true), accumulate || kk > 0);
+}
+
+// One row per thread: 16 packed words (32 elements of 16 bits) to columns taddr ..
+DN8_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+DN8_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
+}
+// (see tmem_wait_st(r) in dn8_common.cuh: the registers of a store stay alive until it has read them)
+DN8_DEV void tmem_wait_st(const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::st.sync.aligned;"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+DN8_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+DN8_DEV uint32_t pack2(__half, float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    uint32_t u;
+    memcpy(&u, &h, 4);
+    return u;
+}
+DN8_DEV uint32_t pack2(__nv_bfloat16, float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    uint32_t u;
+    memcpy(&u, &h, 4);
+    return u;
+}
+
+// Bits [lo, hi] of a row of 128, word w.
+DN8_DEV uint32_t bits_from(int lo, int w) {
+    const int k = lo - 32 * w;
+    return k <= 0 ? 0xFFFFFFFFu : k >= 32 ? 0u : 0xFFFFFFFFu << k;
+}
+DN8_DEV uint32_t bits_upto(int hi, int w) {
+    const int k = hi - 32 * w;
+    return k < 0 ? 0u : k >= 31 ? 0xFFFFFFFFu : (2u << k) - 1u;
+}
+
+// 3-D map over [rows][heads][D] with token / head strides (elements): box 64 elements x 1 head x 128 rows.
+// Elements behind D and rows behind the tensor arrive as zeros.
+cudaError_t make_head_map(CUtensorMap* map, const void* base, int type, int64_t rows, int heads, int D, int64_t stride_t,
+                          int64_t stride_h);
+
+}  // namespace dn8
