@@ -277,7 +277,8 @@ int dn8_rope(const dn8_rope_args* a, dn8_stream stream);
  * for the second product.
  * Offsets are checked on the device: a sequence that leaves [0, Tq] or [0, Tk], or a len_k outside its
  * slot, counts as empty and sets err. D a multiple of 8 up to 128; pointers 16-byte aligned, strides
- * multiples of 8 elements (not 0 where there are several rows or heads); scale > 0; type DN8_F16 or DN8_BF16. */
+ * multiples of 8 elements (not 0 where there are several rows or heads); scale > 0; type DN8_F16 or DN8_BF16; Tq and
+ * Tk below 2^28. */
 typedef struct dn8_attention_args {
     const void* q;          /* [Tq][Hq][D] */
     const void* k;          /* [Tk][Hk][D] */

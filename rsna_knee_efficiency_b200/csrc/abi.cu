@@ -289,14 +289,15 @@ int dn8_rope(const dn8_rope_args* a, dn8_stream stream) {
 // What both directions of attention have in common; `call` names the entry point in the message.
 template <typename A> static int check_attention(const A* a, const char* call) {
     if (a == nullptr) return fail(DN8_EINVAL, "%s: null arguments", call);
-    if (a->B < 0 || a->Tq < 0 || a->Tk < 0 || a->Tq >= (1ll << 30) || a->Tk >= (1ll << 30) || a->Hk < 1 || a->Hk > 65535 ||
+    if (a->B < 0 || a->Tq < 0 || a->Tk < 0 || a->Tq >= (1ll << 28) || a->Tk >= (1ll << 28) || a->Hk < 1 || a->Hk > 65535 ||
         a->Hq < 1 || a->Hq > 65535 || a->Hq % a->Hk)
         return fail(DN8_EINVAL, "%s: bad geometry B=%d Tq=%lld Tk=%lld Hq=%d Hk=%d", call, a->B,
                     static_cast<long long>(a->Tq), static_cast<long long>(a->Tk), a->Hq, a->Hk);
     if (a->Tq * (a->Hq / a->Hk) >= (1ll << 30)) return fail(DN8_EINVAL, "%s: Tq Hq / Hk exceeds 2^30", call);
     if (a->D < 8 || a->D > 128 || a->D % 8) return fail(DN8_EINVAL, "%s: head size %d (a multiple of 8 up to 128)", call, a->D);
     if (a->type != DN8_F16 && a->type != DN8_BF16) return fail(DN8_EINVAL, "%s: type %d (16 bits)", call, a->type);
-    if (a->left < -1 || a->right < -1 || a->sinks < 0 || a->left > (1 << 30) || a->right > (1 << 30))
+    if (a->left < -1 || a->right < -1 || a->sinks < 0 || a->left > (1 << 29) || a->right > (1 << 29) ||
+        a->sinks > (1 << 29))
         return fail(DN8_EINVAL, "%s: window left=%d right=%d sinks=%d", call, a->left, a->right, a->sinks);
     if (!(a->scale > 0.0f && a->scale < 1e30f)) return fail(DN8_EINVAL, "%s: scale %g must be positive", call, a->scale);
     const int64_t strides[] = {a->q_stride_t, a->q_stride_h, a->k_stride_t, a->k_stride_h,
@@ -355,9 +356,9 @@ int dn8_attention_bwd(const dn8_attention_bwd_args* a, dn8_stream stream) {
         return fail(DN8_EINVAL, "dn8_attention_bwd: pointers must be non-null and 16-byte aligned");
     if (a->Tk > 0 && (a->dk == nullptr || a->dv == nullptr || !aligned16(a->dk) || !aligned16(a->dv)))
         return fail(DN8_EINVAL, "dn8_attention_bwd: pointers must be non-null and 16-byte aligned");
-    int sms = 0;
-    if (int s = current_sms(&sms)) return s;
-    cudaError_t e = dn8::launch_attention_bwd(*a, sms, static_cast<cudaStream_t>(stream));
+    if ((a->Tq > 1 && a->do_stride_t == 0) || (a->Hq > 1 && a->do_stride_h == 0))
+        return fail(DN8_EINVAL, "dn8_attention_bwd: rows or heads of dout share memory (stride 0)");
+    cudaError_t e = dn8::launch_attention_bwd(*a, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_attention_bwd launch");
 }
 

@@ -11,7 +11,7 @@
 
 namespace dn8 {
 
-constexpr int ATT_FAR = 1 << 30;              // "no limit": beyond every length (checked < 2^30)
+constexpr int ATT_FAR = 1 << 29;              // "no limit": beyond every length (checked < 2^28; sums stay in 32 bits)
 constexpr float ATT_LOG2E = 1.4426950408889634f, ATT_LN2 = 0.6931471805599453f;
 
 struct Sequence {

@@ -255,7 +255,7 @@ def _attention_common(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right
     _flat(c, "keep", keep, Tk, (torch.bool, torch.uint8))
     _flat(c, "lse", lse, (Tq, Hq), (torch.float32,))
     _flat(c, "err", err, 1, (torch.int32,))
-    far = 1 << 30
+    far = 1 << 29                                        # beyond every length: no limit
     mask = (B, Hq, Hk, D, _TYPES[q.dtype], min(int(left), far), min(int(right), far), min(int(sinks), far),
             D ** -0.5 if scale is None else float(scale))
     strides = [*_head_strides(c, "q", q, (Tq, Hq, D), q.dtype), *_head_strides(c, "k", k, (Tk, Hk, D), q.dtype),

@@ -51,7 +51,7 @@ def _attention(cls=nat.AttentionArgs, **kw):
 
 
 @pytest.mark.parametrize("bad", [dict(D=0), dict(D=12), dict(D=136), dict(Hk=3), dict(Hk=0), dict(type=nat.DN8_F32), dict(B=-1),
-                                 dict(Tq=-1), dict(Tk=1 << 30), dict(left=-2), dict(right=-2), dict(sinks=-1),
+                                 dict(Tq=-1), dict(Tk=1 << 28), dict(left=(1 << 29) + 1), dict(left=-2), dict(right=-2), dict(sinks=-1),
                                  dict(scale=float("nan")), dict(scale=float("inf")), dict(q=4104), dict(k=None), dict(v=8),
                                  dict(q_stride_t=12), dict(scale=0.0), dict(scale=-1.0), dict(k_stride_h=0), dict(q_stride_t=0), dict(k_stride_h=-8), dict(cu_q=None)])
 def test_attention_refusals(bad):
