@@ -18,6 +18,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from .context import ContextHead
 from .encoder import Dense8SEncoder
 
 DEPTH = 3
@@ -107,10 +108,12 @@ class StudyRunner:
 
     def __init__(self, packs: list[dict], dev: int, studies: int, slices: int = 26,
                  flip_tta: bool = False, zoom: tuple | None = None, design: str = "parx",
-                 n_windows: int = 2) -> None:
+                 n_windows: int = 2, context: list[ContextHead] | None = None) -> None:
         """`zoom` = (scale, tx, ty): the geometric view of the reference's TTA (`affine_windows`,
         src/knee/tta.py:131-149; the submission's view is (1.10, 0, 0)): the windows are zoomed on the
-        device (`ops.zoom`) and encoded through the fp16 path instead of the stem's uint8 gather."""
+        device (`ops.zoom`) and encoded through the fp16 path instead of the stem's uint8 gather.
+        `context`: a `ContextHead` per seed, applied to the features of each study's windows in place of the
+        packs' linear head and slice mean (the packs need no head then)."""
         self.dev, self.studies, self.slices, self.flip_tta = dev, studies, slices, flip_tta
         self.design, self.n_windows = design, n_windows
         self.zoom = None if zoom is None or tuple(zoom) == (1.0, 0.0, 0.0) else tuple(float(z) for z in zoom)
@@ -126,10 +129,14 @@ class StudyRunner:
             self.n_img.append(len(src))
             self.per_view.append(len(src) // studies)
         self.encoders = [Dense8SEncoder(p, dev, n) for p, n in zip(packs, self.n_img)]
-        for e in self.encoders:
-            if e.n_head < 1:
-                raise ValueError("StudyRunner needs packs with a head (H_w, H_b)")
-        self.n_out = self.encoders[0].n_head
+        self.context = context
+        if context is None:
+            for e in self.encoders:
+                if e.n_head < 1:
+                    raise ValueError("StudyRunner needs packs with a head (H_w, H_b)")
+            self.n_out = self.encoders[0].n_head
+        else:
+            self.n_out = self._prepare_context(packs)
         self.logits = [torch.zeros((n, self.n_out), dtype=torch.float32, device=d) for n in self.n_img]
         self.views = [torch.zeros((studies, self.n_out), dtype=torch.float32, device=d) for _ in packs]
         self.out = torch.zeros((studies, self.n_out), dtype=torch.float32, device=d)
@@ -137,6 +144,26 @@ class StudyRunner:
         if self.zoom is not None:
             img = int(self.encoders[0].in_shape[2])
             self.zbuf = torch.empty((max(self.n_img), 3, img, img), dtype=torch.float16, device=d)
+
+    def _prepare_context(self, packs: list[dict]) -> int:
+        if len(self.context) != len(packs) or len({c.n_out for c in self.context}) != 1:
+            raise ValueError(f"{len(self.context)} context heads for {len(packs)} packs (one each, of one n_out)")
+        self.layouts, self.pos, self.slot = [], [], []
+        for k, (c, e) in enumerate(zip(self.context, self.encoders)):
+            if c.c != e.n_features:
+                raise ValueError(f"context head of {c.c} channels for {e.n_features} features")
+            c.to(self.device)
+            w = np.tile(self.windows[k], 2 if self.flip_tta else 1)      # a study's windows, then flipped
+            pos = np.stack([w // self.n_win, w % self.n_win], 1).astype(np.int32)
+            self.pos.append(torch.from_numpy(np.tile(pos, (self.studies, 1))).to(self.device))
+            self.slot.append(torch.from_numpy(pos[:, 0].astype(np.int64)).to(self.device))
+            self.layouts.append(c.layout([self.per_view[k]] * self.studies, self.device))
+        return self.context[0].n_out
+
+    @torch.no_grad()
+    def _context_logits(self, k: int, feats: torch.Tensor, present: torch.Tensor | None) -> None:
+        keep = None if present is None else present[:, self.slot[k]].reshape(-1)
+        self.views[k].copy_(self.context[k](feats, self.layouts[k], self.pos[k], keep))
 
     @property
     def images_per_call(self) -> int:
@@ -149,8 +176,13 @@ class StudyRunner:
         passes = sum(-(-n // e.nb) for n, e in zip(self.n_img, self.encoders))
         return per_pass * passes + (len(self.encoders) if self.zoom is not None else 0)
 
-    def run(self, volumes: torch.Tensor) -> torch.Tensor:
-        """Study logits [studies, n_out] (the mean over seeds of each seed's view mean)."""
+    def run(self, volumes: torch.Tensor, present: torch.Tensor | None = None) -> torch.Tensor:
+        """Study logits [studies, n_out] (the mean over seeds of each seed's view mean, or of its context
+        head's logits). `present` (context heads only): bool [studies, n_windows], False for the
+        crop windows that a study lacks; their volumes are encoded but not attended to."""
+        if present is not None and (self.context is None or tuple(present.shape) != (self.studies, self.n_windows)
+                                    or present.dtype != torch.bool):
+            raise ValueError(f"present: bool [{self.studies}, {self.n_windows}] for a runner with context heads")
         if (volumes.dim() != 5 or volumes.shape[0] != self.n_windows or volumes.shape[1] != self.studies
                 or volumes.shape[2] != self.slices or volumes.dtype != torch.uint8):
             raise ValueError(f"volumes {tuple(volumes.shape)} {volumes.dtype}: expected uint8 "
@@ -164,7 +196,12 @@ class StudyRunner:
             for enc in self.encoders:
                 enc.stream.wait_stream(cur)
             for k, enc in enumerate(self.encoders):
-                enc.enqueue_u8(planes, self.src[k], self.flags[k], self.logits[k], self.views[k], self.per_view[k])
+                if self.context is None:
+                    enc.enqueue_u8(planes, self.src[k], self.flags[k], self.logits[k], self.views[k], self.per_view[k])
+                    continue
+                feats = enc.enqueue_u8(planes, self.src[k], self.flags[k])
+                with torch.cuda.stream(enc.stream):
+                    self._context_logits(k, feats, present)
             for enc in self.encoders:
                 cur.wait_stream(enc.stream)
         else:
@@ -174,7 +211,10 @@ class StudyRunner:
             for k, enc in enumerate(self.encoders):
                 zb = self.zbuf[:self.n_img[k]]
                 ops.zoom(planes, self.src[k], zb, self.n_img[k], h, w, *self.zoom, flags=self.flags[k])
-                enc.encode(zb, self.logits[k], self.views[k], self.per_view[k])
+                if self.context is None:
+                    enc.encode(zb, self.logits[k], self.views[k], self.per_view[k])
+                else:
+                    self._context_logits(k, enc.encode(zb), present)
         torch.mean(torch.stack(self.views), 0, out=self.out)
         return self.out
 
