@@ -88,53 +88,102 @@ def head_noalloc(in0: torch.Tensor, seg: torch.Tensor, fab: torch.Tensor, G0: in
 # --- the context transformer's operators -----------------------------------------------------
 # Tensors of one call live on one GPU, which need not be the current one; the work goes to `stream`
 # (default: that GPU's current stream), and so does a workspace that the call allocates.
+# The checks below read each tensor property once and build no message unless they fail: a small call is
+# over in 3 us on the GPU.
 _TYPES = {torch.float32: nat.DN8_F32, torch.float16: nat.DN8_F16, torch.bfloat16: nat.DN8_BF16}
+_ANY = tuple(_TYPES)
+_HALF = (torch.float16, torch.bfloat16)
+_F32, _I32, _U8, _FLAG = (torch.float32,), (torch.int32,), (torch.uint8,), (torch.bool, torch.uint8)
 
 
-def _need(cond: bool, what: str) -> None:
-    if not cond:
-        raise ValueError(what)
+def _refuse(call: str, name: str, t, shape, types, dev, what: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{call}: {name} must be a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{call}: {name} is not on a GPU")
+    raise ValueError(f"{call}: {name} {tuple(t.shape)} {t.dtype} on {t.device}: expected {tuple(shape)} of "
+                     f"{', '.join(str(x) for x in types)} on {dev}, {what}")
 
 
-def _on_gpu(call: str, stream, first: torch.Tensor, **tensors):
-    """The device and the stream of a call whose tensors are `first` and `tensors` (None: absent)."""
-    for name, t in tensors.items():
-        if t is not None:
-            _need(isinstance(t, torch.Tensor), f"{call}: {name} must be a tensor")
-    _need(first.is_cuda, f"{call}: tensors on a GPU expected")
-    for name, t in tensors.items():
-        _need(t is None or t.device == first.device, f"{call}: {name} is not on {first.device}")
-    s = stream if stream is not None else torch.cuda.current_stream(first.device)
-    _need(s.device == first.device, f"{call}: the stream is not of {first.device}")
-    return first.device, s
+def _gpu(call: str, t, dims: int, types, what: str) -> torch.device:
+    """The device of a call's first tensor."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims or t.dtype not in types:
+        raise ValueError(f"{call}: {what} expected")
+    if not t.is_cuda:
+        raise ValueError(f"{call}: tensors on a GPU expected")
+    return t.device
 
 
-def _rows(call: str, name: str, t: torch.Tensor | None, shape, types) -> int:
+def _rows(call: str, name: str, t, shape, types, dev, out: bool = False) -> int:
     """Elements between the rows of a matrix with contiguous rows."""
-    if t is None:
-        return 0
-    _need(tuple(t.shape) == tuple(shape), f"{call}: {name} {tuple(t.shape)}, expected {tuple(shape)}")
-    _need(t.dtype in types, f"{call}: {name} is {t.dtype}")
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{call}: the rows of {name} must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype not in types or t.device != dev:
+        _refuse(call, name, t, shape, types, dev, "rows contiguous")
+    st, last = t.stride()
+    if (last != 1 and shape[1] > 1) or (out and st == 0 and shape[0] > 1):
+        _refuse(call, name, t, shape, types, dev, "rows contiguous, an output's of their own memory")
+    return st if shape[0] > 1 else shape[1]
 
 
-def _flat(call: str, name: str, t: torch.Tensor | None, n, types) -> None:
-    shape = n if isinstance(n, tuple) else (n,)
-    _need(t is None or (tuple(t.shape) == shape and t.dtype in types and t.is_contiguous()),
-          f"{call}: {name} must be contiguous {shape} of {', '.join(str(x) for x in types)}")
+def _flat(call: str, name: str, t, shape, types, dev) -> None:
+    if t is not None and (not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype not in types or t.device != dev
+                          or not t.is_contiguous()):
+        _refuse(call, name, t, shape, types, dev, "contiguous")
 
 
-def _writable(call: str, **tensors) -> None:
-    """Outputs whose elements share memory (an expanded tensor) cannot be written."""
-    for name, t in tensors.items():
-        _need(t is None or all(st > 0 or n <= 1 for st, n in zip(t.stride(), t.shape)),
-              f"{call}: {name} has elements that share memory")
+def _heads(call: str, name: str, t, shape, types, dev, out: bool = False) -> tuple:
+    """Elements between tokens and between heads of a [T, H, D] tensor (0 where there is only one)."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype not in types or t.device != dev:
+        _refuse(call, name, t, shape, types, dev, "last dimension contiguous")
+    st, sh, last = t.stride()
+    if shape[0] <= 1:
+        st = 0
+    elif out and st == 0:
+        _refuse(call, name, t, shape, types, dev, "no two tokens the same memory")
+    if shape[1] <= 1:
+        sh = 0
+    elif out and sh == 0:
+        _refuse(call, name, t, shape, types, dev, "no two heads the same memory")
+    if last != 1 and shape[2] > 1:
+        _refuse(call, name, t, shape, types, dev, "last dimension contiguous")
+    return st, sh
 
 
-def _work(nbytes: int, device, stream) -> torch.Tensor:
+def _launch(what: str, fn, a, dev: torch.device, stream) -> None:
+    """Calls `fn(a, stream)` with the tensors' device current."""
+    if stream is None:
+        s = torch.cuda.current_stream(dev).cuda_stream
+    else:
+        if stream.device != dev:
+            raise ValueError(f"{what}: the stream is not of {dev}")
+        s = stream.cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        status = fn(a, s)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(a, s)
+    if status:
+        nat.check(status, what)
+
+
+def _bytes_of(fn, a, dev: torch.device) -> int:
+    """Workspace bytes of a call on `dev` (they depend on its SM count); -1: the call will be refused."""
+    if torch.cuda.current_device() == dev.index:
+        return fn(a)
+    with torch.cuda.device(dev):
+        return fn(a)
+
+
+def _workspace(what: str, nbytes: int, work, dev, stream):
+    """`work`, checked, or a new workspace that belongs to the call's stream."""
+    if work is not None:
+        if not (isinstance(work, torch.Tensor) and work.dtype == torch.uint8 and work.device == dev
+                and work.is_contiguous() and work.numel() >= nbytes and work.data_ptr() % 16 == 0):
+            raise ValueError(f"{what}: work needs {nbytes} contiguous bytes (uint8, 16-byte aligned) on {dev}")
+        return work
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, out: torch.Tensor,
@@ -146,24 +195,27 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
     type, or None. `mean` / `rstd` [M] fp32 keep the statistics for the backward pass. `out` and
     `sum` may be x or res themselves where types and strides agree."""
     c = "layer_norm"
-    _need(x.dim() == 2 and x.dtype in _TYPES and x.shape[1] > 0, f"{c}: x [M, C] of fp32, fp16 or bf16 expected")
-    dev, s = _on_gpu(c, stream, x, weight=weight, bias=bias, out=out, res=res, sum=sum, mean=mean, rstd=rstd)
-    M, C = x.shape
-    same = (x.dtype,)
-    outs = tuple(_TYPES) if x.dtype == torch.float32 else same
-    _need((res is None) == (sum is None), f"{c}: res and sum come together")
-    strides = [_rows(c, "x", x, (M, C), same), _rows(c, "res", res, (M, C), same), _rows(c, "out", out, (M, C), outs),
-               _rows(c, "sum", sum, (M, C), same)]
-    wt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-    for name, t in (("weight", weight), ("bias", bias)):
-        _flat(c, name, t, C, (wt,) if wt in _TYPES else tuple(_TYPES))
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _flat(c, name, t, M, (torch.float32,))
-    _writable(c, out=out, sum=sum)
+    dev = _gpu(c, x, 2, _ANY, "x [M, C] of fp32, fp16 or bf16")
+    shape = M, C = x.shape
+    t = x.dtype
+    same = (t,)
+    if (res is None) != (sum is None):
+        raise ValueError(f"{c}: res and sum come together")
+    xs = _rows(c, "x", x, shape, same, dev)
+    ys = _rows(c, "out", out, shape, _ANY if t is torch.float32 else same, dev, True)
+    rs = ss = 0
+    if res is not None:
+        rs, ss = _rows(c, "res", res, shape, same, dev), _rows(c, "sum", sum, shape, same, dev, True)
+    wt = (weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32)
+    _flat(c, "weight", weight, (C,), _ANY, dev)
+    _flat(c, "bias", bias, (C,), (wt,), dev)
+    _flat(c, "mean", mean, (M,), _F32, dev)
+    _flat(c, "rstd", rstd, (M,), _F32, dev)
+    if wt not in _TYPES:
+        _refuse(c, "bias", bias, (C,), _ANY, dev, "contiguous")
     a = nat.LayerNormArgs(_ptr(x), _ptr(res), _ptr(weight), _ptr(bias), _ptr(out), _ptr(sum), _ptr(mean), _ptr(rstd),
-                          M, *strides, C, _TYPES[x.dtype], _TYPES[out.dtype], _TYPES[wt], eps)
-    with torch.cuda.device(dev):
-        nat.check(nat.lib().dn8_layer_norm(a, s.cuda_stream), "dn8_layer_norm")
+                          M, xs, rs, ys, ss, C, _TYPES[t], _TYPES[out.dtype], _TYPES[wt], eps)
+    _launch("dn8_layer_norm", nat.lib().dn8_layer_norm, a, dev, stream)
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, mean: torch.Tensor,
@@ -174,43 +226,31 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     gradient of its output (the output's type), dsum the gradient that reaches the sum past the
     norm. dx (x's type) is the gradient of x and of the residual alike; dweight / dbias [C] of the
     weight's type (fp32 without a weight) are sums over the rows, the same bits every call. dx may be
-    dy, x or dsum itself. `work`: uint8 of `dn8_layer_norm_bwd_work(C)` bytes, allocated if not given."""
+    dy, x or dsum itself where types and strides agree. `work`: uint8 of `dn8_layer_norm_bwd_work(C)`
+    bytes, allocated if not given."""
     c = "layer_norm_backward"
-    _need(x.dim() == 2 and x.dtype in _TYPES and x.shape[1] > 0, f"{c}: x [M, C] of fp32, fp16 or bf16 expected")
-    dev, s = _on_gpu(c, stream, x, dy=dy, weight=weight, mean=mean, rstd=rstd, dx=dx, dweight=dweight, dbias=dbias,
-                     dsum=dsum, work=work)
-    M, C = x.shape
-    same = (x.dtype,)
-    outs = tuple(_TYPES) if x.dtype == torch.float32 else same
-    strides = [_rows(c, "dy", dy, (M, C), outs), _rows(c, "x", x, (M, C), same), _rows(c, "dsum", dsum, (M, C), same),
-               _rows(c, "dx", dx, (M, C), same)]
-    wt = weight.dtype if weight is not None else torch.float32
-    for name, t in (("weight", weight), ("dweight", dweight), ("dbias", dbias)):
-        _flat(c, name, t, C, (wt,) if wt in _TYPES else tuple(_TYPES))
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _need(t is not None, f"{c}: {name} is needed")
-        _flat(c, name, t, M, (torch.float32,))
-    _writable(c, dx=dx)
-    with torch.cuda.device(dev):
-        nbytes = nat.lib().dn8_layer_norm_bwd_work(C) if dweight is not None or dbias is not None else 0
-        if work is None and nbytes:
-            work = _work(nbytes, dev, s)
-        _need(nbytes == 0 or (work.dtype == torch.uint8 and work.is_contiguous() and work.numel() >= nbytes
-                              and work.data_ptr() % 16 == 0), f"{c}: work needs {nbytes} contiguous bytes (uint8)")
-        a = nat.LayerNormBwdArgs(_ptr(dy), _ptr(x), _ptr(weight), _ptr(dsum), _ptr(mean), _ptr(rstd), _ptr(dx),
-                                 _ptr(dweight), _ptr(dbias), _ptr(work), M, *strides, C, _TYPES[x.dtype],
-                                 _TYPES[dy.dtype], _TYPES[wt])
-        nat.check(nat.lib().dn8_layer_norm_bwd(a, s.cuda_stream), "dn8_layer_norm_bwd")
-
-
-def _head_strides(call: str, name: str, t: torch.Tensor | None, shape, dtype) -> list:
-    """Elements between tokens and between heads of a [T, H, D] tensor (0 where there is only one)."""
-    if t is None:
-        return [0, 0]
-    _need(tuple(t.shape) == tuple(shape), f"{call}: {name} {tuple(t.shape)}, expected {tuple(shape)}")
-    _need(t.dtype == dtype, f"{call}: {name} is {t.dtype}, expected {dtype}")
-    _need(t.stride(2) == 1, f"{call}: the last dimension of {name} must be contiguous")
-    return [t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0]
+    dev = _gpu(c, x, 2, _ANY, "x [M, C] of fp32, fp16 or bf16")
+    shape = M, C = x.shape
+    t = x.dtype
+    same = (t,)
+    xs, gs = _rows(c, "x", x, shape, same, dev), _rows(c, "dy", dy, shape, _ANY if t is torch.float32 else same, dev)
+    ds = 0 if dsum is None else _rows(c, "dsum", dsum, shape, same, dev)
+    os = _rows(c, "dx", dx, shape, same, dev, True)
+    wt = torch.float32 if weight is None else weight.dtype
+    _flat(c, "weight", weight, (C,), _ANY, dev)
+    _flat(c, "dweight", dweight, (C,), (wt,), dev)
+    _flat(c, "dbias", dbias, (C,), (wt,), dev)
+    if mean is None or rstd is None:
+        raise ValueError(f"{c}: mean and rstd are needed")
+    _flat(c, "mean", mean, (M,), _F32, dev)
+    _flat(c, "rstd", rstd, (M,), _F32, dev)
+    lib = nat.lib()
+    if dweight is not None or dbias is not None:
+        work = _workspace(c, lib.dn8_layer_norm_bwd_work(C), work, dev, stream)
+    a = nat.LayerNormBwdArgs(_ptr(dy), _ptr(x), _ptr(weight), _ptr(dsum), _ptr(mean), _ptr(rstd), _ptr(dx),
+                             _ptr(dweight), _ptr(dbias), _ptr(work), M, gs, xs, ds, os, C, _TYPES[t],
+                             _TYPES[dy.dtype], _TYPES[wt])
+    _launch("dn8_layer_norm_bwd", lib.dn8_layer_norm_bwd, a, dev, stream)
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, q_out: torch.Tensor, k_out: torch.Tensor | None,
@@ -223,56 +263,51 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, q_out: torc
     over all pairs, or one ladder base^(-i / sections[x]) per axis. `inverse` turns back: the
     backward pass. q_out / k_out may be q / k themselves."""
     c = "rope"
-    _need(q.dim() == 3 and q.dtype in _TYPES, f"{c}: q [T, H, D] of fp32, fp16 or bf16 expected")
-    _need((k is None) == (k_out is None), f"{c}: k and k_out come together")
-    dev, s = _on_gpu(c, stream, q, k=k, pos=pos, q_out=q_out, k_out=k_out)
-    T, Hq, D = q.shape
-    _need(k is None or k.dim() == 3, f"{c}: k [T, H, D] expected")
-    Hk = 0 if k is None else k.shape[1]
-    sections = [int(n) for n in sections]
-    _need(1 <= len(sections) <= nat.DN8_ROPE_AXES, f"{c}: 1 to {nat.DN8_ROPE_AXES} axes")
-    _flat(c, "pos", pos, (T, len(sections)), (torch.int32,))
-    _writable(c, q_out=q_out, k_out=k_out)
-    a = nat.RopeArgs(_ptr(q), _ptr(k), _ptr(pos), _ptr(q_out), _ptr(k_out), T,
-                     *_head_strides(c, "q", q, (T, Hq, D), q.dtype), *_head_strides(c, "k", k, (T, Hk, D), q.dtype),
-                     *_head_strides(c, "q_out", q_out, (T, Hq, D), q.dtype),
-                     *_head_strides(c, "k_out", k_out, (T, Hk, D), q.dtype), Hq, Hk, D, _TYPES[q.dtype], len(sections),
-                     (nat.I32 * nat.DN8_ROPE_AXES)(*sections), int(bool(per_axis)), int(bool(interleaved)),
-                     int(bool(inverse)), base)
-    with torch.cuda.device(dev):
-        nat.check(nat.lib().dn8_rope(a, s.cuda_stream), "dn8_rope")
+    dev = _gpu(c, q, 3, _ANY, "q [T, H, D] of fp32, fp16 or bf16")
+    shape = T, Hq, D = q.shape
+    t = (q.dtype,)
+    axes = len(sections)
+    if not 1 <= axes <= nat.DN8_ROPE_AXES:
+        raise ValueError(f"{c}: 1 to {nat.DN8_ROPE_AXES} axes")
+    _flat(c, "pos", pos, (T, axes), _I32, dev)
+    if pos is None or (k is None) != (k_out is None):
+        raise ValueError(f"{c}: pos is needed, and k and k_out come together")
+    qs, qo = _heads(c, "q", q, shape, t, dev), _heads(c, "q_out", q_out, shape, t, dev, True)
+    Hk, ks, ko = 0, (0, 0), (0, 0)
+    if k is not None:
+        if not isinstance(k, torch.Tensor) or k.dim() != 3:
+            raise ValueError(f"{c}: k [T, H, D] expected")
+        Hk = k.shape[1]
+        ks, ko = _heads(c, "k", k, (T, Hk, D), t, dev), _heads(c, "k_out", k_out, (T, Hk, D), t, dev, True)
+    a = nat.RopeArgs(_ptr(q), _ptr(k), _ptr(pos), _ptr(q_out), _ptr(k_out), T, *qs, *ks, *qo, *ko, Hq, Hk, D,
+                     _TYPES[q.dtype], axes, (nat.I32 * nat.DN8_ROPE_AXES)(*sections), per_axis, interleaved, inverse,
+                     base)
+    _launch("dn8_rope", nat.lib().dn8_rope, a, dev, stream)
 
 
-def _attention_common(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale):
-    _need(q.dim() == 3 and k.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16),
-          f"{c}: q [Tq, Hq, D], k [Tk, Hk, D] of fp16 or bf16 expected")
-    Tq, Hq, D = q.shape
-    Tk, Hk, _ = k.shape
-    _need(cu_q.dim() == 1 and cu_q.numel() >= 1, f"{c}: cu_q int32 [B + 1] expected")
-    B = cu_q.numel() - 1
-    for name, t, n in (("cu_q", cu_q, B + 1), ("cu_k", cu_k, B + 1), ("len_k", len_k, B)):
-        _flat(c, name, t, n, (torch.int32,))
-    _flat(c, "keep", keep, Tk, (torch.bool, torch.uint8))
-    _flat(c, "lse", lse, (Tq, Hq), (torch.float32,))
-    _flat(c, "err", err, 1, (torch.int32,))
-    far = 1 << 29                                        # beyond every length: no limit
-    mask = (B, Hq, Hk, D, _TYPES[q.dtype], min(int(left), far), min(int(right), far), min(int(sinks), far),
-            D ** -0.5 if scale is None else float(scale))
-    strides = [*_head_strides(c, "q", q, (Tq, Hq, D), q.dtype), *_head_strides(c, "k", k, (Tk, Hk, D), q.dtype),
-               *_head_strides(c, "v", v, (Tk, Hk, D), q.dtype)]
-    return Tq, Tk, strides, mask
+_FAR = 1 << 29                                               # beyond every length: no limit
 
 
-def _attention_work(c: str, size, a, work, dev, s):
-    nbytes = size(a)
-    if nbytes < 0:
-        nat.check(nat.DN8_EINVAL, c)
-    if work is None and nbytes:
-        work = _work(nbytes, dev, s)
-    _need(nbytes == 0 or (work.dtype == torch.uint8 and work.is_contiguous() and work.numel() >= nbytes),
-          f"{c}: work needs {nbytes} contiguous bytes (uint8)")
-    a.work = _ptr(work)
-    return work
+def _packed(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale):
+    """(device, shapes, head strides of q, k, v, mask fields) of an attention call."""
+    dev = _gpu(c, q, 3, _HALF, "q [Tq, Hq, D], k [Tk, Hk, D] of fp16 or bf16")
+    if not isinstance(k, torch.Tensor) or k.dim() != 3 or not isinstance(cu_q, torch.Tensor) or cu_q.dim() != 1:
+        raise ValueError(f"{c}: k [Tk, Hk, D] and cu_q int32 [B + 1] expected")
+    sq, sk = q.shape, k.shape
+    t = (q.dtype,)
+    n = cu_q.shape[0]
+    if n < 1 or cu_k is None or sk[2] != sq[2]:
+        raise ValueError(f"{c}: cu_q and cu_k int32 [B + 1], q and k of one head size expected")
+    _flat(c, "cu_q", cu_q, (n,), _I32, dev)
+    _flat(c, "cu_k", cu_k, (n,), _I32, dev)
+    _flat(c, "len_k", len_k, (n - 1,), _I32, dev)
+    _flat(c, "keep", keep, sk[:1], _FLAG, dev)
+    _flat(c, "lse", lse, sq[:2], _F32, dev)
+    _flat(c, "err", err, (1,), _I32, dev)
+    strides = (*_heads(c, "q", q, sq, t, dev), *_heads(c, "k", k, sk, t, dev), *_heads(c, "v", v, sk, t, dev))
+    mask = (n - 1, sq[1], sk[1], sq[2], _TYPES[q.dtype], min(left, _FAR), min(right, _FAR), min(sinks, _FAR),
+            sq[2] ** -0.5 if scale is None else scale)
+    return dev, sq, sk, t, strides, mask
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor,
@@ -291,16 +326,16 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tens
     counts as empty and sets `err` (int32 [1]). `work`: uint8 of `dn8_attention_work` bytes,
     allocated if needed and not given."""
     c = "attention"
-    dev, s = _on_gpu(c, stream, q, k=k, v=v, out=out, cu_q=cu_q, cu_k=cu_k, keep=keep, len_k=len_k, lse=lse, err=err,
-                     work=work)
-    Tq, Tk, strides, mask = _attention_common(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale)
-    strides += _head_strides(c, "out", out, q.shape, q.dtype)
-    _writable(c, out=out, lse=lse)
+    dev, sq, sk, t, strides, mask = _packed(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale)
+    os = _heads(c, "out", out, sq, t, dev, True)
     a = nat.AttentionArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cu_q), _ptr(cu_k), _ptr(len_k),
-                          _ptr(keep), _ptr(err), None, Tq, Tk, *strides, *mask)
-    with torch.cuda.device(dev):
-        work = _attention_work("dn8_attention", nat.lib().dn8_attention_work, a, work, dev, s)
-        nat.check(nat.lib().dn8_attention(a, s.cuda_stream), "dn8_attention")
+                          _ptr(keep), _ptr(err), None, sq[0], sk[0], *strides, *os, *mask)
+    lib = nat.lib()
+    nbytes = _bytes_of(lib.dn8_attention_work, a, dev)
+    if nbytes > 0:
+        work = _workspace(c, nbytes, work, dev, stream)
+        a.work = work.data_ptr()
+    _launch("dn8_attention", lib.dn8_attention, a, dev, stream)
 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
@@ -311,21 +346,24 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     """The gradient of `attention` from its inputs, its `out` and `lse` and the gradient `dout` of out:
     dq [Tq, Hq, D], dk and dv [Tk, Hk, D] (summed over the query heads that share a key head), all
     of the inputs' type and with strides of their own. The same bits every call (no atomics). Rows of
-    no sequence are left as they are."""
+    no sequence are left as they are. `work`: uint8 of `dn8_attention_bwd_work` bytes, allocated if not
+    given."""
     c = "attention_backward"
-    dev, s = _on_gpu(c, stream, q, dout=dout, k=k, v=v, out=out, lse=lse, dq=dq, dk=dk, dv=dv, cu_q=cu_q, cu_k=cu_k,
-                     keep=keep, len_k=len_k, err=err, work=work)
-    _need(lse is not None, f"{c}: lse is needed")
-    Tq, Tk, strides, mask = _attention_common(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale)
-    strides = _head_strides(c, "dout", dout, q.shape, q.dtype) + strides
-    for name, t, like in (("out", out, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, k)):
-        strides += _head_strides(c, name, t, like.shape, q.dtype)
-    _writable(c, dq=dq, dk=dk, dv=dv)
+    if lse is None:
+        raise ValueError(f"{c}: lse is needed")
+    dev, sq, sk, t, strides, mask = _packed(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale)
+    gs, os = _heads(c, "dout", dout, sq, t, dev), _heads(c, "out", out, sq, t, dev)
+    outs = (*_heads(c, "dq", dq, sq, t, dev, True), *_heads(c, "dk", dk, sk, t, dev, True),
+            *_heads(c, "dv", dv, sk, t, dev, True))
     a = nat.AttentionBwdArgs(_ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
-                             _ptr(cu_q), _ptr(cu_k), _ptr(len_k), _ptr(keep), _ptr(err), None, Tq, Tk, *strides, *mask)
-    with torch.cuda.device(dev):
-        work = _attention_work("dn8_attention_bwd", nat.lib().dn8_attention_bwd_work, a, work, dev, s)
-        nat.check(nat.lib().dn8_attention_bwd(a, s.cuda_stream), "dn8_attention_bwd")
+                             _ptr(cu_q), _ptr(cu_k), _ptr(len_k), _ptr(keep), _ptr(err), None, sq[0], sk[0], *gs,
+                             *strides, *os, *outs, *mask)
+    lib = nat.lib()
+    nbytes = lib.dn8_attention_bwd_work(a)
+    if nbytes > 0:
+        work = _workspace(c, nbytes, work, dev, stream)
+        a.work = work.data_ptr()
+    _launch("dn8_attention_bwd", lib.dn8_attention_bwd, a, dev, stream)
 
 
 # --- weight preparation (numpy in, numpy out) ----------------------------------------------
