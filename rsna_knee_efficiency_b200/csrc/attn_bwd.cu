@@ -74,15 +74,6 @@ struct BwdWalk {
     KeyTiles keys;           // dq: key tiles
 };
 
-// [128 x DP] += A B with A's 128 columns as two halves of 32 TMEM columns, at 0 and at 64 (each half
-// lies over the part of S that the same threads have read)
-template <typename T, int DP> DN8_DEV void mma_values_split(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
-#pragma unroll
-    for (int kk = 0; kk < AT_TILE / 16; ++kk)
-        umma_f16_ts(d, a + 8 * kk + (kk >= 4 ? 32 : 0), desc_cols(b, kk), idesc_f16<T>(AT_TILE, DP, true),
-                    accumulate || kk > 0);
-}
-
 // The 8 row warps: warp w has the TMEM lanes (resident rows) 32 (w % 4) .. and the columns 64 (w / 4) .. of
 // every step.
 template <typename T, int DP, bool KV>
@@ -418,7 +409,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             ok = mbar_wait_w(&sh.pready, u & 1, a.err, abort_flag, ERR_WAIT_ACC | (89 << 4));
             if (!ok) break;
             tc_fence_after();
-            if (kv) mma_values_split<T, DP>(tmem + C::ACC0, tmem + C::S, x0 + C::TILE, u > 0);
+            if (kv) mma_values<T, DP>(tmem + C::ACC0, tmem + C::S, x0 + C::TILE, u > 0);
             if (u + 1 < wk.steps) {
                 ok = wait_x(u + 1);
                 if (!ok) break;
@@ -429,7 +420,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             ok = mbar_wait_w(&sh.dsready, u & 1, a.err, abort_flag, ERR_WAIT_ACC | (90 << 4));
             if (!ok) break;
             tc_fence_after();
-            mma_values_split<T, DP>(tmem + (kv ? C::ACC1 : C::ACC0), tmem + C::DPC, x0, u > 0);
+            mma_values<T, DP>(tmem + (kv ? C::ACC1 : C::ACC0), tmem + C::DPC, x0, u > 0);
             umma_commit_w(&sh.xempty[u % C::ST]);
             if (u + 1 < wk.steps) {
                 mma_scores<T, DP>(tmem + C::DPC, r1, xn + C::TILE);

@@ -28,44 +28,50 @@ DN8_DEV int checked_len(int s, int e, int64_t T, int* err) {
     if (err != nullptr) atomicCAS(err, 0, ERR_SHAPE);
     return 0;
 }
-template <typename A> DN8_DEV int keys_of(const A& a, int b) {
-    const int s = a.cu_k[b], full = checked_len(s, a.cu_k[b + 1], a.Tk, a.err);
-    if (a.len_k == nullptr) return full;
-    return checked_len(0, a.len_k[b], full, a.err);
-}
-
 // Block `unit` of the batch when every sequence is cut into ceil(len mul / per) blocks, len being its
 // queries (KEYS = false) or its keys. Called by one whole warp.
 template <bool KEYS, typename A> DN8_DEV Sequence find_block(const A& a, int unit, int mul, int per) {
+    constexpr int BATCH = 4;                  // 32 sequences each, their offsets loaded together
     const int lane = threadIdx.x & 31;
     int run = 0;
     Sequence s;
     s.b = -1;
-    for (int base = 0; base < a.B; base += 32) {
-        const int b = base + lane;
-        int n = 0;
-        if (b < a.B) n = KEYS ? keys_of(a, b) : checked_len(a.cu_q[b], a.cu_q[b + 1], a.Tq, a.err);
-        const int mine = static_cast<int>((static_cast<int64_t>(n) * mul + per - 1) / per);
-        int incl = mine;
+    for (int base = 0; base < a.B && s.b < 0; base += 32 * BATCH) {
+        int q0[BATCH], q1[BATCH], k0[BATCH], k1[BATCH], kn[BATCH];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
+        for (int x = 0; x < BATCH; ++x) {
+            const int b = base + 32 * x + lane;
+            const bool in = b < a.B;
+            q0[x] = in ? a.cu_q[b] : 0;
+            q1[x] = in ? a.cu_q[b + 1] : 0;
+            k0[x] = in ? a.cu_k[b] : 0;
+            k1[x] = in ? a.cu_k[b + 1] : 0;
+            kn[x] = in && a.len_k != nullptr ? a.len_k[b] : 0;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, unit < run + incl);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            s.b = base + src;
-            s.blk = unit - run - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src));
-            break;
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+            const int nq = checked_len(q0[x], q1[x], a.Tq, a.err);
+            int nk = checked_len(k0[x], k1[x], a.Tk, a.err);
+            if (a.len_k != nullptr) nk = checked_len(0, kn[x], nk, a.err);
+            const int mine = static_cast<int>((static_cast<int64_t>(KEYS ? nk : nq) * mul + per - 1) / per);
+            int incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, unit < run + incl);
+            if (s.b < 0 && hit) {
+                const int src = __ffs(hit) - 1;
+                s.b = base + 32 * x + src;
+                s.blk = unit - run - __shfl_sync(0xffffffffu, incl - mine, src);
+                s.q0 = __shfl_sync(0xffffffffu, q0[x], src);
+                s.nq = __shfl_sync(0xffffffffu, nq, src);
+                s.k0 = __shfl_sync(0xffffffffu, k0[x], src);
+                s.nk = __shfl_sync(0xffffffffu, nk, src);
+            }
+            run += __shfl_sync(0xffffffffu, incl, 31);
         }
-        run += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (s.b >= 0) {
-        s.q0 = a.cu_q[s.b];
-        s.nq = checked_len(s.q0, a.cu_q[s.b + 1], a.Tq, a.err);
-        s.k0 = a.cu_k[s.b];
-        s.nk = keys_of(a, s.b);
     }
     return s;
 }

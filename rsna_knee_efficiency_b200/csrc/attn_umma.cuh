@@ -35,33 +35,56 @@ template <typename T> DN8_DEV constexpr uint32_t idesc_f16(int M, int N, bool bc
     return (1u << 4) | (t << 7) | (t << 10) | (static_cast<uint32_t>(bcols) << 16) |
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
-// Issued by a whole converged warp (one elected lane).
-DN8_DEV void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, e;\n\t.reg .b32 l;\n\t"
+// ---- issue ------------------------------------------------------------------------------------
+// An MMA takes its descriptors and addresses from uniform registers. Where the compiler cannot see that a
+// value is the same in the whole warp, it moves it there for every MMA (measured: 80 clocks per MMA, more
+// than the MMA's own time). So the issuing warp makes its values uniform once (`uniform`, a reduction whose
+// result lives in a uniform register), keeps its control flow uniform (conditions that come from a `vote`),
+// and issues four MMAs (64 elements of K) per block with offsets that are constants.
+DN8_DEV uint32_t uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
+DN8_DEV bool vote(bool x) { return __any_sync(0xffffffffu, x) != 0; }
+
+// Issued by a whole converged warp (one elected lane). D (+)= A B^T over 64 elements, 128-byte rows both.
+DN8_DEV void umma_f16_ss4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, e, t;\n\t.reg .b32 l;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
+                 "setp.eq.b32 t, 0, 0;\n\t"
+                 "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+                 "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
                  "elect.sync l|e, 0xffffffff;\n\t"
-                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// A from TMEM: 16 elements of a row in 8 columns, elements 2c and 2c + 1 in column c.
-DN8_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, e;\n\t.reg .b32 l;\n\t"
+// A from TMEM: 64 elements of a row in 32 columns, elements 2c and 2c + 1 in column c; B: 64 rows.
+DN8_DEV void umma_f16_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, e, t;\n\t.reg .b32 l, a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
+                 "setp.eq.b32 t, 0, 0;\n\t"
+                 "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+                 "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
                  "elect.sync l|e, 0xffffffff;\n\t"
-                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // D[128 x 128] = A B^T over DP elements, both tiles in shared memory
 template <typename T, int DP> DN8_DEV void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
-        umma_f16_ss(d, desc_rows(a, kk), desc_rows(b, kk), idesc_f16<T>(AT_TILE, AT_TILE, false), kk > 0);
+    for (int k = 0; k < DP / 64; ++k)
+        umma_f16_ss4(d, desc_rows(a, 4 * k), desc_rows(b, 4 * k), idesc_f16<T>(AT_TILE, AT_TILE, false), k > 0);
 }
-// D[128 x DP] (+)= A B, A [128 x 128] in TMEM (64 columns), B a tile of 128 rows
+// D[128 x DP] (+)= A B, A [128 x 128] in TMEM, B a tile of 128 rows. A lies over the fp32 tile it was made
+// from: its columns 0-63 in the 32 TMEM columns at 0, 64-127 in those at 64, each half over the part that
+// the same threads have read.
 template <typename T, int DP> DN8_DEV void mma_values(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
 #pragma unroll
-    for (int kk = 0; kk < AT_TILE / 16; ++kk)
-        umma_f16_ts(d, a + 8 * kk, desc_cols(b, kk), idesc_f16<T>(AT_TILE, DP, true), accumulate || kk > 0);
+    for (int k = 0; k < 2; ++k)
+        umma_f16_ts4(d, a + 64 * k, desc_cols(b, 4 * k), idesc_f16<T>(AT_TILE, DP, true), accumulate || k > 0);
 }
 
 // One row per thread: 16 packed words (32 elements of 16 bits) to columns taddr ..
@@ -88,6 +111,29 @@ DN8_DEV void tmem_wait_st(const uint32_t (&r)[16]) {
                  ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
+}
+
+// ---- work taken over from blocks that have not started ------------------------------------------
+// The grid has one block per piece of work; a running block asks the launch hardware for the index of a
+// block that has not been launched yet (that one then never is) and does its work too: setup once per
+// SM, no tail between pieces, and whoever is free takes the next one. One thread asks; the 16-byte answer
+// arrives in shared memory and completes on `bar`. After a refusal nothing may be asked again.
+DN8_DEV void ask_for_block(void* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+// The block's index, or -1: there is none left.
+DN8_DEV int answered_block(const void* answer) {
+    uint32_t ok, x = 0;
+    asm volatile("{\n\t.reg .b128 h;\n\t.reg .b64 lo, hi;\n\t.reg .pred p;\n\t"
+                 "ld.shared.v2.b64 {lo, hi}, [%2];\n\t"
+                 "mov.b128 h, {lo, hi};\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t"
+                 "mov.u32 %1, 0;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+                 : "=r"(ok), "=r"(x) : "r"(smem_u32(answer)) : "memory");
+    return ok ? static_cast<int>(x) : -1;
 }
 
 DN8_DEV float ex2(float x) {
