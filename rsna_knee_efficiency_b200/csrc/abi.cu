@@ -238,7 +238,9 @@ int dn8_layer_norm(const dn8_layer_norm_args* a, dn8_stream stream) {
     if (a->rows == 0) return DN8_OK;
     if (a->x == nullptr || a->y == nullptr || (a->res != nullptr && a->sum == nullptr))
         return fail(DN8_EINVAL, "dn8_layer_norm: x and y, and sum with res, must not be null");
-    cudaError_t e = dn8::launch_layer_norm(*a, static_cast<cudaStream_t>(stream));
+    int sms = 0;
+    if (int s = current_sms(&sms)) return s;
+    cudaError_t e = dn8::launch_layer_norm(*a, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_layer_norm launch");
 }
 

@@ -7,19 +7,17 @@ namespace dn8 {
 // ---- few rows over a long key axis -----------------------------------------------------------
 // The query rows of one key head's group (row r = query r / G, head r % G of the group) in blocks of
 // 16, one CTA per (row block, key head, share of the key tiles). Bound by reading keys and values once:
-// every warp streams its own tiles of 32 keys through its own ring of cp.async stages (no barrier
-// between warps), multiplies with 16-row matrix instructions (a tcgen05 tile has 128 rows, of which a
-// single token with 4 heads per group would fill 4) and keeps its own running maximum, sum and output;
-// the warps are joined in shared memory, the shares of the key axis by attn_join_kernel.
-// Rows of keys and values that no query may see (behind the sequence's end, or keep = 0) are filled
-// with zeros on the way in, so whatever they hold never meets an arithmetic instruction.
-constexpr int AR_WARPS = 4, AR_ROWS = 16, AR_KEYS = 32, AR_STAGES = 3;
+// every warp streams its own tiles (16 KB / D keys: 4 KB of keys, 4 KB of values) through its own ring of
+// TMA stages (no barrier between warps), multiplies with 16-row matrix instructions (a tcgen05 tile has
+// 128 rows, of which a single token with 4 heads per group would fill 4) and keeps its own running
+// maximum, sum and output; the warps are joined in shared memory, the shares of the key axis by
+// attn_join_kernel. Loads by cp.async with an address and a mask test per 16 bytes took 767 instructions
+// per tile and left the memory half idle; a TMA tile takes one, and tests are made per tile.
+// Rows of values that no query may see (behind the sequence's end, or keep = 0) are zeroed in shared
+// memory, since 0 * NaN is not 0; their scores are replaced, so keys may hold anything.
+constexpr int AR_WARPS = 4, AR_ROWS = 16, AR_STAGES = 3;
+constexpr uint32_t AR_TILE_BYTES = 4096, AR_STAGE = 2 * AR_TILE_BYTES;
 
-DN8_DEV void cp16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-DN8_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> DN8_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 DN8_DEV void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -48,25 +46,54 @@ struct RowsPlan {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(AR_WARPS * 32) attn_rows_kernel(const dn8_attention_args a, const RowsPlan plan) {
-    constexpr int CH = DP / 8;                           // 16-byte chunks of a row
-    constexpr int STAGE = 2 * AR_KEYS * DP * 2;          // keys and values of a stage, bytes
-    extern __shared__ __align__(128) uint8_t sm[];
+__global__ void __launch_bounds__(AR_WARPS * 32, 2)
+attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                 const dn8_attention_args a, const RowsPlan plan) {
+    constexpr int KEYS = AR_TILE_BYTES / (DP * 2);       // keys of a tile
+    constexpr uint32_t BLOCK = KEYS * 128;               // bytes of its 64 first elements
+    extern __shared__ uint8_t sm_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     __shared__ Sequence s_seq;
-    __shared__ uint32_t s_words[AR_WARPS][AR_STAGES];
+    __shared__ uint64_t s_full[AR_WARPS][AR_STAGES];
+    __shared__ int s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hk, kvh = blockIdx.z;
+    griddep_launch_dependents();
     if (warp == 0) {
         const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS);
         if (lane == 0) s_seq = f;
+    } else if (threadIdx.x == 32) {
+        for (int w = 0; w < AR_WARPS; ++w)
+            for (int k = 0; k < AR_STAGES; ++k) mbar_init(&s_full[w][k], 1);
+        s_abort = 0;
+        mbar_fence_init();
     }
     __syncthreads();
     const Sequence sq = s_seq;
     if (sq.b < 0) return;
+    volatile int* abort_flag = &s_abort;
     const int r0 = sq.blk * AR_ROWS, nrows = min(AR_ROWS, sq.nq * G - r0);
     const int off = sq.nk - sq.nq;
     const int left = a.left < 0 ? ATT_FAR : a.left, right = a.right < 0 ? ATT_FAR : a.right;
-    const KeyTiles kt = key_tiles(r0 / G + off, (r0 + nrows - 1) / G + off, sq.nk, left, right, a.sinks, AR_KEYS);
+    const int p0 = r0 / G + off, p1 = (r0 + nrows - 1) / G + off;      // first and last row's position
+    const KeyTiles kt = key_tiles(p0, p1, sq.nk, left, right, a.sinks, KEYS);
+    const int workers = plan.splits * AR_WARPS, me = blockIdx.y * AR_WARPS + warp;
+    uint8_t* ring = sm + warp * AR_STAGES * AR_STAGE;
+
+    auto issue = [&](int t, int stage) {                 // (lane 0)
+        if (t >= kt.count) return;
+        const int row = sq.k0 + kt.tile(t) * KEYS;
+        uint8_t* dst = ring + stage * AR_STAGE;
+        mbar_expect_tx(&s_full[warp][stage], AR_STAGE);
+#pragma unroll
+        for (int b = 0; b < DP / 64; ++b) {
+            tma_load_3d(dst + b * BLOCK, &mk, &s_full[warp][stage], b * 64, kvh, row);
+            tma_load_3d(dst + AR_TILE_BYTES + b * BLOCK, &mv, &s_full[warp][stage], b * 64, kvh, row);
+        }
+    };
+    if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < AR_STAGES; ++k) issue(me + k * workers, k);
 
     // the queries as matrix-instruction fragments
     uint32_t qf[DP / 16][4];
@@ -86,129 +113,120 @@ __global__ void __launch_bounds__(AR_WARPS * 32) attn_rows_kernel(const dn8_atte
                 qf[kk][half + 2 * c] = live && d < a.D ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
             }
     }
-    const uint32_t ring = smem_u32(sm) + warp * AR_STAGES * STAGE;
-    const int workers = plan.splits * AR_WARPS, me = blockIdx.y * AR_WARPS + warp;
-    const T* kbase = static_cast<const T*>(a.k) + static_cast<int64_t>(sq.k0) * a.k_stride_t + kvh * a.k_stride_h;
-    const T* vbase = static_cast<const T*>(a.v) + static_cast<int64_t>(sq.k0) * a.v_stride_t + kvh * a.v_stride_h;
-
     auto kept = [&](int t) -> bool {                     // this lane's key of tile index t may be seen
-        if (t >= kt.count) return false;
-        const int j = kt.tile(t) * AR_KEYS + lane;
+        if (t >= kt.count || lane >= KEYS) return true;
+        const int j = kt.tile(t) * KEYS + lane;
         return j < sq.nk && (a.keep == nullptr || a.keep[sq.k0 + j] != 0);
     };
     bool next_kept = kept(me);
-    auto issue = [&](int t, int stage) {
-        const uint32_t word = __ballot_sync(0xffffffffu, next_kept);
-        next_kept = kept(t + workers);
-        if (t < kt.count) {
-            const int j0 = kt.tile(t) * AR_KEYS;
-            const uint32_t base = ring + stage * STAGE;
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-                const int idx = k * 32 + lane, r = idx / CH, c = idx % CH;
-                const bool live = ((word >> r) & 1u) && c * 8 < a.D;
-                const uint32_t dst = base + r * (DP * 2) + ((c ^ (r & 7)) << 4);
-                const int64_t j = live ? j0 + r : 0;
-                const int cc = live ? c * 8 : 0;
-                cp16(dst, kbase + j * a.k_stride_t + cc, live);
-                cp16(dst + AR_KEYS * DP * 2, vbase + j * a.v_stride_t + cc, live);
-            }
-            if (lane == 0) s_words[warp][stage] = word;
-        }
-        cp_commit();
-    };
 
     float o[DP / 8][4];
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};          // references (times sc) and sums
     const float sc = a.scale * ATT_LOG2E;
-    int issued = me, stage = 0;
-#pragma unroll
-    for (int k = 0; k < AR_STAGES - 1; ++k) {
-        issue(issued, k);
-        issued += workers;
-    }
+    const int mat = lane >> 3, mr = lane & 7;
+    int stage = 0, phase = 0;
     for (int t = me; t < kt.count; t += workers) {
-        cp_wait<AR_STAGES - 2>();
-        __syncwarp();
-        const uint32_t kb = ring + stage * STAGE, vb = kb + AR_KEYS * DP * 2;
-        const uint32_t word = s_words[warp][stage];
-        float s[4][4];
+        const uint32_t word = __ballot_sync(0xffffffffu, next_kept);
+        next_kept = kept(t + workers);
+        if (!mbar_wait_w(&s_full[warp][stage], phase, a.err, abort_flag, ERR_WAIT_FULL | (57 << 4))) break;
+        uint8_t* tile = ring + stage * AR_STAGE;
+        const uint32_t kb = smem_u32(tile), vb = kb + AR_TILE_BYTES;
+        const int j0 = kt.tile(t) * KEYS;
+        if (word != 0xFFFFFFFFu) {
+            if (!((word >> lane) & 1u))
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+                for (int b = 0; b < DP / 64; ++b)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        reinterpret_cast<uint4*>(tile + AR_TILE_BYTES + b * BLOCK + lane * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
+            fence_async_smem();                          // (before the stage's next load)
+            __syncwarp();
+        }
+        float s[KEYS / 8][4];
+#pragma unroll
+        for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
-        const int mat = lane >> 3, mr = lane & 7;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-            for (int np = 0; np < 2; ++np) {
+            for (int np = 0; np < KEYS / 16; ++np) {
                 uint32_t b[4];
-                const int key = np * 16 + (mat >> 1) * 8 + mr, ch = kk * 2 + (mat & 1);
-                ldsm4(b, kb + key * (DP * 2) + ((ch ^ (key & 7)) << 4));
+                const int key = np * 16 + (mat >> 1) * 8 + mr, ch = (kk & 3) * 2 + (mat & 1);
+                ldsm4(b, kb + (kk >> 2) * BLOCK + key * 128 + ((ch ^ (key & 7)) << 4));
                 mma16<T>(s[2 * np], qf[kk], b[0], b[1]);
                 mma16<T>(s[2 * np + 1], qf[kk], b[2], b[3]);
             }
-        const int j0 = kt.tile(t) * AR_KEYS;
-        float mx[2] = {m[0], m[1]};
+        // does every row see every key of the tile?
+        if (word != 0xFFFFFFFFu || j0 + KEYS - 1 > p0 + right || (j0 < p1 - left && j0 + KEYS > a.sinks))
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int jl = n * 8 + (lane & 3) * 2 + (e & 1), j = j0 + jl, p = pos[e >> 1];
-                const bool see = ((word >> jl) & 1u) && j <= p + right && (j >= p - left || j < a.sinks);
-                s[n][e] = see ? s[n][e] * sc : -INFINITY;
-                mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-            }
-        float mref[2];
+                for (int e = 0; e < 4; ++e) {
+                    const int jl = n * 8 + (lane & 3) * 2 + (e & 1), j = j0 + jl, p = pos[e >> 1];
+                    const bool see = ((word >> jl) & 1u) && j <= p + right && (j >= p - left || j < a.sinks);
+                    s[n][e] = see ? s[n][e] : -INFINITY;
+                }
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            mref[h] = mx[h] == -INFINITY ? 0.0f : mx[h];       // a row that has seen nothing yet
-            const float f = exp2f(m[h] - mref[h]);
-            m[h] = mx[h];
-            l[h] *= f;
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-                o[n][2 * h] *= f;
-                o[n][2 * h + 1] *= f;
-            }
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * sc;
         }
+        // (rescaled only when a maximum has grown by more than 2^8: the weights stay below 256)
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.0f || mx[1] > m[1] + 8.0f))
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+            for (int h = 0; h < 2; ++h) {
+                const float mn = fmaxf(m[h], mx[h]);
+                const float f = ex2(m[h] - (mn == -INFINITY ? 0.0f : mn));
+                m[h] = mn;
+                l[h] *= f;
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n) {
+                    o[n][2 * h] *= f;
+                    o[n][2 * h + 1] *= f;
+                }
+            }
+        const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+        for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[n][e] = exp2f(s[n][e] - mref[e >> 1]);
+                s[n][e] = ex2(fmaf(s[n][e], sc, -ref[e >> 1]));
                 l[e >> 1] += s[n][e];
             }
 #pragma unroll
-        for (int kp = 0; kp < 2; ++kp) {
-            // weights in [0, 1] rounded to the values' type, the type of the matrix instruction
+        for (int kp = 0; kp < KEYS / 16; ++kp) {
+            // weights rounded to the values' type, the type of the matrix instruction
             const uint32_t p[4] = {pack2(T(), s[2 * kp][0], s[2 * kp][1]), pack2(T(), s[2 * kp][2], s[2 * kp][3]),
                                    pack2(T(), s[2 * kp + 1][0], s[2 * kp + 1][1]),
                                    pack2(T(), s[2 * kp + 1][2], s[2 * kp + 1][3])};
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n) {
                 uint32_t b[4];
-                const int key = kp * 16 + (mat & 1) * 8 + mr, ch = n * 2 + (mat >> 1);
-                ldsm4t(b, vb + key * (DP * 2) + ((ch ^ (key & 7)) << 4));
+                const int key = kp * 16 + (mat & 1) * 8 + mr, ch = (n & 3) * 2 + (mat >> 1);
+                ldsm4t(b, vb + (n >> 2) * BLOCK + key * 128 + ((ch ^ (key & 7)) << 4));
                 mma16<T>(o[2 * n], p, b[0], b[1]);
                 mma16<T>(o[2 * n + 1], p, b[2], b[3]);
             }
         }
         __syncwarp();                                    // every lane has read the stage
-        int fill = stage + AR_STAGES - 1;
-        if (fill >= AR_STAGES) fill -= AR_STAGES;
-        issue(issued, fill);
-        issued += workers;
-        if (++stage == AR_STAGES) stage = 0;
+        if (lane == 0) issue(t + AR_STAGES * workers, stage);
+        if (++stage == AR_STAGES) {
+            stage = 0;
+            phase ^= 1;
+        }
     }
-    cp_wait<0>();
     __syncthreads();                                     // the rings are free: join the warps there
+    if (*abort_flag) return;
     float* so = reinterpret_cast<float*>(sm);            // [warp][16][DP]
     float* sml = so + AR_WARPS * AR_ROWS * DP;           // [warp][16][2]
 #pragma unroll
@@ -218,9 +236,8 @@ __global__ void __launch_bounds__(AR_WARPS * 32) attn_rows_kernel(const dn8_atte
         const int r = lane / 4 + 8 * h;
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                so[(warp * AR_ROWS + r) * DP + n * 8 + (lane & 3) * 2 + e] = o[n][2 * h + e];
+            *reinterpret_cast<float2*>(so + (warp * AR_ROWS + r) * DP + n * 8 + (lane & 3) * 2) =
+                make_float2(o[n][2 * h], o[n][2 * h + 1]);
         if ((lane & 3) == 0) {
             sml[(warp * AR_ROWS + r) * 2] = m[h];
             sml[(warp * AR_ROWS + r) * 2 + 1] = l[h];
@@ -237,7 +254,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32) attn_rows_kernel(const dn8_atte
         float ov = 0.0f, lv = 0.0f;
 #pragma unroll
         for (int w = 0; w < AR_WARPS; ++w) {
-            const float f = exp2f(sml[(w * AR_ROWS + r) * 2] - ref);
+            const float f = ex2(sml[(w * AR_ROWS + r) * 2] - ref);
             ov = fmaf(f, so[(w * AR_ROWS + r) * DP + d], ov);
             lv = fmaf(f, sml[(w * AR_ROWS + r) * 2 + 1], lv);
         }
@@ -257,39 +274,52 @@ __global__ void __launch_bounds__(AR_WARPS * 32) attn_rows_kernel(const dn8_atte
     }
 }
 
-// Adds the shares of a row block: weights 2^(m_s - max m).
+// Adds the shares of a row block, one warp per row: weights 2^(m_s - max m), a share per lane (32 at a
+// time), then the lanes hold DP / 32 elements each and read the shares' rows.
 template <typename T, int DP>
-__global__ void __launch_bounds__(128) attn_join_kernel(const dn8_attention_args a, const RowsPlan plan) {
+__global__ void __launch_bounds__(AR_ROWS * 32) attn_join_kernel(const dn8_attention_args a, const RowsPlan plan) {
     __shared__ Sequence s_seq;
-    const int G = a.Hq / a.Hk, kvh = blockIdx.y;
-    if (threadIdx.x < 32) {
+    const int G = a.Hq / a.Hk, kvh = blockIdx.y, r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (r == 0) {
         const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS);
-        if (threadIdx.x == 0) s_seq = f;
+        if (lane == 0) s_seq = f;
     }
     __syncthreads();
     const Sequence sq = s_seq;
-    if (sq.b < 0) return;
-    const int r0 = sq.blk * AR_ROWS, nrows = min(AR_ROWS, sq.nq * G - r0);
+    if (sq.b < 0 || sq.blk * AR_ROWS + r >= sq.nq * G) return;
     const size_t slot = (static_cast<size_t>(blockIdx.x) * a.Hk + kvh) * plan.splits;
     griddep_wait();
-    for (int k = threadIdx.x; k < nrows * DP; k += 128) {
-        const int r = k / DP, d = k % DP;
-        float mm = -INFINITY;
-        for (int s = 0; s < plan.splits; ++s) mm = fmaxf(mm, plan.ml[((slot + s) * AR_ROWS + r) * 2]);
-        const float ref = mm == -INFINITY ? 0.0f : mm;
-        float ov = 0.0f, lv = 0.0f;
-        for (int s = 0; s < plan.splits; ++s) {
-            const float* ml = plan.ml + ((slot + s) * AR_ROWS + r) * 2;
-            const float f = exp2f(ml[0] - ref);
-            ov = fmaf(f, plan.o[((slot + s) * AR_ROWS + r) * DP + d], ov);
-            lv = fmaf(f, ml[1], lv);
+    float mm = -INFINITY;
+    for (int s = lane; s < plan.splits; s += 32) mm = fmaxf(mm, plan.ml[((slot + s) * AR_ROWS + r) * 2]);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    float lv = 0.0f, ov[DP / 32] = {};
+    for (int s0 = 0; s0 < plan.splits; s0 += 32) {
+        float w = 0.0f;
+        if (s0 + lane < plan.splits) {
+            const float2 ml = *reinterpret_cast<const float2*>(plan.ml + ((slot + s0 + lane) * AR_ROWS + r) * 2);
+            w = ex2(ml.x - ref);
+            lv = fmaf(w, ml.y, lv);
         }
-        const int64_t row = sq.q0 + (r0 + r) / G;
-        const int h = kvh * G + (r0 + r) % G;
-        if (d < a.D)
-            (static_cast<T*>(a.out) + row * a.o_stride_t + h * a.o_stride_h)[d] = from_f32<T>(lv > 0.0f ? ov / lv : 0.0f);
-        if (d == 0 && a.lse != nullptr) a.lse[row * a.Hq + h] = lv > 0.0f ? (mm + log2f(lv)) * ATT_LN2 : -INFINITY;
+        const int ns = min(32, plan.splits - s0);
+#pragma unroll 8
+        for (int s = 0; s < ns; ++s) {
+            float v[DP / 32];
+            load_f32(plan.o + ((slot + s0 + s) * AR_ROWS + r) * DP + lane * (DP / 32), v);
+            const float ws = __shfl_sync(0xffffffffu, w, s);
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e) ov[e] = fmaf(ws, v[e], ov[e]);
+        }
     }
+    lv = warp_sum(lv);
+    const int rr = sq.blk * AR_ROWS + r;
+    const int64_t row = sq.q0 + rr / G;
+    const int h = kvh * G + rr % G;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) ov[e] = lv > 0.0f ? ov[e] / lv : 0.0f;
+    if (lane * (DP / 32) < a.D) store_f32(static_cast<T*>(a.out) + row * a.o_stride_t + h * a.o_stride_h + lane * (DP / 32), ov);
+    if (lane == 0 && a.lse != nullptr) a.lse[row * a.Hq + h] = lv > 0.0f ? (mm + log2f(lv)) * ATT_LN2 : -INFINITY;
 }
 
 namespace {
@@ -307,8 +337,8 @@ RowsPlan rows_plan(const dn8_attention_args& a, int sms) {
         const int64_t w = static_cast<int64_t>(a.left) + a.right + 1 + a.sinks + a.Tq / a.B;
         if (w < seen) seen = w;
     }
-    const int64_t tiles = (seen + AR_KEYS - 1) / AR_KEYS;
-    int64_t s = 8ll * sms / (static_cast<int64_t>(p.blocks) * a.Hk);
+    const int64_t tiles = seen * head_pad(a.D) * 2 / AR_TILE_BYTES;
+    int64_t s = 12ll * sms / (static_cast<int64_t>(p.blocks) * a.Hk);
     if (s > tiles / (4 * AR_WARPS)) s = tiles / (4 * AR_WARPS);
     p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
     return p;
@@ -319,19 +349,27 @@ size_t rows_work(const dn8_attention_args& a, const RowsPlan& p) {
 }
 
 template <typename T, int DP> cudaError_t rows_go(const dn8_attention_args& a, RowsPlan p, cudaStream_t st) {
-    const size_t ring = static_cast<size_t>(AR_WARPS) * AR_STAGES * 2 * AR_KEYS * DP * 2;
-    const size_t join = static_cast<size_t>(AR_WARPS) * AR_ROWS * (DP + 2) * 4;
-    const size_t smem = ring > join ? ring : join;
+    constexpr size_t ring = static_cast<size_t>(AR_WARPS) * AR_STAGES * AR_STAGE;
+    constexpr size_t join = static_cast<size_t>(AR_WARPS) * AR_ROWS * (DP + 2) * 4;
+    constexpr size_t smem = 1024 + (ring > join ? ring : join);
     cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
+    CUtensorMap mk = {}, mv = {};
+    constexpr int keys = AR_TILE_BYTES / (DP * 2);
+    if (a.Tk > 0) {
+        e = make_head_map(&mk, a.k, a.type, a.Tk, a.Hk, a.D, a.k_stride_t, a.k_stride_h, keys);
+        if (e == cudaSuccess) e = make_head_map(&mv, a.v, a.type, a.Tk, a.Hk, a.D, a.v_stride_t, a.v_stride_h, keys);
+        if (e != cudaSuccess) return e;
+    }
     if (p.splits > 1) {
         p.o = static_cast<float*>(a.work);
         p.ml = p.o + static_cast<size_t>(p.blocks) * a.Hk * p.splits * AR_ROWS * DP;
     }
-    e = launch_pdl(false, attn_rows_kernel<T, DP>, dim3(p.blocks, p.splits, a.Hk), dim3(AR_WARPS * 32), smem, st, a, p);
+    e = launch_pdl(false, attn_rows_kernel<T, DP>, dim3(p.blocks, p.splits, a.Hk), dim3(AR_WARPS * 32), smem, st, mk, mv,
+                   a, p);
     if (e != cudaSuccess || p.splits == 1) return e;
-    return launch_pdl(true, attn_join_kernel<T, DP>, dim3(p.blocks, a.Hk), dim3(128), 0, st, a, p);
+    return launch_pdl(true, attn_join_kernel<T, DP>, dim3(p.blocks, a.Hk), dim3(AR_ROWS * 32), 0, st, a, p);
 }
 
 }  // namespace

@@ -482,7 +482,7 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 cudaError_t make_head_map(CUtensorMap* map, const void* base, int type, int64_t rows, int heads, int D, int64_t stride_t,
-                          int64_t stride_h) {
+                          int64_t stride_h, int box_rows) {
     static EncodeTiledFn encode = nullptr;
     if (encode == nullptr) {
         cudaDriverEntryPointQueryResult q;
@@ -496,7 +496,7 @@ cudaError_t make_head_map(CUtensorMap* map, const void* base, int type, int64_t 
     if (rows == 1) stride_t = stride_h * heads;
     cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
     cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride_h) * 2, static_cast<cuuint64_t>(stride_t) * 2};
-    cuuint32_t box[3] = {64, 1, AT_TILE};
+    cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_rows)};
     cuuint32_t estr[3] = {1, 1, 1};
     const CUtensorMapDataType t = type == DN8_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     CUresult r = encode(map, t, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -141,19 +141,6 @@ DN8_DEV float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-DN8_DEV uint32_t pack2(__half, float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    uint32_t u;
-    memcpy(&u, &h, 4);
-    return u;
-}
-DN8_DEV uint32_t pack2(__nv_bfloat16, float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    uint32_t u;
-    memcpy(&u, &h, 4);
-    return u;
-}
-
 // Bits [lo, hi] of a row of 128, word w.
 DN8_DEV uint32_t bits_from(int lo, int w) {
     const int k = lo - 32 * w;
@@ -164,9 +151,9 @@ DN8_DEV uint32_t bits_upto(int hi, int w) {
     return k < 0 ? 0u : k >= 31 ? 0xFFFFFFFFu : (2u << k) - 1u;
 }
 
-// 3-D map over [rows][heads][D] with token / head strides (elements): box 64 elements x 1 head x 128 rows.
-// Elements behind D and rows behind the tensor arrive as zeros.
+// 3-D map over [rows][heads][D] with token / head strides (elements): box 64 elements x 1 head x `box_rows`
+// rows. Elements behind D and rows behind the tensor arrive as zeros.
 cudaError_t make_head_map(CUtensorMap* map, const void* base, int type, int64_t rows, int heads, int D, int64_t stride_t,
-                          int64_t stride_h);
+                          int64_t stride_h, int box_rows = AT_TILE);
 
 }  // namespace dn8

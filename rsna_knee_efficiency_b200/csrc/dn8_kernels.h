@@ -64,7 +64,7 @@ int trans_chunk(int cout);
 cudaError_t launch_stem(const dn8_stem_args& a, int sms, cudaStream_t st);
 cudaError_t launch_head(const dn8_head_args& a, cudaStream_t st, bool pdl = false);
 cudaError_t launch_zoom(const dn8_zoom_args& a, int sms, cudaStream_t st);
-cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, cudaStream_t st);
+cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, int sms, cudaStream_t st);
 cudaError_t launch_layer_norm_bwd(const dn8_layer_norm_bwd_args& a, cudaStream_t st);
 size_t layer_norm_bwd_work(int C);
 cudaError_t launch_rope(const dn8_rope_args& a, int sms, cudaStream_t st);

@@ -47,70 +47,106 @@ template <int TPR> DN8_DEV void team_sum2(float& a, float& b, float* red) {
     __syncthreads();
 }
 
-// One row per team; a block holds 128 / TPR teams (at least one).
+// A team's rows are gridDim.x teams apart; the next row's loads are in flight while this one is reduced.
+// Weight and bias, for every row of a team the same, come from shared memory: in registers they cost
+// more in warps per SM than they save, and warps are what keeps enough bytes in flight.
 template <typename TX, typename TY, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) ln_kernel(const dn8_layer_norm_args a) {
-    constexpr int TEAMS = TPR < 128 ? 128 / TPR : 1;
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR < 512 ? (VEC * NV <= 16 ? 8 : 4) : (VEC * NV <= 16 ? 2 : 1))
+ln_kernel(const dn8_layer_norm_args a) {
+    constexpr int THREADS = TPR < 128 ? 128 : TPR, TEAMS = THREADS / TPR;
     __shared__ float red[TPR / 32];
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + threadIdx.x / TPR;
-    if (row >= a.rows) return;                               // a whole team (TPR > 32: a whole block)
+    extern __shared__ __align__(16) float wb[];              // [C] weights, [C] biases
     const int t = threadIdx.x % TPR, C = a.C;
-    const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
-    float h[NV][VEC];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (t + k * TPR) * VEC;
-        if (c < C) load_f32(x + c, h[k]);
-    }
-    if (a.res != nullptr) {
-        const TX* res = static_cast<const TX*>(a.res) + row * a.res_stride;
-        TX* sum = static_cast<TX*>(a.sum) + row * a.sum_stride;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * TEAMS;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + threadIdx.x / TPR;
+    Vec<TX, VEC> nx[NV], nr[NV];
+    auto fetch = [&](int64_t r) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (t + k * TPR) * VEC;
             if (c < C) {
-                float r[VEC];
-                load_f32(res + c, r);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) h[k][e] = to_f32(from_f32<TX>(h[k][e] + r[e]));
-                store_f32(sum + c, h[k]);
+                nx[k] = load_vec<TX, VEC>(static_cast<const TX*>(a.x) + r * a.x_stride + c);
+                if (a.res != nullptr)
+                    nr[k] = load_vec<TX, VEC>(static_cast<const TX*>(a.res) + r * a.res_stride + c);
             }
         }
-    }
-    float s = 0.0f;
+    };
+    if (row < a.rows) fetch(row);
+    for (int c = threadIdx.x * VEC; c < C; c += THREADS * VEC) {
+        float w[VEC], bi[VEC];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if ((t + k * TPR) * VEC < C)
+        for (int e = 0; e < VEC; ++e) {
+            w[e] = 1.0f;
+            bi[e] = 0.0f;
+        }
+        if (a.w != nullptr) load_param(a.w, a.w_type, c, w);
+        if (a.b != nullptr) load_param(a.b, a.w_type, c, bi);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            wb[c + e] = w[e];
+            wb[C + c + e] = bi[e];
+        }
+    }
+    __syncthreads();
+    if (row >= a.rows) return;                               // a whole team (TPR > 32: a whole block)
+    for (; row < a.rows; row += step) {
+        float h[NV][VEC];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (t + k * TPR) * VEC;
+            if (c < C) {
+                if (a.res != nullptr) {
+                    Vec<TX, VEC> s;
+                    float rv[VEC];
+                    nx[k].get(h[k]);
+                    nr[k].get(rv);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) h[k][e] += rv[e];
+                    s.set(h[k]);
+                    store_vec(static_cast<TX*>(a.sum) + row * a.sum_stride + c, s);
+                    s.get(h[k]);
+                } else {
+                    nx[k].get(h[k]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) h[k][e] = 0.0f;
+            }
+        }
+        if (row + step < a.rows) fetch(row + step);
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s += h[k][e];
-    const float mu = team_sum<TPR>(s, red) / static_cast<float>(C);
-    float q = 0.0f;
+        const float mu = team_sum<TPR>(s, red) / static_cast<float>(C);
+        float q = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-        if ((t + k * TPR) * VEC < C)
+        for (int k = 0; k < NV; ++k)
+            if ((t + k * TPR) * VEC < C)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float d = h[k][e] - mu;
-                q = fmaf(d, d, q);
+                for (int e = 0; e < VEC; ++e) {
+                    h[k][e] -= mu;
+                    q = fmaf(h[k][e], h[k][e], q);
+                }
+        const float r = rsqrtf(team_sum<TPR>(q, red) / static_cast<float>(C) + a.eps);
+        TY* y = static_cast<TY*>(a.y) + row * a.y_stride;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (t + k * TPR) * VEC;
+            if (c < C) {
+                float o[VEC], w[VEC], bi[VEC];
+                load_f32(wb + c, w);
+                load_f32(wb + C + c, bi);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o[e] = fmaf(h[k][e] * r, w[e], bi[e]);
+                store_f32(y + c, o);
             }
-    const float r = rsqrtf(team_sum<TPR>(q, red) / static_cast<float>(C) + a.eps);
-    TY* y = static_cast<TY*>(a.y) + row * a.y_stride;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (t + k * TPR) * VEC;
-        if (c < C) {
-            float w[VEC], b[VEC], o[VEC];
-            if (a.w != nullptr) load_param(a.w, a.w_type, c, w);
-            if (a.b != nullptr) load_param(a.b, a.w_type, c, b);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                o[e] = fmaf((h[k][e] - mu) * r, a.w != nullptr ? w[e] : 1.0f, a.b != nullptr ? b[e] : 0.0f);
-            store_f32(y + c, o);
         }
-    }
-    if (t == 0) {
-        if (a.mean != nullptr) a.mean[row] = mu;
-        if (a.rstd != nullptr) a.rstd[row] = r;
+        if (t == 0) {
+            if (a.mean != nullptr) a.mean[row] = mu;
+            if (a.rstd != nullptr) a.rstd[row] = r;
+        }
     }
 }
 
@@ -160,58 +196,79 @@ __global__ void __launch_bounds__(512) ln_long_kernel(const dn8_layer_norm_args 
 // shared memory and written as one row of the workspace [gridDim.x][2][C]; ln_cols_kernel adds the
 // rows in a fixed order (no atomics: the same bits every call).
 template <typename TX, typename TY, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) ln_bwd_kernel(const dn8_layer_norm_bwd_args a) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1) ln_bwd_kernel(const dn8_layer_norm_bwd_args a) {
     constexpr int THREADS = TPR < 256 ? 256 : TPR;
     constexpr int TEAMS = THREADS / TPR, CB = NV * VEC * TPR;      // columns a team covers
     __shared__ float red[TEAMS][2 * TPR / 32];
     __shared__ float part[TEAMS > 1 ? 2 * CB : 1];
     griddep_launch_dependents();
+    extern __shared__ __align__(16) float ws_[];             // [C] weights
     const int team = threadIdx.x / TPR, t = threadIdx.x % TPR, C = a.C;
-    float dw[NV][VEC], db[NV][VEC], w[NV][VEC];
+    float dw[NV][VEC], db[NV][VEC];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (t + k * TPR) * VEC;
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            dw[k][e] = db[k][e] = 0.0f;
-            w[k][e] = 1.0f;
-        }
-        if (c < C && a.w != nullptr) load_param(a.w, a.w_type, c, w[k]);
+        for (int e = 0; e < VEC; ++e) dw[k][e] = db[k][e] = 0.0f;
+    for (int c = threadIdx.x * VEC; c < C; c += THREADS * VEC) {
+        float w[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] = 1.0f;
+        if (a.w != nullptr) load_param(a.w, a.w_type, c, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) ws_[c + e] = w[e];
     }
+    __syncthreads();
     const float inv_c = 1.0f / static_cast<float>(C);
-    // every team of a block makes the same number of steps (the barriers of team_sum2)
+    // every team of a block makes the same number of steps (the barriers of team_sum2); the next row's loads
+    // are in flight while this one is reduced
     const int64_t step = static_cast<int64_t>(gridDim.x) * TEAMS;
+    Vec<TX, VEC> nx[NV], nd[NV];
+    Vec<TY, VEC> ng[NV];
+    float nmu = 0.0f, nr = 0.0f;
+    auto fetch = [&](int64_t r) {
+        if (r >= a.rows) return;
+        nmu = a.mean[r];
+        nr = a.rstd[r];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (t + k * TPR) * VEC;
+            if (c < C) {
+                nx[k] = load_vec<TX, VEC>(static_cast<const TX*>(a.x) + r * a.x_stride + c);
+                ng[k] = load_vec<TY, VEC>(static_cast<const TY*>(a.dy) + r * a.dy_stride + c);
+                if (a.dsum != nullptr)
+                    nd[k] = load_vec<TX, VEC>(static_cast<const TX*>(a.dsum) + r * a.dsum_stride + c);
+            }
+        }
+    };
+    fetch(static_cast<int64_t>(blockIdx.x) * TEAMS + team);
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * TEAMS; base < a.rows; base += step) {
         const int64_t row = base + team;
         const bool live = row < a.rows;
         float dy[NV][VEC], xh[NV][VEC];
-        float s1 = 0.0f, s2 = 0.0f, r = 0.0f;
+        Vec<TX, VEC> d[NV];
+        float s1 = 0.0f, s2 = 0.0f;
+        const float mu = nmu, r = nr;
         if (live) {
-            const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
-            const TY* g = static_cast<const TY*>(a.dy) + row * a.dy_stride;
-            const float mu = a.mean[row];
-            r = a.rstd[row];
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c = (t + k * TPR) * VEC;
-                if (c < C) {
-                    load_f32(x + c, xh[k]);
-                    load_f32(g + c, dy[k]);
-                }
-            }
 #pragma unroll
             for (int k = 0; k < NV; ++k)
-                if ((t + k * TPR) * VEC < C)
+                if ((t + k * TPR) * VEC < C) {
+                    float w[VEC];
+                    load_f32(ws_ + (t + k * TPR) * VEC, w);
+                    d[k] = nd[k];
+                    nx[k].get(xh[k]);
+                    ng[k].get(dy[k]);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         xh[k][e] = (xh[k][e] - mu) * r;
-                        const float gv = dy[k][e] * w[k][e];
-                        s1 += gv;
-                        s2 = fmaf(gv, xh[k][e], s2);
                         dw[k][e] = fmaf(dy[k][e], xh[k][e], dw[k][e]);
                         db[k][e] += dy[k][e];
+                        dy[k][e] *= w[e];
+                        s1 += dy[k][e];
+                        s2 = fmaf(dy[k][e], xh[k][e], s2);
                     }
+                }
         }
+        fetch(row + step);
         team_sum2<TPR>(s1, s2, red[team]);
         if (!live) continue;
         s1 *= inv_c;
@@ -221,15 +278,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) ln_bwd_kernel(const dn8
         for (int k = 0; k < NV; ++k) {
             const int c = (t + k * TPR) * VEC;
             if (c < C) {
-                float o[VEC];
+                float o[VEC], dv[VEC] = {};
+                if (a.dsum != nullptr) d[k].get(dv);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) o[e] = r * (dy[k][e] * w[k][e] - s1 - xh[k][e] * s2);
-                if (a.dsum != nullptr) {
-                    float d[VEC];
-                    load_f32(static_cast<const TX*>(a.dsum) + row * a.dsum_stride + c, d);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) o[e] += d[e];
-                }
+                for (int e = 0; e < VEC; ++e) o[e] = r * (dy[k][e] - s1 - xh[k][e] * s2) + dv[e];
                 store_f32(dx + c, o);
             }
         }
@@ -357,14 +409,32 @@ template <typename F> cudaError_t with_types(int tx, int ty, F&& f) {
     return ty == DN8_F16 ? f(float(), __half()) : f(float(), __nv_bfloat16());
 }
 
+// Blocks: enough for every SM's threads (8 blocks of 128 threads hold the registers of an SM), each with
+// several rows per team when there are many.
+template <typename TX, typename TY, int VEC, int NV, int TPR>
+cudaError_t ln_team(const dn8_layer_norm_args& a, int sms, cudaStream_t st) {
+    constexpr int THREADS = TPR < 128 ? 128 : TPR, TEAMS = THREADS / TPR;
+    const int64_t want = (a.rows + TEAMS - 1) / TEAMS, most = static_cast<int64_t>(sms) * (1024 / THREADS);
+    const size_t smem = static_cast<size_t>(a.C) * 2 * sizeof(float);
+    if (smem > 40 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(ln_kernel<TX, TY, VEC, NV, TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, TPR>, dim3(static_cast<unsigned>(want < most ? want : most)),
+                      dim3(THREADS), smem, st, a);
+}
+// The smallest team that holds a row: 16 elements per thread, else up to 32 (and then 16 in wider teams)
 template <typename TX, typename TY, int VEC, int NV>
-cudaError_t ln_go(const dn8_layer_norm_args& a, cudaStream_t st) {
-    const int per = VEC * NV;
-    const dim3 rows(static_cast<unsigned>(a.rows)), rows4(static_cast<unsigned>((a.rows + 3) / 4));
-    if (a.C <= 32 * per) return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, 32>, rows4, dim3(128), 0, st, a);
-    if (a.C <= 128 * per) return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, 128>, rows, dim3(128), 0, st, a);
-    if (a.C <= 512 * per) return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, 512>, rows, dim3(512), 0, st, a);
-    return launch_pdl(false, ln_long_kernel<TX, TY>, rows, dim3(512), 0, st, a);
+cudaError_t ln_go(const dn8_layer_norm_args& a, int sms, cudaStream_t st) {
+    constexpr int per = VEC * NV;
+    if (a.C <= 32 * per) return ln_team<TX, TY, VEC, NV, 32>(a, sms, st);
+    if (a.C <= 64 * per) return ln_team<TX, TY, VEC, 2 * NV, 32>(a, sms, st);
+    if (a.C <= 128 * per) return ln_team<TX, TY, VEC, NV, 128>(a, sms, st);
+    if (a.C <= 256 * per) return ln_team<TX, TY, VEC, 2 * NV, 128>(a, sms, st);
+    if (a.C <= 512 * per) return ln_team<TX, TY, VEC, NV, 512>(a, sms, st);
+    if (a.C <= 1024 * per) return ln_team<TX, TY, VEC, 2 * NV, 512>(a, sms, st);
+    return launch_pdl(false, ln_long_kernel<TX, TY>, dim3(static_cast<unsigned>(a.rows)), dim3(512), 0, st, a);
 }
 
 template <typename TX, typename TY, int VEC, int NV>
@@ -374,9 +444,10 @@ cudaError_t ln_bwd_go(const dn8_layer_norm_bwd_args& a, cudaStream_t st, int* nr
     const int64_t want = (a.rows + teams - 1) / teams;
     const int grid = static_cast<int>(want < LN_COLS_ROWS ? want : LN_COLS_ROWS);
     *nrows = grid;
-    if (a.C <= 32 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 32>, dim3(grid), dim3(256), 0, st, a);
-    if (a.C <= 128 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 128>, dim3(grid), dim3(256), 0, st, a);
-    if (a.C <= 512 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 512>, dim3(grid), dim3(512), 0, st, a);
+    const size_t smem = static_cast<size_t>(a.C) * sizeof(float);
+    if (a.C <= 32 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 32>, dim3(grid), dim3(256), smem, st, a);
+    if (a.C <= 128 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 128>, dim3(grid), dim3(256), smem, st, a);
+    if (a.C <= 512 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 512>, dim3(grid), dim3(512), smem, st, a);
     if (a.work != nullptr) {
         const int slabs = static_cast<int>(a.rows < 32 ? 1 : a.rows / 32 < LN_COLS_ROWS ? a.rows / 32 : LN_COLS_ROWS);
         *nrows = slabs;
@@ -388,7 +459,7 @@ cudaError_t ln_bwd_go(const dn8_layer_norm_bwd_args& a, cudaStream_t st, int* nr
 
 }  // namespace
 
-cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, cudaStream_t st) {
+cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, int sms, cudaStream_t st) {
     const int sx = type_size(a.x_type), sy = type_size(a.y_type);
     const bool vec = a.C % 8 == 0 && vec_ok(a.w, 0, 4) && vec_ok(a.b, 0, 4) && vec_ok(a.x, a.x_stride, sx) &&
                      vec_ok(a.y, a.y_stride, sy) &&
@@ -397,9 +468,9 @@ cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, cudaStream_t st) {
         using TX = decltype(tx);
         using TY = decltype(ty);
         // 16-byte loads where every row allows them, single elements otherwise
-        if (!vec) return ln_go<TX, TY, 1, 16>(a, st);
-        if (sizeof(TX) == 4) return ln_go<TX, TY, 4, 8>(a, st);
-        return ln_go<TX, TY, 8, 4>(a, st);
+        if (!vec) return ln_go<TX, TY, 1, 16>(a, sms, st);
+        if (sizeof(TX) == 4) return ln_go<TX, TY, 4, 4>(a, sms, st);
+        return ln_go<TX, TY, 8, 2>(a, sms, st);
     });
 }
 

@@ -20,7 +20,8 @@ namespace dn8 {
 
 constexpr int RP_THREADS = 256;
 constexpr int RP_MAX_PAIRS = 128;
-constexpr int RP_BATCH = 4;                       // items a thread has in flight
+constexpr int RP_BATCH = 2;                       // items a thread has in flight
+constexpr int RP_BLOCK_ITEMS = 4;                 // and the items per thread a block is cut for
 
 struct RopeTable {
     double turns[RP_MAX_PAIRS];                   // f_j / (2 pi)
@@ -29,9 +30,9 @@ struct RopeTable {
 
 // An item is VEC pairs of one head of one token (or VEC of the elements behind the pairs).
 template <typename T, int VEC, bool INTER>
-__global__ void __launch_bounds__(RP_THREADS) rope_kernel(const dn8_rope_args a, const __grid_constant__ RopeTable tab,
+__global__ void __launch_bounds__(RP_THREADS, 4) rope_kernel(const dn8_rope_args a, const __grid_constant__ RopeTable tab,
                                                           int pairs, int tokens_per_block) {
-    extern __shared__ float2 cs[];                // [tokens of the block][pairs]
+    extern __shared__ __align__(16) float2 cs[];  // [tokens of the block][pairs]
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * tokens_per_block;
     const int nt = static_cast<int>(min(static_cast<int64_t>(tokens_per_block), a.T - t0));
     for (int k = threadIdx.x; k < nt * pairs; k += RP_THREADS) {
@@ -45,71 +46,67 @@ __global__ void __launch_bounds__(RP_THREADS) rope_kernel(const dn8_rope_args a,
     __syncthreads();
     const int heads = a.Hq + a.Hk;
     const int pv = pairs / VEC, tail = (a.D - 2 * pairs) / VEC, per_head = pv + tail;
-    const int items = nt * heads * per_head;
-    for (int i0 = threadIdx.x; i0 < items; i0 += RP_THREADS * RP_BATCH) {
-        float x1[RP_BATCH][VEC], x2[RP_BATCH][VEC];
+    // Item i = (token, head, v). A thread's items are RP_THREADS apart: the three indices advance by
+    // constant steps with a carry, instead of two divisions per item.
+    const int sv = RP_THREADS % per_head, sh = RP_THREADS / per_head % heads, st = RP_THREADS / per_head / heads;
+    int v = threadIdx.x % per_head, h = threadIdx.x / per_head % heads, t = threadIdx.x / per_head / heads;
+    while (t < nt) {
+        Vec<T, VEC> x1[RP_BATCH], x2[RP_BATCH];              // (interleaved: 2 VEC consecutive elements)
         T* dst[RP_BATCH];
-        int at[RP_BATCH], tok[RP_BATCH];
+        const float2* c[RP_BATCH];
 #pragma unroll
         for (int b = 0; b < RP_BATCH; ++b) {
-            const int i = i0 + b * RP_THREADS;
             dst[b] = nullptr;
-            if (i >= items) continue;
-            const int v = i % per_head, th = i / per_head;
-            const int h = th % heads;
-            tok[b] = th / heads;
-            const T* src;
-            if (h < a.Hq) {
-                src = static_cast<const T*>(a.q) + (t0 + tok[b]) * a.q_stride_t + h * a.q_stride_h;
-                dst[b] = static_cast<T*>(a.q_out) + (t0 + tok[b]) * a.qo_stride_t + h * a.qo_stride_h;
-            } else {
-                src = static_cast<const T*>(a.k) + (t0 + tok[b]) * a.k_stride_t + (h - a.Hq) * a.k_stride_h;
-                dst[b] = static_cast<T*>(a.k_out) + (t0 + tok[b]) * a.ko_stride_t + (h - a.Hq) * a.ko_stride_h;
-            }
-            if (v >= pv) {
-                at[b] = -(2 * pairs + (v - pv) * VEC);
-                load_f32(src - at[b], x1[b]);
-            } else if (INTER) {
-                at[b] = v * VEC;
-                float x[2 * VEC];
-                load_f32(src + 2 * at[b], x);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    x1[b][e] = x[2 * e];
-                    x2[b][e] = x[2 * e + 1];
+            if (t < nt) {
+                const bool isq = h < a.Hq;
+                const int hh = isq ? h : h - a.Hq;
+                const int64_t row = t0 + t;
+                const T* src = (isq ? static_cast<const T*>(a.q) + row * a.q_stride_t + hh * a.q_stride_h
+                                    : static_cast<const T*>(a.k) + row * a.k_stride_t + hh * a.k_stride_h);
+                T* out = (isq ? static_cast<T*>(a.q_out) + row * a.qo_stride_t + hh * a.qo_stride_h
+                              : static_cast<T*>(a.k_out) + row * a.ko_stride_t + hh * a.ko_stride_h);
+                // where the item's elements start, and those of its other half
+                const int at = v >= pv ? 2 * pairs + (v - pv) * VEC : INTER ? 2 * v * VEC : v * VEC;
+                c[b] = v >= pv ? nullptr : cs + t * pairs + v * VEC;
+                dst[b] = out + at;
+                x1[b] = load_vec<T, VEC>(src + at);
+                if (v < pv) x2[b] = load_vec<T, VEC>(src + at + (INTER ? VEC : pairs));
+                v += sv;
+                h += sh;
+                t += st;
+                if (v >= per_head) {
+                    v -= per_head;
+                    ++h;
                 }
-            } else {
-                at[b] = v * VEC;
-                load_f32(src + at[b], x1[b]);
-                load_f32(src + pairs + at[b], x2[b]);
+                if (h >= heads) {
+                    h -= heads;
+                    ++t;
+                }
             }
         }
 #pragma unroll
         for (int b = 0; b < RP_BATCH; ++b) {
             if (dst[b] == nullptr) continue;
-            if (at[b] < 0) {
-                store_f32(dst[b] - at[b], x1[b]);
+            if (c[b] == nullptr) {
+                store_vec(dst[b], x1[b]);
                 continue;
             }
-            const float2* c = cs + tok[b] * pairs + at[b];
-            float y1[VEC], y2[VEC];
+            float u[2 * VEC], y[2 * VEC];                    // the loaded elements in order, and the turned ones
+            float (&lo)[VEC] = reinterpret_cast<float (&)[VEC]>(u);
+            float (&hi)[VEC] = reinterpret_cast<float (&)[VEC]>(u[VEC]);
+            x1[b].get(lo);
+            x2[b].get(hi);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                y1[e] = x1[b][e] * c[e].x - x2[b][e] * c[e].y;
-                y2[e] = x2[b][e] * c[e].x + x1[b][e] * c[e].y;
+                const int i1 = INTER ? 2 * e : e, i2 = INTER ? 2 * e + 1 : VEC + e;
+                const float2 w = c[b][e];                    // cos, sin
+                y[i1] = u[i1] * w.x - u[i2] * w.y;
+                y[i2] = u[i2] * w.x + u[i1] * w.y;
             }
-            if (INTER) {
-                float y[2 * VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    y[2 * e] = y1[e];
-                    y[2 * e + 1] = y2[e];
-                }
-                store_f32(dst[b] + 2 * at[b], y);
-            } else {
-                store_f32(dst[b] + at[b], y1);
-                store_f32(dst[b] + pairs + at[b], y2);
-            }
+            x1[b].set(reinterpret_cast<const float (&)[VEC]>(y));
+            x2[b].set(reinterpret_cast<const float (&)[VEC]>(y[VEC]));
+            store_vec(dst[b], x1[b]);
+            store_vec(dst[b] + (INTER ? VEC : pairs), x2[b]);
         }
     }
 }
@@ -147,10 +144,10 @@ cudaError_t launch_rope(const dn8_rope_args& a, int sms, cudaStream_t st) {
     for (const void* p : {a.q, static_cast<const void*>(a.q_out), a.k, static_cast<const void*>(a.k_out)})
         wide = wide && (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
     const int v = wide ? vec : 1;
-    // Tokens per block: about RP_BATCH items per thread, but at least two blocks per SM while there
+    // Tokens per block: about RP_BLOCK_ITEMS items per thread, but at least two blocks per SM while there
     // are tokens for them.
     const int per_token = heads * (pairs / v + (a.D - 2 * pairs) / v);
-    int64_t tpb = RP_THREADS * RP_BATCH / (per_token > 0 ? per_token : 1);
+    int64_t tpb = RP_THREADS * RP_BLOCK_ITEMS / (per_token > 0 ? per_token : 1);
     const int64_t spread = a.T / (2 * sms);
     if (tpb > spread) tpb = spread;
     if (tpb < 1) tpb = 1;
