@@ -342,7 +342,10 @@ int dn8_attention(const dn8_attention_args* a, dn8_stream stream) {
 
 int64_t dn8_attention_bwd_work(const dn8_attention_bwd_args* a) {
     if (check_attention(a, "dn8_attention_bwd_work")) return -1;
-    return a->B == 0 ? 0 : static_cast<int64_t>(dn8::attention_bwd_work(*a));
+    if (a->B == 0) return 0;
+    int sms = 0;
+    if (current_sms(&sms)) return -1;
+    return static_cast<int64_t>(dn8::attention_bwd_work(*a, sms));
 }
 
 int dn8_attention_bwd(const dn8_attention_bwd_args* a, dn8_stream stream) {
@@ -360,7 +363,9 @@ int dn8_attention_bwd(const dn8_attention_bwd_args* a, dn8_stream stream) {
         return fail(DN8_EINVAL, "dn8_attention_bwd: pointers must be non-null and 16-byte aligned");
     if ((a->Tq > 1 && a->do_stride_t == 0) || (a->Hq > 1 && a->do_stride_h == 0))
         return fail(DN8_EINVAL, "dn8_attention_bwd: rows or heads of dout share memory (stride 0)");
-    cudaError_t e = dn8::launch_attention_bwd(*a, static_cast<cudaStream_t>(stream));
+    int sms = 0;
+    if (int s = current_sms(&sms)) return s;
+    cudaError_t e = dn8::launch_attention_bwd(*a, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_attention_bwd launch");
 }
 

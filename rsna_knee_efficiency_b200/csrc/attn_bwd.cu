@@ -13,9 +13,12 @@
 //   dk, dv: R = k, v; X = q, dout: P and dS go back to TMEM in 16 bits over S and dP, and
 //           dv += P X1, dk += dS X0
 //   dq:     R = q, dout; X = k, v: dS goes back, dq += dS X0
-// so no operand is ever transposed or written to shared memory by a thread. The issue order dv(u),
-// S(u + 1), dk(u), dP(u + 1) keeps the tensor cores on one of them while the threads work on the other:
-// exponentials of S while dP is made, dS while dv and the next S are made.
+// so no operand is ever transposed or written to shared memory by a thread. Where TMEM has room for two
+// S tiles (all but dk, dv with D > 64) S(u + 1) is made while the threads are still on step u, and dP(u + 1)
+// while they take the exponentials of S(u + 1); else S(u + 1) is made while they work on dS(u).
+//
+// A CTA takes one piece (one walk) after the other (ask_for_block). Under a window, the first tokens' key
+// tile is seen by every query: its walk is cut into shares, whose sums attn_bwd_join_kernel adds.
 #include "attn_umma.cuh"
 
 namespace dn8 {
@@ -47,212 +50,234 @@ __global__ void __launch_bounds__(32 * LANES) attn_bwd_prep_kernel(const dn8_att
 }
 
 // ---- the two walks -----------------------------------------------------------------------------
-constexpr int AB_THREADS = 384;             // warps 0-7: rows; 8: tcgen05 issue; 9: TMA; 10: masked rows
+constexpr int AB_THREADS = 640;             // warps 0-15: rows; 16: tcgen05 issue; 17: TMA; 18: masked rows; 19: pieces
+// The launch gives every thread 96 registers: 16 x 32 x 104 + 4 x 32 x 64 = 20 x 32 x 96.
+constexpr int AB_REGS_ROWS = 104, AB_REGS_OTHER = 64;
 template <int DP> struct BwdCfg {
     static constexpr int ST = DP == 64 ? 3 : 2;
     static constexpr uint32_t TILE = AT_TILE * DP * 2;
-    static constexpr uint32_t SMEM = 1024 + TILE * 2 * (1 + ST) + 4096 + 1024;
-    static constexpr uint32_t S = 0, DPC = 128, ACC0 = 256, ACC1 = 256 + DP;     // TMEM columns
+    static constexpr uint32_t SMEM = 1024 + TILE * 2 * (1 + ST) + 4096;
+    // TMEM columns: dP, then S (one or two tiles), then the sums at the end
+    static constexpr uint32_t DPC = 0, S = 128, ACC1 = 512 - DP, ACC0 = 512 - 2 * DP;
+};
+// S tiles: the sums are dv (ACC0) and dk (ACC1), or dq (ACC1)
+template <int DP> DN8_DEV constexpr int s_tiles(bool kv) { return kv && DP == 128 ? 1 : 2; }
+
+// Shares of the walks over the first tokens' key tiles (shares = 1: none are cut).
+struct BwdPlan {
+    int kv_blocks, split_blocks, tiles, shares;
+    float* part;                              // [sequence][tile][key head][share][dv, dk][128][DP]
+};
+
+struct BwdPiece {
+    Sequence seq;                             // seq.b = -2: no more pieces
+    int kv;                                   // dk, dv of a key tile, or dq of a query tile
+    int r0;                                   // first resident row, within the sequence
+    int h;                                    // key head (kv) or query head
+    int begin, steps;                         // kv: the share's first step of the tile's walk; steps
+    int first, per;                           // kv: first query tile and query tiles per head
+    int share;                                // kv: where a share's sums go, or -1: straight to dk, dv
+    KeyTiles keys;                            // dq: key tiles
+    // query or key tile of step u, and for dk, dv the head within the group
+    DN8_DEV int tile(int u) const { return kv ? first + (begin + u) % per : keys.tile(u); }
+    DN8_DEV int head(int u) const { return kv ? (begin + u) / per : 0; }
 };
 struct BwdShared {
-    float lse2[3][AT_TILE], delta[3][AT_TILE];
+    uint64_t answer[2];
+    uint64_t answered, pfilled, pread, rfull, rempty, fin, aempty, dpfull, dsready;
+    // (of even and odd steps: the rows may be done with S(u + 1), where there are two S tiles, before the
+    // issuing warp, held up by its own queue, has looked for S(u))
+    uint64_t pready[2];
+    uint64_t sfull[2], xfull[3], xempty[3], xok[3];
+    BwdPiece piece[2];
     uint32_t words[3][4];
-    uint64_t rfull, fin, sfull, dpfull, pready, dsready;
-    uint64_t xfull[3], xempty[3], xok[3];
     uint32_t tmem;
     int abort;
-    Sequence seq;
+    alignas(16) float lse2[3][AT_TILE], delta[3][AT_TILE];
 };
 
-// What a CTA does: its resident rows and the tiles it walks over.
-struct BwdWalk {
-    bool kv;                 // dk, dv of a key tile, or dq of a query tile
-    int r0;                  // first resident row, within the sequence
-    int h;                   // key head (kv) or query head
-    int steps;
-    int first, per;          // kv: first query tile and query tiles per head
-    KeyTiles keys;           // dq: key tiles
-};
-
-// The 8 row warps: warp w has the TMEM lanes (resident rows) 32 (w % 4) .. and the columns 64 (w / 4) .. of
-// every step.
+// The 16 row warps on one piece: warp w has the TMEM lanes (resident rows) 32 (w % 4) .. and the columns
+// 32 (w / 4) .. of every step. c: steps of this CTA so far; sp: phases of sfull.
 template <typename T, int DP, bool KV>
-DN8_DEV void bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdWalk& wk, uint32_t tmem) {
+DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdPiece& pc, float* part, uint32_t tmem,
+                      uint32_t& c, uint32_t& sp, uint32_t& fp) {
     using C = BwdCfg<DP>;
+    constexpr int NS = s_tiles<DP>(KV);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t quad = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + C::S + quad + half * 64, tp = tmem + C::DPC + quad + half * 64;
+    const int quarter = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     volatile int* abort_flag = &sh.abort;
-    const Sequence seq = sh.seq;
-    const int off = seq.nk - seq.nq;
     const int left = a.left < 0 ? ATT_FAR : a.left, right = a.right < 0 ? ATT_FAR : a.right;
     const float sc = a.scale * ATT_LOG2E;
-    const int r = wk.r0 + row;                                   // key j (KV) or query i
-    const bool inside = r < (KV ? seq.nk : seq.nq);
+    const int r = pc.r0 + row;                                   // key j (KV) or query i
+    const bool inside = r < (KV ? pc.seq.nk : pc.seq.nq);
     // KV: the key may be seen at all; dq: the row's statistics
-    const bool keep = KV && inside && (a.keep == nullptr || a.keep[seq.k0 + r] != 0);
+    const bool keep = KV && inside && (a.keep == nullptr || a.keep[pc.seq.k0 + r] != 0);
     float row_lse = INFINITY, row_delta = 0.0f;
     if (!KV && inside) {
-        const float* w = static_cast<const float*>(a.work) + wk.h * a.Tq + seq.q0 + r;
+        const float* w = static_cast<const float*>(a.work) + pc.h * a.Tq + pc.seq.q0 + r;
         row_lse = w[0];
         row_delta = w[a.Hq * a.Tq];
     }
-    const int rlast = min(wk.r0 + AT_TILE, KV ? seq.nk : seq.nq) - 1;
     bool ok = true;
-    for (int u = 0; u < wk.steps; ++u) {
-        const int st = u % C::ST;
-        const int c0 = (KV ? wk.first + u % wk.per : wk.keys.tile(u)) * AT_TILE, cl = c0 + AT_TILE - 1;
-        ok = mbar_wait_w(&sh.xok[st], (u / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (80 << 4));
-        if (!ok) break;
-        uint32_t word[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+    for (int u = 0; u < pc.steps; ++u, ++c) {
+        const uint32_t st = c % C::ST;
+        const int off = pc.seq.nk - pc.seq.nq, c0 = pc.tile(u) * AT_TILE, cl = c0 + AT_TILE - 1;
+        const int rlast = min(pc.r0 + AT_TILE, KV ? pc.seq.nk : pc.seq.nq) - 1;
+        ok = mbar_wait_w(&sh.xok[st], (c / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (80 << 4));
+        if (!ok) return false;
+        uint32_t word = 0xFFFFFFFFu;
         bool masked;
         if (KV) {
             // columns are queries: seen from j - right - off on, up to j + left - off (first tokens: by all).
             // Queries behind the end are zero rows with lse2 = inf.
-            masked = a.keep != nullptr || wk.r0 + AT_TILE > seq.nk || c0 + off < rlast - right ||
-                     (cl + off > wk.r0 + left && rlast >= a.sinks);
+            masked = a.keep != nullptr || pc.r0 + AT_TILE > pc.seq.nk || c0 + off < rlast - right ||
+                     (cl + off > pc.r0 + left && rlast >= a.sinks);
             if (masked) {
                 const int lo = r - right - off - c0, hi = r < a.sinks ? ATT_FAR : r + left - off - c0;
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
-                    word[w] = keep ? bits_from(lo, 2 * half + w) & bits_upto(hi, 2 * half + w) : 0u;
+                word = keep ? bits_from(lo, quarter) & bits_upto(hi, quarter) : 0u;
             }
         } else {
-            const int p = r + off;
-            masked = a.keep != nullptr || cl > min(seq.nk - 1, wk.r0 + off + right) || (c0 < rlast + off - left && cl >= a.sinks);
+            masked = a.keep != nullptr || cl > min(pc.seq.nk - 1, pc.r0 + off + right) ||
+                     (c0 < rlast + off - left && cl >= a.sinks);
             if (masked) {
-                const int hi = min(seq.nk - 1, p + right) - c0, lo = p - left - c0;
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
-                    word[w] = bits_upto(hi, 2 * half + w) & sh.words[st][2 * half + w] &
-                              (bits_from(lo, 2 * half + w) | bits_upto(a.sinks - 1 - c0, 2 * half + w));
+                const int p = r + off, hi = min(pc.seq.nk - 1, p + right) - c0, lo = p - left - c0;
+                word = bits_upto(hi, quarter) & sh.words[st][quarter] &
+                       (bits_from(lo, quarter) | bits_upto(a.sinks - 1 - c0, quarter));
             }
         }
-        ok = mbar_wait_w(&sh.sfull, u & 1, a.err, abort_flag, ERR_WAIT_ACC | (81 << 4));
-        if (!ok) break;
+        const int sb = NS == 1 ? 0 : u & 1;
+        const uint32_t ts = lanes + C::S + sb * 128 + quarter * 32, tp = lanes + C::DPC + quarter * 32;
+        ok = mbar_wait_w(&sh.sfull[sb], (sp >> sb) & 1, a.err, abort_flag, ERR_WAIT_ACC | (81 << 4));
+        if (!ok) return false;
+        sp ^= 1u << sb;
         tc_fence_after();
-        uint32_t pr[2][32];                                      // P of this thread's 64 columns, fp32
-        tmem_ld32(ts, pr[0]);
-        tmem_ld32(ts + 32, pr[1]);
-        tmem_wait_ld(pr[0]);
-        reg_bind(pr[1]);
-        if (!KV) {                                               // S is in registers: the next one may come
+        uint32_t pr[32];                                         // P of this thread's columns, fp32
+        tmem_ld32(ts, pr);
+        tmem_wait_ld(pr);
+        if (!KV) {                                               // S is in registers: its tile is free
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.pready);
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (KV) {
-                const float4* l4 = reinterpret_cast<const float4*>(sh.lse2[st] + half * 64 + c * 32);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float4 l = l4[e];
-                    const float ls[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        pr[c][4 * e + x] = __float_as_uint(ex2(fmaf(__uint_as_float(pr[c][4 * e + x]), sc, -ls[x])));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    pr[c][e] = __float_as_uint(ex2(fmaf(__uint_as_float(pr[c][e]), sc, -row_lse)));
-            }
-            if (masked)
-#pragma unroll
-                for (int e = 0; e < 32; ++e) pr[c][e] = (word[c] >> e) & 1u ? pr[c][e] : 0u;
+            if (lane == 0) mbar_arrive(&sh.pready[c & 1]);
         }
         if (KV) {
+            const float4* l4 = reinterpret_cast<const float4*>(sh.lse2[st] + quarter * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float4 l = l4[e];
+                const float ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    pr[4 * e + x] = __float_as_uint(ex2(fmaf(__uint_as_float(pr[4 * e + x]), sc, -ls[x])));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pr[e] = __float_as_uint(ex2(fmaf(__uint_as_float(pr[e]), sc, -row_lse)));
+        }
+        if (masked)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pr[e] = (word >> e) & 1u ? pr[e] : 0u;
+        if (KV) {
             // P in [0, 1], rounded to the inputs' type for dv
-            uint32_t pk[32];
+            uint32_t pk[16];
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    pk[16 * c + e] = pack2(T(), __uint_as_float(pr[c][2 * e]), __uint_as_float(pr[c][2 * e + 1]));
-            tmem_st32(ts, pk);
+            for (int e = 0; e < 16; ++e) pk[e] = pack2(T(), __uint_as_float(pr[2 * e]), __uint_as_float(pr[2 * e + 1]));
+            tmem_st16(ts, pk);
             tmem_wait_st(pk);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.pready);
+            if (lane == 0) mbar_arrive(&sh.pready[c & 1]);
         }
-        ok = mbar_wait_w(&sh.dpfull, u & 1, a.err, abort_flag, ERR_WAIT_ACC | (82 << 4));
-        if (!ok) break;
+        ok = mbar_wait_w(&sh.dpfull, c & 1, a.err, abort_flag, ERR_WAIT_ACC | (82 << 4));
+        if (!ok) return false;
         tc_fence_after();
-        uint32_t pk[32];
+        uint32_t dp[32], pk[16];
+        tmem_ld32(tp, dp);
+        tmem_wait_ld(dp);
+        // (a masked pair's P is 0, but its dP may be NaN, and 0 * NaN is not 0)
+        if (masked)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            uint32_t dp[32];
-            tmem_ld32(tp + 32 * c, dp);
-            tmem_wait_ld(dp);
-            float ds[32];
-            if (KV) {
-                const float4* d4 = reinterpret_cast<const float4*>(sh.delta[st] + half * 64 + c * 32);
+            for (int e = 0; e < 32; ++e) dp[e] = (word >> e) & 1u ? dp[e] : 0u;
+        if (KV) {
+            const float4* d4 = reinterpret_cast<const float4*>(sh.delta[st] + quarter * 32);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float4 d = d4[e];
-                    const float de[4] = {d.x, d.y, d.z, d.w};
+            for (int e = 0; e < 8; ++e) {
+                const float4 d = d4[e];
+                const float de[4] = {d.x, d.y, d.z, d.w};
+                float ds[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        ds[4 * e + x] = __uint_as_float(pr[c][4 * e + x]) * ((__uint_as_float(dp[4 * e + x]) - de[x]) * a.scale);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    ds[e] = __uint_as_float(pr[c][e]) * ((__uint_as_float(dp[e]) - row_delta) * a.scale);
+                for (int x = 0; x < 4; ++x)
+                    ds[x] = __uint_as_float(pr[4 * e + x]) * ((__uint_as_float(dp[4 * e + x]) - de[x]) * a.scale);
+                pk[2 * e] = pack2(T(), ds[0], ds[1]);
+                pk[2 * e + 1] = pack2(T(), ds[2], ds[3]);
             }
-            // (a masked pair's dP may be NaN, and 0 * NaN is not 0)
-            if (masked)
+        } else {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) ds[e] = (word[c] >> e) & 1u ? ds[e] : 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pk[16 * c + e] = pack2(T(), ds[2 * e], ds[2 * e + 1]);
+            for (int e = 0; e < 16; ++e)
+                pk[e] = pack2(T(), __uint_as_float(pr[2 * e]) * ((__uint_as_float(dp[2 * e]) - row_delta) * a.scale),
+                              __uint_as_float(pr[2 * e + 1]) * ((__uint_as_float(dp[2 * e + 1]) - row_delta) * a.scale));
         }
-        tmem_st32(tp, pk);
+        tmem_st16(tp, pk);
         tmem_wait_st(pk);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.dsready);
     }
-    if (ok && wk.steps > 0) {
-        ok = mbar_wait_w(&sh.fin, 0, a.err, abort_flag, ERR_WAIT_ACC | (83 << 4));
+    if (pc.steps > 0) {
+        ok = mbar_wait_w(&sh.fin, fp, a.err, abort_flag, ERR_WAIT_ACC | (83 << 4));
+        if (!ok) return false;
+        fp ^= 1;
         tc_fence_after();
     }
-    // the sums: half 0 writes dv and half 1 dk, or each half its columns of dq
-    const int64_t at = static_cast<int64_t>(KV ? seq.k0 : seq.q0) + r;
-    T* dst = KV ? (half == 0 ? static_cast<T*>(a.dv) + at * a.dv_stride_t + wk.h * a.dv_stride_h
-                             : static_cast<T*>(a.dk) + at * a.dk_stride_t + wk.h * a.dk_stride_h)
-                : static_cast<T*>(a.dq) + at * a.dq_stride_t + wk.h * a.dq_stride_h;
-    const uint32_t acc = tmem + quad + (KV && half == 1 ? C::ACC1 : C::ACC0);
-    const bool zero = wk.steps == 0 || (!KV && row_lse == INFINITY);
-    constexpr int CHUNKS = DP / 32;
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        if (!KV && (c < CHUNKS / 2) != (half == 0)) continue;
-        uint32_t o[32];
-        if (wk.steps > 0 && ok) {
-            tmem_ld32(acc + 32 * c, o);
+    // the sums: quarters 0, 1 write dv and 2, 3 dk, half of the elements each, or each a quarter of dq's
+    constexpr int COLS = KV ? DP / 2 : DP / 4;
+    const int d0 = KV ? (quarter & 1) * COLS : quarter * COLS;
+    const uint32_t acc = lanes + (KV && quarter < 2 ? C::ACC0 : C::ACC1) + d0;
+    const int64_t at = static_cast<int64_t>(KV ? pc.seq.k0 : pc.seq.q0) + r;
+    T* dst = KV ? (quarter < 2 ? static_cast<T*>(a.dv) + at * a.dv_stride_t + pc.h * a.dv_stride_h
+                               : static_cast<T*>(a.dk) + at * a.dk_stride_t + pc.h * a.dk_stride_h)
+                : static_cast<T*>(a.dq) + at * a.dq_stride_t + pc.h * a.dq_stride_h;
+    const bool zero = pc.steps == 0 || (!KV && row_lse == INFINITY);
+#pragma unroll 1
+    for (int k = 0; k < COLS; k += 16) {
+        uint32_t o[16] = {};
+        if (pc.steps > 0) {
+            tmem_ld16(acc + k, o);
             tmem_wait_ld(o);
         }
-        if (ok && inside)
+        if (zero)
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-                if (32 * c + e < a.D) {
-                    float v[8];
+            for (int e = 0; e < 16; ++e) o[e] = 0u;
+        if (KV && pc.share >= 0) {
+            float* p = part + ((static_cast<size_t>(pc.share) * 2 + (quarter >> 1)) * AT_TILE + row) * DP + d0 + k;
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) v[x] = zero ? 0.0f : __uint_as_float(o[e + x]);
-                    store_f32(dst + 32 * c + e, v);
-                }
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<uint4*>(p + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else if (inside) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+                float v[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(o[e + x]);
+                if (d0 + k + e < a.D) store_f32(dst + d0 + k + e, v);
+            }
+        }
     }
+    if (pc.steps > 0) {                                          // the sums have been read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.aempty);
+    }
+    return true;
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(AB_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
-                const dn8_attention_bwd_args a, int kv_blocks) {
+                const dn8_attention_bwd_args a, const BwdPlan plan) {
     using C = BwdCfg<DP>;
+    static_assert(sizeof(BwdShared) <= 4096, "shared state");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sr = smem;                                  // R0, R1
@@ -261,189 +286,373 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     volatile int* abort_flag = &sh.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hk;
-    const bool kv = static_cast<int>(blockIdx.x) < kv_blocks;
-    const int idx = kv ? blockIdx.x : blockIdx.x - kv_blocks, heads = kv ? a.Hk : a.Hq;
-    if (warp == 8) {
-        const Sequence f = kv ? find_block<true>(a, idx / heads, 1, AT_TILE) : find_block<false>(a, idx / heads, 1, AT_TILE);
-        if (lane == 0) {
-            sh.seq = f;
-            mbar_init(&sh.rfull, 1);
-            mbar_init(&sh.fin, 1);
-            mbar_init(&sh.sfull, 1);
-            mbar_init(&sh.dpfull, 1);
-            mbar_init(&sh.pready, 8);
-            mbar_init(&sh.dsready, 8);
-            for (int s = 0; s < 3; ++s) {
-                mbar_init(&sh.xfull[s], 1);
-                mbar_init(&sh.xempty[s], 2);             // the last product and warp 10
-                mbar_init(&sh.xok[s], 1);
-            }
-            sh.abort = 0;
-            mbar_fence_init();
+    if (threadIdx.x == 512) {
+        mbar_init(&sh.answered, 1);
+        mbar_init(&sh.pfilled, 1);
+        mbar_init(&sh.pread, 19);
+        mbar_init(&sh.rfull, 1);
+        mbar_init(&sh.rempty, 1);
+        mbar_init(&sh.fin, 1);
+        mbar_init(&sh.aempty, 16);
+        mbar_init(&sh.dpfull, 1);
+        mbar_init(&sh.dsready, 16);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sh.sfull[s], 1);
+            mbar_init(&sh.pready[s], 16);
         }
-        __syncwarp();
+        for (int s = 0; s < 3; ++s) {
+            mbar_init(&sh.xfull[s], 1);
+            mbar_init(&sh.xempty[s], 1);
+            mbar_init(&sh.xok[s], 1);
+        }
+        sh.abort = 0;
+        mbar_fence_init();
     }
-    if (warp == 9) tmem_alloc(&sh.tmem, 512);
+    if (warp == 17) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const Sequence seq = sh.seq;
-    const int off = seq.nk - seq.nq;
     const int left = a.left < 0 ? ATT_FAR : a.left, right = a.right < 0 ? ATT_FAR : a.right;
-    BwdWalk wk;
-    wk.kv = kv;
-    wk.h = idx % heads;
-    wk.steps = wk.first = wk.r0 = 0;
-    wk.per = 1;
-    wk.keys.count = wk.keys.first = wk.keys.start = 0;
-    if (seq.b >= 0) {
-        if (kv) {
-            // first key tiles first: first tokens and open left sides make them the longest
-            wk.r0 = seq.blk * AT_TILE;
-            const int jl = min(wk.r0 + AT_TILE, seq.nk) - 1;
-            const int lo = max(0, wk.r0 - right - off), hi = wk.r0 < a.sinks ? seq.nq - 1 : min(seq.nq - 1, jl + left - off);
-            if (lo <= hi) {
-                wk.first = lo / AT_TILE;
-                wk.per = hi / AT_TILE - wk.first + 1;
-                wk.steps = wk.per * G;
-            }
-        } else {
-            wk.r0 = ((seq.nq - 1) / AT_TILE - seq.blk) * AT_TILE;
-            wk.keys = key_tiles(wk.r0 + off, min(wk.r0 + AT_TILE, seq.nq) - 1 + off, seq.nk, left, right, a.sinks, AT_TILE);
-            wk.steps = wk.keys.count;
-        }
-    }
-    // tile and head of step u
-    auto tile_of = [&](int u) -> int { return kv ? wk.first + u % wk.per : wk.keys.tile(u); };
-    auto head_of = [&](int u) -> int { return kv ? wk.h * G + u / wk.per : wk.h / G; };
+
+    // Piece n of this CTA: sh.piece[n % 2], from the moment it is filled until every warp has begun with the
+    // next one. Every warp but the last calls this for n = 0, 1, ... when it begins; false: there is
+    // none (or a wait gave up).
+    auto begin_piece = [&](int n) -> bool {
+        if (!mbar_wait_w(&sh.pfilled, n & 1, a.err, abort_flag, ERR_WAIT_FULL | (91 << 4))) return false;
+        if (lane == 0) mbar_arrive(&sh.pread);
+        return sh.piece[n & 1].seq.b >= 0;
+    };
     griddep_wait();                                      // delta and lse2
 
-    if (seq.b >= 0 && warp == 9) {
-        // ---------------- TMA ----------------
-        if (lane == 0 && wk.steps > 0) {
-            const int r0 = (kv ? seq.k0 : seq.q0) + wk.r0;
-            mbar_expect_tx(&sh.rfull, 2 * C::TILE);
-            load_tile<DP>(sr, kv ? &mk : &mq, &sh.rfull, wk.h, r0);
-            load_tile<DP>(sr + C::TILE, kv ? &mv : &mdo, &sh.rfull, wk.h, r0);
-            for (int u = 0; u < wk.steps; ++u) {
-                const int s = u % C::ST;
-                if (!mbar_wait(&sh.xempty[s], ((u / C::ST) & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (84 << 4))) break;
-                const int x0 = (kv ? seq.q0 : seq.k0) + tile_of(u) * AT_TILE, hx = head_of(u);
-                mbar_expect_tx(&sh.xfull[s], 2 * C::TILE);
-                load_tile<DP>(sx + 2 * s * C::TILE, kv ? &mq : &mk, &sh.xfull[s], hx, x0);
-                load_tile<DP>(sx + (2 * s + 1) * C::TILE, kv ? &mdo : &mv, &sh.xfull[s], hx, x0);
-            }
-        }
-        __syncwarp();
-    } else if (seq.b >= 0 && warp == 10) {
-        // ---------------- masked rows of the streamed tiles, statistics of the query rows ----------------
-        // Streamed rows are summed over: a row whose weights are all zero must not hold NaN.
-        for (int u = 0; u < wk.steps; ++u) {
-            const int s = u % C::ST, t0 = tile_of(u) * AT_TILE;
-            uint32_t word[4];
-            float l2[4], de[4];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int x = t0 + w * 32 + lane;
-                bool live;
-                if (kv) {
-                    l2[w] = INFINITY;
-                    de[w] = 0.0f;
-                    if (x < seq.nq) {
-                        const float* ws = static_cast<const float*>(a.work) + head_of(u) * a.Tq + seq.q0 + x;
-                        l2[w] = ws[0];
-                        de[w] = ws[a.Hq * a.Tq];
-                    }
-                    live = l2[w] != INFINITY;
-                } else {
-                    live = x < seq.nk && (a.keep == nullptr || a.keep[seq.k0 + x] != 0);
-                }
-                word[w] = __ballot_sync(0xffffffffu, live);
-            }
-            if (!mbar_wait_w(&sh.xfull[s], (u / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (85 << 4))) break;
-            const bool fix = (word[0] & word[1] & word[2] & word[3]) != 0xFFFFFFFFu;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if (kv) {
-                    sh.lse2[s][w * 32 + lane] = l2[w];
-                    sh.delta[s][w * 32 + lane] = de[w];
-                } else if (lane == w) {
-                    sh.words[s][w] = word[w];
-                }
-                if (fix && !((word[w] >> lane) & 1u)) {
-                    // X0, and for dk, dv X1 too (dout): the tiles that are right operands of a sum over rows
-                    const int blocks = (kv ? 2 : 1) * (DP / 64);
-                    for (int b = 0; b < blocks; ++b) {
-                        uint4* row = reinterpret_cast<uint4*>(sx + 2 * s * C::TILE + b * AT_BLOCK + (w * 32 + lane) * 128);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) row[c] = make_uint4(0u, 0u, 0u, 0u);
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AB_REGS_OTHER));
+        if (warp == 19) {
+            // ---------------- pieces ----------------
+            int block = blockIdx.x, asked = 0;
+            BwdPiece pc;
+            for (int n = 0;;) {
+                pc.seq.b = -2;
+                pc.steps = pc.begin = pc.first = 0;
+                pc.per = 1;
+                pc.share = -1;
+                pc.keys.count = pc.keys.first = pc.keys.start = 0;
+                if (block >= 0) {
+                    pc.kv = block < plan.kv_blocks;
+                    if (block < plan.split_blocks) {
+                        // share s of the walk over tile t of sequence b and key head h: block = ((b tiles + t) Hk + h)
+                        // shares + s
+                        const int s = block % plan.shares, x = block / plan.shares;
+                        pc.seq = sequence_of(a, x / a.Hk / plan.tiles);
+                        pc.seq.blk = x / a.Hk % plan.tiles;
+                        pc.h = x % a.Hk;
+                        pc.share = block;
+                        if (pc.seq.blk * AT_TILE >= pc.seq.nk) pc.seq.b = -1;
+                        pc.begin = s;
+                    } else if (pc.kv) {
+                        const int x = block - plan.split_blocks;
+                        pc.seq = find_block<true>(a, x / a.Hk, 1, AT_TILE);
+                        pc.h = x % a.Hk;
+                        if (plan.shares > 1 && pc.seq.blk < plan.tiles) pc.seq.b = -1;
+                    } else {
+                        const int x = block - plan.kv_blocks;
+                        pc.seq = find_block<false>(a, x / a.Hq, 1, AT_TILE);
+                        pc.h = x % a.Hq;
                     }
                 }
+                if (pc.seq.b >= 0) {
+                    const int off = pc.seq.nk - pc.seq.nq;
+                    if (pc.kv) {
+                        // first key tiles first: open left sides make them the longest
+                        pc.r0 = pc.seq.blk * AT_TILE;
+                        const int jl = min(pc.r0 + AT_TILE, pc.seq.nk) - 1;
+                        const int lo = max(0, pc.r0 - right - off);
+                        const int hi = pc.r0 < a.sinks ? pc.seq.nq - 1 : min(pc.seq.nq - 1, jl + left - off);
+                        if (lo <= hi) {
+                            pc.first = lo / AT_TILE;
+                            pc.per = hi / AT_TILE - pc.first + 1;
+                            pc.steps = pc.per * G;
+                        }
+                        if (pc.share >= 0) {             // steps [s n / shares, (s + 1) n / shares)
+                            const int s = pc.begin, n_ = pc.steps;
+                            pc.begin = static_cast<int>(static_cast<int64_t>(s) * n_ / plan.shares);
+                            pc.steps = static_cast<int>(static_cast<int64_t>(s + 1) * n_ / plan.shares) - pc.begin;
+                        }
+                    } else {
+                        pc.r0 = ((pc.seq.nq - 1) / AT_TILE - pc.seq.blk) * AT_TILE;
+                        pc.keys = key_tiles(pc.r0 + off, min(pc.r0 + AT_TILE, pc.seq.nq) - 1 + off, pc.seq.nk, left, right,
+                                            a.sinks, AT_TILE);
+                        pc.steps = pc.keys.count;
+                    }
+                }
+                if (pc.seq.b != -1) {                    // (-1: nothing there)
+                    if (lane == 0) {
+                        sh.piece[n & 1] = pc;
+                        mbar_arrive(&sh.pfilled);
+                    }
+                    if (pc.seq.b == -2) break;
+                    // (the row warps begin a piece last: one is known ahead, no more)
+                    if (!mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (92 << 4))) break;
+                    ++n;
+                }
+                if (lane == 0) {
+                    fence_async_smem();                  // the last answer has been read
+                    mbar_expect_tx(&sh.answered, 16);
+                    ask_for_block(sh.answer, &sh.answered);
+                }
+                if (!mbar_wait_w(&sh.answered, asked & 1, a.err, abort_flag, ERR_WAIT_FULL | (93 << 4))) break;
+                ++asked;
+                block = answered_block(sh.answer);
+                __syncwarp();
             }
-            if (fix) fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sh.xok[s]);
-                mbar_arrive(&sh.xempty[s]);
+        } else if (warp == 17) {
+            // ---------------- TMA ----------------
+            uint32_t c = 0, np = 0;
+            for (int n = 0; begin_piece(n); ++n) {
+                const BwdPiece& pc = sh.piece[n & 1];
+                if (pc.steps == 0) continue;
+                if (lane == 0) {
+                    const bool kv = pc.kv != 0;
+                    const int hk = kv ? pc.h : pc.h / G;
+                    bool ok = mbar_wait(&sh.rempty, (np & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (94 << 4));
+                    if (ok) {
+                        const int r0 = (kv ? pc.seq.k0 : pc.seq.q0) + pc.r0;
+                        mbar_expect_tx(&sh.rfull, 2 * C::TILE);
+                        load_tile<DP>(sr, kv ? &mk : &mq, &sh.rfull, pc.h, r0);
+                        load_tile<DP>(sr + C::TILE, kv ? &mv : &mdo, &sh.rfull, pc.h, r0);
+                    }
+                    for (int u = 0; ok && u < pc.steps; ++u, ++c) {
+                        const uint32_t s = c % C::ST;
+                        ok = mbar_wait(&sh.xempty[s], ((c / C::ST) & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (84 << 4));
+                        if (!ok) break;
+                        const int x0 = (kv ? pc.seq.q0 : pc.seq.k0) + pc.tile(u) * AT_TILE;
+                        const int hx = kv ? pc.h * G + pc.head(u) : hk;
+                        mbar_expect_tx(&sh.xfull[s], 2 * C::TILE);
+                        load_tile<DP>(sx + 2 * s * C::TILE, kv ? &mq : &mk, &sh.xfull[s], hx, x0);
+                        load_tile<DP>(sx + (2 * s + 1) * C::TILE, kv ? &mdo : &mv, &sh.xfull[s], hx, x0);
+                    }
+                }
+                ++np;
+                __syncwarp();
             }
-        }
-    } else if (seq.b >= 0 && warp == 8 && wk.steps > 0) {
-        // ---------------- tcgen05 issue ----------------
-        const uint32_t r0 = smem_u32(sr), r1 = r0 + C::TILE, x = smem_u32(sx);
-        auto wait_x = [&](int u) -> bool {
-            const int s = u % C::ST;
-            return mbar_wait_w(&sh.xfull[s], (u / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (86 << 4)) &&
-                   mbar_wait_w(&sh.xok[s], (u / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (87 << 4));
-        };
-        bool ok = mbar_wait_w(&sh.rfull, 0, a.err, abort_flag, ERR_WAIT_FULL | (88 << 4)) && wait_x(0);
-        if (ok) {
-            tc_fence_after();
-            mma_scores<T, DP>(tmem + C::S, r0, x);
-            umma_commit_w(&sh.sfull);
-            mma_scores<T, DP>(tmem + C::DPC, r1, x + C::TILE);
-            umma_commit_w(&sh.dpfull);
-        }
-        for (int u = 0; ok && u < wk.steps; ++u) {
-            const uint32_t x0 = x + 2 * (u % C::ST) * C::TILE, xn = x + 2 * ((u + 1) % C::ST) * C::TILE;
-            ok = mbar_wait_w(&sh.pready, u & 1, a.err, abort_flag, ERR_WAIT_ACC | (89 << 4));
-            if (!ok) break;
-            tc_fence_after();
-            if (kv) mma_values<T, DP>(tmem + C::ACC0, tmem + C::S, x0 + C::TILE, u > 0);
-            if (u + 1 < wk.steps) {
-                ok = wait_x(u + 1);
+        } else if (warp == 18) {
+            // ---------------- masked rows of the streamed tiles, statistics of the query rows ----------------
+            // Streamed rows are summed over: a row whose weights are all zero must not hold NaN.
+            uint32_t c = 0;
+            bool ok = true;
+            for (int n = 0; ok && begin_piece(n); ++n) {
+                const BwdPiece& pc = sh.piece[n & 1];
+                const bool kv = pc.kv != 0;
+                for (int u = 0; u < pc.steps; ++u, ++c) {
+                    const uint32_t s = c % C::ST;
+                    const int t0 = pc.tile(u) * AT_TILE;
+                    uint32_t word[4];
+                    float l2[4], de[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int x = t0 + w * 32 + lane;
+                        bool live;
+                        if (kv) {
+                            l2[w] = INFINITY;
+                            de[w] = 0.0f;
+                            if (x < pc.seq.nq) {
+                                const float* ws =
+                                    static_cast<const float*>(a.work) + (pc.h * G + pc.head(u)) * a.Tq + pc.seq.q0 + x;
+                                l2[w] = ws[0];
+                                de[w] = ws[a.Hq * a.Tq];
+                            }
+                            live = l2[w] != INFINITY;
+                        } else {
+                            live = x < pc.seq.nk && (a.keep == nullptr || a.keep[pc.seq.k0 + x] != 0);
+                        }
+                        word[w] = __ballot_sync(0xffffffffu, live);
+                    }
+                    ok = mbar_wait_w(&sh.xfull[s], (c / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (85 << 4));
+                    if (!ok) break;
+                    const bool fix = (word[0] & word[1] & word[2] & word[3]) != 0xFFFFFFFFu;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        if (kv) {
+                            sh.lse2[s][w * 32 + lane] = l2[w];
+                            sh.delta[s][w * 32 + lane] = de[w];
+                        } else if (lane == w) {
+                            sh.words[s][w] = word[w];
+                        }
+                        if (fix && !((word[w] >> lane) & 1u)) {
+                            // X0, and for dk, dv X1 too (dout): the right operands of sums over rows
+                            const int blocks = (kv ? 2 : 1) * (DP / 64);
+                            for (int b = 0; b < blocks; ++b) {
+                                uint4* row =
+                                    reinterpret_cast<uint4*>(sx + 2 * s * C::TILE + b * AT_BLOCK + (w * 32 + lane) * 128);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) row[k] = make_uint4(0u, 0u, 0u, 0u);
+                            }
+                        }
+                    }
+                    if (fix) fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.xok[s]);
+                }
+            }
+        } else {
+            // ---------------- tcgen05 issue (every value and branch uniform, see attn_umma.cuh) ----------------
+            const uint32_t r0 = uniform(smem_u32(sr)), x0 = uniform(smem_u32(sx)), tm = uniform(tmem);
+            uint32_t xs = 0, xp = 0, c = 0, np = 0;      // next stage to wait for and its phase; steps, pieces
+            bool ok = true;
+            auto wait_x = [&]() -> uint32_t {            // the next streamed pair's address
+                const uint32_t at = x0 + 2 * xs * C::TILE;
+                ok = mbar_wait_w(&sh.xfull[xs], xp, a.err, abort_flag, ERR_WAIT_FULL | (86 << 4)) &&
+                     mbar_wait_w(&sh.xok[xs], xp, a.err, abort_flag, ERR_WAIT_FULL | (87 << 4));
+                if (++xs == C::ST) {
+                    xs = 0;
+                    xp ^= 1;
+                }
+                return at;
+            };
+            for (int n = 0; vote(begin_piece(n)); ++n) {
+                const int steps = uniform(sh.piece[n & 1].steps);
+                const bool kv = vote(sh.piece[n & 1].kv != 0);
+                if (vote(steps == 0)) continue;
+                const bool two = !kv || DP == 64;        // two S tiles
+                ok = mbar_wait_w(&sh.rfull, np & 1, a.err, abort_flag, ERR_WAIT_FULL | (88 << 4));
+                if (!ok) break;
+                uint32_t st = xs, x = wait_x(), xn = 0;  // stage and address of step u's tiles
                 if (!ok) break;
                 tc_fence_after();
-                mma_scores<T, DP>(tmem + C::S, r0, xn);
-                umma_commit_w(&sh.sfull);
-            }
-            ok = mbar_wait_w(&sh.dsready, u & 1, a.err, abort_flag, ERR_WAIT_ACC | (90 << 4));
-            if (!ok) break;
-            tc_fence_after();
-            mma_values<T, DP>(tmem + (kv ? C::ACC1 : C::ACC0), tmem + C::DPC, x0, u > 0);
-            umma_commit_w(&sh.xempty[u % C::ST]);
-            if (u + 1 < wk.steps) {
-                mma_scores<T, DP>(tmem + C::DPC, r1, xn + C::TILE);
+                mma_scores<T, DP>(tm + C::S, r0, x);
+                umma_commit_w(&sh.sfull[0]);
+                mma_scores<T, DP>(tm + C::DPC, r0 + C::TILE, x + C::TILE);
                 umma_commit_w(&sh.dpfull);
+                for (int u = 0; vote(u < steps); ++u, ++c) {
+                    const bool more = vote(u + 1 < steps), first = vote(u == 0);
+                    const uint32_t sb = two && (u & 1) ? 1u : 0u, sn = two ? sb ^ 1u : 0u;
+                    // the last piece's sums have been read (with D > 64 dv's lie where dq has its second S tile)
+                    if (first) {
+                        ok = mbar_wait_w(&sh.aempty, (np & 1) ^ 1, a.err, abort_flag, ERR_WAIT_ACC | (95 << 4));
+                        if (!ok) break;
+                    }
+                    if (more && two) {
+                        // (its tile: P(u - 1), whose product was issued, or S(u - 1), which has been read)
+                        xn = wait_x();
+                        if (!ok) break;
+                        tc_fence_after();
+                        mma_scores<T, DP>(tm + C::S + sn * 128, r0, xn);
+                        umma_commit_w(&sh.sfull[sn]);
+                    }
+                    ok = mbar_wait_w(&sh.pready[c & 1], (c >> 1) & 1, a.err, abort_flag, ERR_WAIT_ACC | (89 << 4));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (kv) mma_values<T, DP, 32>(tm + C::ACC0, tm + C::S + sb * 128, x + C::TILE, !first);
+                    if (more && !two) {
+                        xn = wait_x();
+                        if (!ok) break;
+                        tc_fence_after();
+                        mma_scores<T, DP>(tm + C::S, r0, xn);
+                        umma_commit_w(&sh.sfull[0]);
+                    }
+                    ok = mbar_wait_w(&sh.dsready, c & 1, a.err, abort_flag, ERR_WAIT_ACC | (90 << 4));
+                    if (!ok) break;
+                    tc_fence_after();
+                    mma_values<T, DP, 32>(tm + C::ACC1, tm + C::DPC, x, !first);
+                    umma_commit_w(&sh.xempty[st]);
+                    if (more) {
+                        mma_scores<T, DP>(tm + C::DPC, r0 + C::TILE, xn + C::TILE);
+                        umma_commit_w(&sh.dpfull);
+                    }
+                    if (vote(u + 2 == steps || steps == 1)) umma_commit_w(&sh.rempty);    // no more products with R
+                    x = xn;
+                    if (++st == C::ST) st = 0;
+                }
+                if (!ok) break;
+                umma_commit_w(&sh.fin);
+                ++np;
             }
+            __syncwarp();
         }
-        if (ok) umma_commit_w(&sh.fin);
-        __syncwarp();
-    } else if (seq.b >= 0 && warp < 8) {
-        if (kv) bwd_rows<T, DP, true>(a, sh, wk, tmem);
-        else bwd_rows<T, DP, false>(a, sh, wk, tmem);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AB_REGS_ROWS));
+        uint32_t c = 0, sp = 0, fp = 0;
+        for (int n = 0; begin_piece(n); ++n) {
+            const BwdPiece& pc = sh.piece[n & 1];
+            if (!(pc.kv ? bwd_rows<T, DP, true>(a, sh, pc, plan.part, tmem, c, sp, fp)
+                        : bwd_rows<T, DP, false>(a, sh, pc, plan.part, tmem, c, sp, fp)))
+                break;
+        }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         tc_fence_after();
         tmem_free(tmem, 512);
     }
 }
 
-size_t attention_bwd_work(const dn8_attention_bwd_args& a) { return static_cast<size_t>(a.Tq) * a.Hq * 2 * sizeof(float); }
+// dk, dv of the first tokens' key tiles: the shares' sums, in order. One block per 16 rows of a tile and key
+// head; thread: 4 elements of a row.
+template <typename T, int DP>
+__global__ void __launch_bounds__(16 * (DP / 4)) attn_bwd_join_kernel(const dn8_attention_bwd_args a, const BwdPlan plan) {
+    const int x = blockIdx.x / (AT_TILE / 16), h = x % a.Hk, tile = x / a.Hk % plan.tiles, b = x / a.Hk / plan.tiles;
+    const int row = blockIdx.x % (AT_TILE / 16) * 16 + threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+    const int k0 = a.cu_k[b];
+    int nk = checked_len(k0, a.cu_k[b + 1], a.Tk, a.err);
+    if (a.len_k != nullptr) nk = checked_len(0, a.len_k[b], nk, a.err);
+    const int j = tile * AT_TILE + row;
+    griddep_wait();
+    if (j >= nk || d >= a.D) return;
+    const int64_t at = static_cast<int64_t>(k0) + j;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int y = 0; y < plan.shares; ++y) {
+            const float4 v = *reinterpret_cast<const float4*>(
+                plan.part + (((static_cast<size_t>(x) * plan.shares + y) * 2 + k) * AT_TILE + row) * DP + d);
+            s[0] += v.x;
+            s[1] += v.y;
+            s[2] += v.z;
+            s[3] += v.w;
+        }
+        T* dst = k == 0 ? static_cast<T*>(a.dv) + at * a.dv_stride_t + h * a.dv_stride_h
+                        : static_cast<T*>(a.dk) + at * a.dk_stride_t + h * a.dk_stride_h;
+        store_f32(dst + d, s);
+    }
+}
 
-template <typename T, int DP> static cudaError_t bwd_go(const dn8_attention_bwd_args& a, cudaStream_t st) {
+// Shares: under a window the tiles of the first tokens are walked over by all queries, the others by a few
+// tiles of them. They are cut when that makes them the longest by far, into as many shares as leave them
+// no longer than the others, or as fill the SMs.
+static BwdPlan bwd_plan(const dn8_attention_bwd_args& a, int sms) {
+    BwdPlan p = {};
+    p.shares = 1;
+    p.tiles = 1;
+    if (a.left >= 0 && a.sinks > 0 && a.Tk > 0 && a.Tq > 0) {
+        const int64_t G = a.Hq / a.Hk;
+        const int64_t tiles = (static_cast<int64_t>(a.sinks < a.Tk ? a.sinks : a.Tk) + AT_TILE - 1) / AT_TILE;
+        const int64_t all = G * (a.Tq / a.B / AT_TILE + 1);
+        const int64_t width = static_cast<int64_t>(a.left) + (a.right < 0 ? a.Tq / a.B : a.right) + AT_TILE;
+        const int64_t others = G * (width / AT_TILE + 1);
+        const int64_t walks = a.B * tiles * a.Hk;
+        int64_t s = (all + others - 1) / others;
+        const int64_t fill = (2ll * sms + walks - 1) / walks;
+        if (s > fill) s = fill;
+        if (s > 1 && all > 2 * others) {
+            p.tiles = static_cast<int>(tiles);
+            p.shares = static_cast<int>(s < 32 ? s : 32);
+            p.split_blocks = static_cast<int>(walks * p.shares);
+        }
+    }
+    return p;
+}
+static size_t bwd_stat_bytes(const dn8_attention_bwd_args& a) {
+    return (static_cast<size_t>(a.Tq) * a.Hq * 2 * sizeof(float) + 255) / 256 * 256;
+}
+
+size_t attention_bwd_work(const dn8_attention_bwd_args& a, int sms) {
+    const int DP = a.D <= 64 ? 64 : 128;
+    return bwd_stat_bytes(a) + static_cast<size_t>(bwd_plan(a, sms).split_blocks) * 2 * AT_TILE * DP * sizeof(float);
+}
+
+template <typename T, int DP> static cudaError_t bwd_go(const dn8_attention_bwd_args& a, int sms, cudaStream_t st) {
     CUtensorMap mq = {}, mk = {}, mv = {}, mdo = {};
     cudaError_t e = cudaSuccess;
     if (a.Tq > 0) {
@@ -457,22 +666,29 @@ template <typename T, int DP> static cudaError_t bwd_go(const dn8_attention_bwd_
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(attn_bwd_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdCfg<DP>::SMEM);
     if (e != cudaSuccess) return e;
+    BwdPlan plan = bwd_plan(a, sms);
     // bounds on the tiles: every sequence may leave one unfilled
-    const int64_t kt = (a.Tk / AT_TILE + (a.B < a.Tk ? a.B : a.Tk)) * a.Hk;
+    const int64_t kt = (a.Tk / AT_TILE + (a.B < a.Tk ? a.B : a.Tk)) * a.Hk + plan.split_blocks;
     const int64_t qt = (a.Tq / AT_TILE + (a.B < a.Tq ? a.B : a.Tq)) * a.Hq;
     if (kt + qt > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+    plan.kv_blocks = static_cast<int>(kt);
+    plan.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + bwd_stat_bytes(a));
     if (a.Tq > 0) {
         e = launch_pdl(false, attn_bwd_prep_kernel<T, DP / 8>, dim3(static_cast<unsigned>((a.Tq + 31) / 32), a.Hq),
                        dim3(32 * (DP / 8)), 0, st, a);
         if (e != cudaSuccess) return e;
     }
-    return launch_pdl(a.Tq > 0, attn_bwd_kernel<T, DP>, dim3(static_cast<unsigned>(kt + qt)), dim3(AB_THREADS),
-                      BwdCfg<DP>::SMEM, st, mq, mk, mv, mdo, a, static_cast<int>(kt));
+    e = launch_pdl(a.Tq > 0, attn_bwd_kernel<T, DP>, dim3(static_cast<unsigned>(kt + qt)), dim3(AB_THREADS),
+                   BwdCfg<DP>::SMEM, st, mq, mk, mv, mdo, a, plan);
+    if (e != cudaSuccess || plan.shares == 1) return e;
+    return launch_pdl(true, attn_bwd_join_kernel<T, DP>,
+                      dim3(static_cast<unsigned>(plan.split_blocks / plan.shares * (AT_TILE / 16))), dim3(16 * (DP / 4)), 0, st,
+                      a, plan);
 }
 
-cudaError_t launch_attention_bwd(const dn8_attention_bwd_args& a, cudaStream_t st) {
-    if (a.type == DN8_F16) return a.D <= 64 ? bwd_go<__half, 64>(a, st) : bwd_go<__half, 128>(a, st);
-    return a.D <= 64 ? bwd_go<__nv_bfloat16, 64>(a, st) : bwd_go<__nv_bfloat16, 128>(a, st);
+cudaError_t launch_attention_bwd(const dn8_attention_bwd_args& a, int sms, cudaStream_t st) {
+    if (a.type == DN8_F16) return a.D <= 64 ? bwd_go<__half, 64>(a, sms, st) : bwd_go<__half, 128>(a, sms, st);
+    return a.D <= 64 ? bwd_go<__nv_bfloat16, 64>(a, sms, st) : bwd_go<__nv_bfloat16, 128>(a, sms, st);
 }
 
 }  // namespace dn8

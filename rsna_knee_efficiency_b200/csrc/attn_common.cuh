@@ -28,6 +28,19 @@ DN8_DEV int checked_len(int s, int e, int64_t T, int* err) {
     if (err != nullptr) atomicCAS(err, 0, ERR_SHAPE);
     return 0;
 }
+// Sequence b (one thread or a whole warp).
+template <typename A> DN8_DEV Sequence sequence_of(const A& a, int b) {
+    Sequence s;
+    s.b = b;
+    s.blk = 0;
+    s.q0 = a.cu_q[b];
+    s.nq = checked_len(s.q0, a.cu_q[b + 1], a.Tq, a.err);
+    s.k0 = a.cu_k[b];
+    s.nk = checked_len(s.k0, a.cu_k[b + 1], a.Tk, a.err);
+    if (a.len_k != nullptr) s.nk = checked_len(0, a.len_k[b], s.nk, a.err);
+    return s;
+}
+
 // Block `unit` of the batch when every sequence is cut into ceil(len mul / per) blocks, len being its
 // queries (KEYS = false) or its keys. Called by one whole warp.
 template <bool KEYS, typename A> DN8_DEV Sequence find_block(const A& a, int unit, int mul, int per) {

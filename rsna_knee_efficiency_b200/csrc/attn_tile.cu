@@ -276,7 +276,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                                 op ^= 1u << g;
                             }
                             tc_fence_after();
-                            mma_values<T, DP>(tm + C::O0 + g * DP, tm + C::S0 + g * 128, vt, begun);
+                            mma_values<T, DP, 64>(tm + C::O0 + g * DP, tm + C::S0 + g * 128, vt, begun);
                             begun = true;
                         }
                         if (g ? now1 : now0) {

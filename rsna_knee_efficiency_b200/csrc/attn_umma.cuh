@@ -58,19 +58,20 @@ DN8_DEV void umma_f16_ss4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, ui
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// A from TMEM: 64 elements of a row in 32 columns, elements 2c and 2c + 1 in column c; B: 64 rows.
-DN8_DEV void umma_f16_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A from TMEM: 64 elements of a row, 16 in each 8 columns (elements 2c and 2c + 1 in column c) from a, a + 8,
+// a + STEP, a + STEP + 8 on; B: 64 rows.
+template <int STEP> DN8_DEV void umma_f16_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p, e, t;\n\t.reg .b32 l, a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
                  "setp.eq.b32 t, 0, 0;\n\t"
-                 "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+                 "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, %5;\n\tadd.s32 a3, %1, %6;\n\t"
                  "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
                  "elect.sync l|e, 0xffffffff;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(STEP), "n"(STEP + 8) : "memory");
 }
 // D[128 x 128] = A B^T over DP elements, both tiles in shared memory
 template <typename T, int DP> DN8_DEV void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
@@ -79,12 +80,13 @@ template <typename T, int DP> DN8_DEV void mma_scores(uint32_t d, uint32_t a, ui
         umma_f16_ss4(d, desc_rows(a, 4 * k), desc_rows(b, 4 * k), idesc_f16<T>(AT_TILE, AT_TILE, false), k > 0);
 }
 // D[128 x DP] (+)= A B, A [128 x 128] in TMEM, B a tile of 128 rows. A lies over the fp32 tile it was made
-// from: its columns 0-63 in the 32 TMEM columns at 0, 64-127 in those at 64, each half over the part that
-// the same threads have read.
-template <typename T, int DP> DN8_DEV void mma_values(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+// from: each PART columns of it in the first PART / 2 TMEM columns of their own, so that the threads that
+// read a part write over nothing else (PART = 64 or 32).
+template <typename T, int DP, int PART> DN8_DEV void mma_values(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-        umma_f16_ts4(d, a + 64 * k, desc_cols(b, 4 * k), idesc_f16<T>(AT_TILE, DP, true), accumulate || k > 0);
+        umma_f16_ts4<PART == 64 ? 16 : 32>(d, a + 64 * k, desc_cols(b, 4 * k), idesc_f16<T>(AT_TILE, DP, true),
+                                           accumulate || k > 0);
 }
 
 // One row per thread: 16 packed words (32 elements of 16 bits) to columns taddr ..

@@ -71,8 +71,8 @@ cudaError_t launch_rope(const dn8_rope_args& a, int sms, cudaStream_t st);
 cudaError_t launch_attention(const dn8_attention_args& a, int sms, cudaStream_t st);
 cudaError_t launch_attention_tile(const dn8_attention_args& a, cudaStream_t st);
 size_t attention_work(const dn8_attention_args& a, int sms);
-cudaError_t launch_attention_bwd(const dn8_attention_bwd_args& a, cudaStream_t st);
-size_t attention_bwd_work(const dn8_attention_bwd_args& a);
+cudaError_t launch_attention_bwd(const dn8_attention_bwd_args& a, int sms, cudaStream_t st);
+size_t attention_bwd_work(const dn8_attention_bwd_args& a, int sms);
 constexpr int DN8_MAX_DEVICES = 64;
 cudaError_t head_scratch_tickets(int32_t** out);
 
