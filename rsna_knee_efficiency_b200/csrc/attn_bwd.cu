@@ -54,12 +54,15 @@ constexpr int AB_THREADS = 640;             // warps 0-15: rows; 16: tcgen05 iss
 // The launch gives every thread 96 registers: 16 x 32 x 104 + 4 x 32 x 64 = 20 x 32 x 96.
 constexpr int AB_REGS_ROWS = 104, AB_REGS_OTHER = 64;
 template <int DP> struct BwdCfg {
-    static constexpr int ST = DP == 64 ? 3 : 2;
+    // Slots of the streamed tiles. X1 is done with early in a step (dP, dv), X0 at its end (dq, dk) and asked
+    // for again at the next one's start (S), so where memory is short X0 has the third slot.
+    static constexpr int N0 = 3, N1 = DP == 64 ? 3 : 2;
     static constexpr uint32_t TILE = AT_TILE * DP * 2;
-    static constexpr uint32_t SMEM = 1024 + TILE * 2 * (1 + ST) + 4096;
+    static constexpr uint32_t SMEM = TILE * (2 + N0 + N1) + 3072;
     // TMEM columns: dP, then S (one or two tiles), then the sums at the end
     static constexpr uint32_t DPC = 0, S = 128, ACC1 = 512 - DP, ACC0 = 512 - 2 * DP;
 };
+constexpr int AB_POLY = 3;                    // of 8 pairs of exponentials, those taken by polynomial
 // S tiles: the sums are dv (ACC0) and dk (ACC1), or dq (ACC1)
 template <int DP> DN8_DEV constexpr int s_tiles(bool kv) { return kv && DP == 128 ? 1 : 2; }
 
@@ -74,13 +77,13 @@ struct BwdPiece {
     int kv;                                   // dk, dv of a key tile, or dq of a query tile
     int r0;                                   // first resident row, within the sequence
     int h;                                    // key head (kv) or query head
-    int begin, steps;                         // kv: the share's first step of the tile's walk; steps
-    int first, per;                           // kv: first query tile and query tiles per head
+    int steps;
     int share;                                // kv: where a share's sums go, or -1: straight to dk, dv
-    KeyTiles keys;                            // dq: key tiles
-    // query or key tile of step u, and for dk, dv the head within the group
-    DN8_DEV int tile(int u) const { return kv ? first + (begin + u) % per : keys.tile(u); }
-    DN8_DEV int head(int u) const { return kv ? (begin + u) / per : 0; }
+    // Streamed tiles: `tile0`, then one after the other; after `turn` comes `back` (dk, dv: the next head's first
+    // tile; dq: from the first tokens' tiles to the window's). hx: the first step's head.
+    int tile0, turn, back, hx;
+    // A step whose first column is above `hic`, or below `loc` but above `skc`, or every step, needs a mask.
+    int always, hic, loc, skc;
 };
 struct BwdShared {
     uint64_t answer[2];
@@ -88,12 +91,12 @@ struct BwdShared {
     // (of even and odd steps: the rows may be done with S(u + 1), where there are two S tiles, before the
     // issuing warp, held up by its own queue, has looked for S(u))
     uint64_t pready[2];
-    uint64_t sfull[2], xfull[3], xempty[3], xok[3];
+    uint64_t sfull[2], x0full[3], x0empty[3], x0ok[3], x1full[3], x1empty[3], x1ok[3], sempty[2];
     BwdPiece piece[2];
-    uint32_t words[3][4];
+    uint32_t words[2][4];                     // of even and odd steps, as the statistics
     uint32_t tmem;
     int abort;
-    alignas(16) float lse2[3][AT_TILE], delta[3][AT_TILE];
+    alignas(16) float lse2[2][AT_TILE], delta[2][AT_TILE];
 };
 
 // The 16 row warps on one piece: warp w has the TMEM lanes (resident rows) 32 (w % 4) .. and the columns
@@ -120,29 +123,27 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
         row_delta = w[a.Hq * a.Tq];
     }
     bool ok = true;
-    for (int u = 0; u < pc.steps; ++u, ++c) {
-        const uint32_t st = c % C::ST;
-        const int off = pc.seq.nk - pc.seq.nq, c0 = pc.tile(u) * AT_TILE, cl = c0 + AT_TILE - 1;
-        const int rlast = min(pc.r0 + AT_TILE, KV ? pc.seq.nk : pc.seq.nq) - 1;
-        ok = mbar_wait_w(&sh.xok[st], (c / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (80 << 4));
+    const int steps = pc.steps, turn = pc.turn, hic = pc.hic, loc = pc.loc, skc = pc.skc;
+    const bool always = pc.always != 0;
+    int tile = pc.tile0;
+    for (int u = 0; u < steps; ++u, ++c) {
+        const int c0 = tile * AT_TILE;
+        tile = tile == turn ? pc.back : tile + 1;
+        const uint32_t sx = c & 1;
+        ok = mbar_wait_w(&sh.x0ok[c % C::N0], (c / C::N0) & 1, a.err, abort_flag, ERR_WAIT_FULL | (80 << 4));
         if (!ok) return false;
         uint32_t word = 0xFFFFFFFFu;
-        bool masked;
-        if (KV) {
-            // columns are queries: seen from j - right - off on, up to j + left - off (first tokens: by all).
-            // Queries behind the end are zero rows with lse2 = inf.
-            masked = a.keep != nullptr || pc.r0 + AT_TILE > pc.seq.nk || c0 + off < rlast - right ||
-                     (cl + off > pc.r0 + left && rlast >= a.sinks);
-            if (masked) {
+        const bool masked = always || c0 > hic || (c0 < loc && c0 > skc);
+        if (masked) {
+            const int off = pc.seq.nk - pc.seq.nq;
+            if (KV) {
+                // columns are queries: seen from j - right - off on, up to j + left - off (first tokens: by all).
+                // Queries behind the end are zero rows with lse2 = inf.
                 const int lo = r - right - off - c0, hi = r < a.sinks ? ATT_FAR : r + left - off - c0;
                 word = keep ? bits_from(lo, quarter) & bits_upto(hi, quarter) : 0u;
-            }
-        } else {
-            masked = a.keep != nullptr || cl > min(pc.seq.nk - 1, pc.r0 + off + right) ||
-                     (c0 < rlast + off - left && cl >= a.sinks);
-            if (masked) {
+            } else {
                 const int p = r + off, hi = min(pc.seq.nk - 1, p + right) - c0, lo = p - left - c0;
-                word = bits_upto(hi, quarter) & sh.words[st][quarter] &
+                word = bits_upto(hi, quarter) & sh.words[sx][quarter] &
                        (bits_from(lo, quarter) | bits_upto(a.sinks - 1 - c0, quarter));
             }
         }
@@ -160,19 +161,18 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.pready[c & 1]);
         }
-        if (KV) {
-            const float4* l4 = reinterpret_cast<const float4*>(sh.lse2[st] + quarter * 32);
+        const float2 sc2 = f2_pack(sc, sc);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float4 l = l4[e];
-                const float ls[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    pr[4 * e + x] = __float_as_uint(ex2(fmaf(__uint_as_float(pr[4 * e + x]), sc, -ls[x])));
+        for (int e = 0; e < 16; ++e) {
+            float2 l = f2_pack(-row_lse, -row_lse);
+            if (KV) {
+                l = *reinterpret_cast<const float2*>(sh.lse2[sx] + quarter * 32 + 2 * e);
+                l = f2_pack(-l.x, -l.y);
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) pr[e] = __float_as_uint(ex2(fmaf(__uint_as_float(pr[e]), sc, -row_lse)));
+            const float2 x = ex2_pair<AB_POLY>(
+                f2_fma(f2_pack(__uint_as_float(pr[2 * e]), __uint_as_float(pr[2 * e + 1])), sc2, l), e);
+            pr[2 * e] = __float_as_uint(x.x);
+            pr[2 * e + 1] = __float_as_uint(x.y);
         }
         if (masked)
 #pragma unroll
@@ -199,7 +199,7 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
 #pragma unroll
             for (int e = 0; e < 32; ++e) dp[e] = (word >> e) & 1u ? dp[e] : 0u;
         if (KV) {
-            const float4* d4 = reinterpret_cast<const float4*>(sh.delta[st] + quarter * 32);
+            const float4* d4 = reinterpret_cast<const float4*>(sh.delta[sx] + quarter * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float4 d = d4[e];
@@ -221,9 +221,12 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
         tmem_wait_st(pk);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.dsready);
+        if (lane == 0) {
+            mbar_arrive(&sh.dsready);
+            mbar_arrive(&sh.sempty[sx]);
+        }
     }
-    if (pc.steps > 0) {
+    if (steps > 0) {
         ok = mbar_wait_w(&sh.fin, fp, a.err, abort_flag, ERR_WAIT_ACC | (83 << 4));
         if (!ok) return false;
         fp ^= 1;
@@ -237,11 +240,11 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
     T* dst = KV ? (quarter < 2 ? static_cast<T*>(a.dv) + at * a.dv_stride_t + pc.h * a.dv_stride_h
                                : static_cast<T*>(a.dk) + at * a.dk_stride_t + pc.h * a.dk_stride_h)
                 : static_cast<T*>(a.dq) + at * a.dq_stride_t + pc.h * a.dq_stride_h;
-    const bool zero = pc.steps == 0 || (!KV && row_lse == INFINITY);
+    const bool zero = steps == 0 || (!KV && row_lse == INFINITY);
 #pragma unroll 1
     for (int k = 0; k < COLS; k += 16) {
         uint32_t o[16] = {};
-        if (pc.steps > 0) {
+        if (steps > 0) {
             tmem_ld16(acc + k, o);
             tmem_wait_ld(o);
         }
@@ -263,7 +266,7 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
             }
         }
     }
-    if (pc.steps > 0) {                                          // the sums have been read
+    if (steps > 0) {                                             // the sums have been read
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.aempty);
@@ -277,15 +280,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
                 const dn8_attention_bwd_args a, const BwdPlan plan) {
     using C = BwdCfg<DP>;
-    static_assert(sizeof(BwdShared) <= 4096, "shared state");
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    static_assert(sizeof(BwdShared) <= 3072, "shared state");
+    extern __shared__ __align__(1024) uint8_t smem[];    // (no static shared memory, so it starts aligned)
     uint8_t* sr = smem;                                  // R0, R1
-    uint8_t* sx = smem + 2 * C::TILE;                    // stages of X0, X1
-    BwdShared& sh = *reinterpret_cast<BwdShared*>(sx + 2 * C::ST * C::TILE);
+    uint8_t* sx0 = smem + 2 * C::TILE;                   // slots of X0
+    uint8_t* sx1 = sx0 + C::N0 * C::TILE;                // slots of X1
+    BwdShared& sh = *reinterpret_cast<BwdShared*>(sx1 + C::N1 * C::TILE);
     volatile int* abort_flag = &sh.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hk;
+    if (smem_u32(smem) & 1023u) {                        // the tiles' swizzle needs it; never seen
+        if (threadIdx.x == 0 && a.err != nullptr) atomicCAS(a.err, 0, ERR_SHAPE);
+        return;
+    }
     if (threadIdx.x == 512) {
         mbar_init(&sh.answered, 1);
         mbar_init(&sh.pfilled, 1);
@@ -299,11 +306,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sh.sfull[s], 1);
             mbar_init(&sh.pready[s], 16);
+            mbar_init(&sh.sempty[s], 16);
         }
         for (int s = 0; s < 3; ++s) {
-            mbar_init(&sh.xfull[s], 1);
-            mbar_init(&sh.xempty[s], 1);
-            mbar_init(&sh.xok[s], 1);
+            mbar_init(&sh.x0full[s], 1);
+            mbar_init(&sh.x0empty[s], 1);
+            mbar_init(&sh.x0ok[s], 1);
+            mbar_init(&sh.x1full[s], 1);
+            mbar_init(&sh.x1empty[s], 1);
+            mbar_init(&sh.x1ok[s], 1);
         }
         sh.abort = 0;
         mbar_fence_init();
@@ -333,10 +344,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             BwdPiece pc;
             for (int n = 0;;) {
                 pc.seq.b = -2;
-                pc.steps = pc.begin = pc.first = 0;
-                pc.per = 1;
-                pc.share = -1;
-                pc.keys.count = pc.keys.first = pc.keys.start = 0;
+                pc.steps = pc.tile0 = pc.hx = 0;
+                pc.turn = pc.back = pc.share = -1;
+                int begin = 0;                           // which share
                 if (block >= 0) {
                     pc.kv = block < plan.kv_blocks;
                     if (block < plan.split_blocks) {
@@ -348,7 +358,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                         pc.h = x % a.Hk;
                         pc.share = block;
                         if (pc.seq.blk * AT_TILE >= pc.seq.nk) pc.seq.b = -1;
-                        pc.begin = s;
+                        begin = s;
                     } else if (pc.kv) {
                         const int x = block - plan.split_blocks;
                         pc.seq = find_block<true>(a, x / a.Hk, 1, AT_TILE);
@@ -361,28 +371,41 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     }
                 }
                 if (pc.seq.b >= 0) {
-                    const int off = pc.seq.nk - pc.seq.nq;
+                    const int nq = pc.seq.nq, nk = pc.seq.nk, off = nk - nq;
                     if (pc.kv) {
                         // first key tiles first: open left sides make them the longest
                         pc.r0 = pc.seq.blk * AT_TILE;
-                        const int jl = min(pc.r0 + AT_TILE, pc.seq.nk) - 1;
+                        const int jl = min(pc.r0 + AT_TILE, nk) - 1;
                         const int lo = max(0, pc.r0 - right - off);
-                        const int hi = pc.r0 < a.sinks ? pc.seq.nq - 1 : min(pc.seq.nq - 1, jl + left - off);
-                        if (lo <= hi) {
-                            pc.first = lo / AT_TILE;
-                            pc.per = hi / AT_TILE - pc.first + 1;
-                            pc.steps = pc.per * G;
-                        }
+                        const int hi = pc.r0 < a.sinks ? nq - 1 : min(nq - 1, jl + left - off);
+                        const int first = lo / AT_TILE, per = lo <= hi ? hi / AT_TILE - first + 1 : 1;
+                        pc.steps = lo <= hi ? per * G : 0;
                         if (pc.share >= 0) {             // steps [s n / shares, (s + 1) n / shares)
-                            const int s = pc.begin, n_ = pc.steps;
-                            pc.begin = static_cast<int>(static_cast<int64_t>(s) * n_ / plan.shares);
-                            pc.steps = static_cast<int>(static_cast<int64_t>(s + 1) * n_ / plan.shares) - pc.begin;
+                            const int s = begin, n_ = pc.steps;
+                            begin = static_cast<int>(static_cast<int64_t>(s) * n_ / plan.shares);
+                            pc.steps = static_cast<int>(static_cast<int64_t>(s + 1) * n_ / plan.shares) - begin;
                         }
+                        pc.tile0 = first + begin % per;
+                        pc.hx = pc.h * G + begin / per;
+                        pc.turn = first + per - 1;
+                        pc.back = first;
+                        pc.always = a.keep != nullptr || pc.r0 + AT_TILE > nk;
+                        pc.loc = jl - right - off;
+                        pc.skc = -1;
+                        pc.hic = jl < a.sinks ? ATT_FAR : pc.r0 + left - off - (AT_TILE - 1);
                     } else {
-                        pc.r0 = ((pc.seq.nq - 1) / AT_TILE - pc.seq.blk) * AT_TILE;
-                        pc.keys = key_tiles(pc.r0 + off, min(pc.r0 + AT_TILE, pc.seq.nq) - 1 + off, pc.seq.nk, left, right,
-                                            a.sinks, AT_TILE);
-                        pc.steps = pc.keys.count;
+                        pc.r0 = ((nq - 1) / AT_TILE - pc.seq.blk) * AT_TILE;
+                        const int il = min(pc.r0 + AT_TILE, nq) - 1;
+                        const KeyTiles k = key_tiles(pc.r0 + off, il + off, nk, left, right, a.sinks, AT_TILE);
+                        pc.steps = k.count;
+                        pc.tile0 = k.tile(0);
+                        pc.hx = pc.h / G;
+                        pc.turn = k.first - 1;
+                        pc.back = k.start;
+                        pc.always = a.keep != nullptr;
+                        pc.hic = min(nk - 1, pc.r0 + off + right) - (AT_TILE - 1);
+                        pc.loc = il + off - left;
+                        pc.skc = a.sinks - AT_TILE;
                     }
                 }
                 if (pc.seq.b != -1) {                    // (-1: nothing there)
@@ -413,7 +436,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 if (pc.steps == 0) continue;
                 if (lane == 0) {
                     const bool kv = pc.kv != 0;
-                    const int hk = kv ? pc.h : pc.h / G;
                     bool ok = mbar_wait(&sh.rempty, (np & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (94 << 4));
                     if (ok) {
                         const int r0 = (kv ? pc.seq.k0 : pc.seq.q0) + pc.r0;
@@ -421,15 +443,24 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                         load_tile<DP>(sr, kv ? &mk : &mq, &sh.rfull, pc.h, r0);
                         load_tile<DP>(sr + C::TILE, kv ? &mv : &mdo, &sh.rfull, pc.h, r0);
                     }
+                    int tile = pc.tile0, hx = pc.hx;
                     for (int u = 0; ok && u < pc.steps; ++u, ++c) {
-                        const uint32_t s = c % C::ST;
-                        ok = mbar_wait(&sh.xempty[s], ((c / C::ST) & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (84 << 4));
+                        const uint32_t s0 = c % C::N0, s1 = c % C::N1;
+                        const int x0 = (kv ? pc.seq.q0 : pc.seq.k0) + tile * AT_TILE;
+                        ok = mbar_wait(&sh.x0empty[s0], ((c / C::N0) & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (84 << 4));
                         if (!ok) break;
-                        const int x0 = (kv ? pc.seq.q0 : pc.seq.k0) + pc.tile(u) * AT_TILE;
-                        const int hx = kv ? pc.h * G + pc.head(u) : hk;
-                        mbar_expect_tx(&sh.xfull[s], 2 * C::TILE);
-                        load_tile<DP>(sx + 2 * s * C::TILE, kv ? &mq : &mk, &sh.xfull[s], hx, x0);
-                        load_tile<DP>(sx + (2 * s + 1) * C::TILE, kv ? &mdo : &mv, &sh.xfull[s], hx, x0);
+                        mbar_expect_tx(&sh.x0full[s0], C::TILE);
+                        load_tile<DP>(sx0 + s0 * C::TILE, kv ? &mq : &mk, &sh.x0full[s0], hx, x0);
+                        ok = mbar_wait(&sh.x1empty[s1], ((c / C::N1) & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (96 << 4));
+                        if (!ok) break;
+                        mbar_expect_tx(&sh.x1full[s1], C::TILE);
+                        load_tile<DP>(sx1 + s1 * C::TILE, kv ? &mdo : &mv, &sh.x1full[s1], hx, x0);
+                        if (tile == pc.turn) {
+                            tile = pc.back;
+                            hx += kv ? 1 : 0;
+                        } else {
+                            ++tile;
+                        }
                     }
                 }
                 ++np;
@@ -437,77 +468,105 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             }
         } else if (warp == 18) {
             // ---------------- masked rows of the streamed tiles, statistics of the query rows ----------------
-            // Streamed rows are summed over: a row whose weights are all zero must not hold NaN.
+            // Streamed rows are summed over: a row whose weights are all zero must not hold NaN. The next step's
+            // statistics are on their way while this one's tiles are waited for.
             uint32_t c = 0;
             bool ok = true;
             for (int n = 0; ok && begin_piece(n); ++n) {
                 const BwdPiece& pc = sh.piece[n & 1];
                 const bool kv = pc.kv != 0;
-                for (int u = 0; u < pc.steps; ++u, ++c) {
-                    const uint32_t s = c % C::ST;
-                    const int t0 = pc.tile(u) * AT_TILE;
+                const int steps = pc.steps, q0 = pc.seq.q0, nq = pc.seq.nq, nk = pc.seq.nk;
+                int tile = pc.tile0, hx = pc.hx;
+                float l2[4], de[4];
+                bool live[4];
+                auto fetch = [&]() {                     // of the step that `tile` and `hx` stand at
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int x = tile * AT_TILE + w * 32 + lane;
+                        l2[w] = INFINITY;
+                        de[w] = 0.0f;
+                        live[w] = true;
+                        if (kv && x < nq) {
+                            const float* ws = static_cast<const float*>(a.work) + static_cast<int64_t>(hx) * a.Tq + q0 + x;
+                            l2[w] = ws[0];
+                            de[w] = ws[a.Hq * a.Tq];
+                        }
+                        if (!kv) live[w] = x < nk && (a.keep == nullptr || a.keep[pc.seq.k0 + x] != 0);
+                    }
+                    if (tile == pc.turn) {
+                        tile = pc.back;
+                        hx += kv ? 1 : 0;
+                    } else {
+                        ++tile;
+                    }
+                };
+                if (steps > 0) fetch();
+                for (int u = 0; u < steps; ++u, ++c) {
+                    const uint32_t s0 = c % C::N0, s1 = c % C::N1, sx = c & 1;
                     uint32_t word[4];
-                    float l2[4], de[4];
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int x = t0 + w * 32 + lane;
-                        bool live;
-                        if (kv) {
-                            l2[w] = INFINITY;
-                            de[w] = 0.0f;
-                            if (x < pc.seq.nq) {
-                                const float* ws =
-                                    static_cast<const float*>(a.work) + (pc.h * G + pc.head(u)) * a.Tq + pc.seq.q0 + x;
-                                l2[w] = ws[0];
-                                de[w] = ws[a.Hq * a.Tq];
-                            }
-                            live = l2[w] != INFINITY;
-                        } else {
-                            live = x < pc.seq.nk && (a.keep == nullptr || a.keep[pc.seq.k0 + x] != 0);
-                        }
-                        word[w] = __ballot_sync(0xffffffffu, live);
-                    }
-                    ok = mbar_wait_w(&sh.xfull[s], (c / C::ST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (85 << 4));
+                    // (the step before the last has been read)
+                    ok = mbar_wait_w(&sh.sempty[sx], ((c >> 1) & 1) ^ 1, a.err, abort_flag, ERR_WAIT_EMPTY | (97 << 4));
                     if (!ok) break;
-                    const bool fix = (word[0] & word[1] & word[2] & word[3]) != 0xFFFFFFFFu;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
+                        word[w] = __ballot_sync(0xffffffffu, kv ? l2[w] != INFINITY : live[w]);
                         if (kv) {
-                            sh.lse2[s][w * 32 + lane] = l2[w];
-                            sh.delta[s][w * 32 + lane] = de[w];
+                            sh.lse2[sx][w * 32 + lane] = l2[w];
+                            sh.delta[sx][w * 32 + lane] = de[w];
                         } else if (lane == w) {
-                            sh.words[s][w] = word[w];
-                        }
-                        if (fix && !((word[w] >> lane) & 1u)) {
-                            // X0, and for dk, dv X1 too (dout): the right operands of sums over rows
-                            const int blocks = (kv ? 2 : 1) * (DP / 64);
-                            for (int b = 0; b < blocks; ++b) {
-                                uint4* row =
-                                    reinterpret_cast<uint4*>(sx + 2 * s * C::TILE + b * AT_BLOCK + (w * 32 + lane) * 128);
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) row[k] = make_uint4(0u, 0u, 0u, 0u);
-                            }
+                            sh.words[sx][w] = word[w];
                         }
                     }
-                    if (fix) fence_async_smem();
+                    if (u + 1 < steps) fetch();
+                    const bool fix = (word[0] & word[1] & word[2] & word[3]) != 0xFFFFFFFFu;
+                    auto zero_rows = [&](uint8_t* x) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            if (!((word[w] >> lane) & 1u))
+                                for (int b = 0; b < DP / 64; ++b) {
+                                    uint4* row = reinterpret_cast<uint4*>(x + b * AT_BLOCK + (w * 32 + lane) * 128);
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) row[k] = make_uint4(0u, 0u, 0u, 0u);
+                                }
+                        fence_async_smem();
+                    };
+                    ok = mbar_wait_w(&sh.x0full[s0], (c / C::N0) & 1, a.err, abort_flag, ERR_WAIT_FULL | (85 << 4));
+                    if (!ok) break;
+                    if (fix) zero_rows(sx0 + s0 * C::TILE);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.xok[s]);
+                    if (lane == 0) mbar_arrive(&sh.x0ok[s0]);
+                    ok = mbar_wait_w(&sh.x1full[s1], (c / C::N1) & 1, a.err, abort_flag, ERR_WAIT_FULL | (98 << 4));
+                    if (!ok) break;
+                    if (fix && kv) zero_rows(sx1 + s1 * C::TILE);      // (dq: V's rows meet no sum over rows)
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.x1ok[s1]);
                 }
             }
         } else {
             // ---------------- tcgen05 issue (every value and branch uniform, see attn_umma.cuh) ----------------
-            const uint32_t r0 = uniform(smem_u32(sr)), x0 = uniform(smem_u32(sx)), tm = uniform(tmem);
-            uint32_t xs = 0, xp = 0, c = 0, np = 0;      // next stage to wait for and its phase; steps, pieces
+            const uint32_t r0 = uniform(smem_u32(sr)), x0b = uniform(smem_u32(sx0)), x1b = uniform(smem_u32(sx1));
+            const uint32_t tm = uniform(tmem);
+            uint32_t s0 = 0, p0 = 0, s1 = 0, p1 = 0;     // the slots of the next tiles to wait for, their phases
+            uint32_t c = 0, np = 0;                      // steps and pieces so far
             bool ok = true;
-            auto wait_x = [&]() -> uint32_t {            // the next streamed pair's address
-                const uint32_t at = x0 + 2 * xs * C::TILE;
-                ok = mbar_wait_w(&sh.xfull[xs], xp, a.err, abort_flag, ERR_WAIT_FULL | (86 << 4)) &&
-                     mbar_wait_w(&sh.xok[xs], xp, a.err, abort_flag, ERR_WAIT_FULL | (87 << 4));
-                if (++xs == C::ST) {
-                    xs = 0;
-                    xp ^= 1;
+            // (x0ok and x1ok come after the tiles' own barriers)
+            auto wait_x0 = [&]() -> uint32_t {
+                const uint32_t s = s0;
+                ok = mbar_wait_w(&sh.x0ok[s], p0, a.err, abort_flag, ERR_WAIT_FULL | (86 << 4));
+                if (++s0 == C::N0) {
+                    s0 = 0;
+                    p0 ^= 1;
                 }
-                return at;
+                return s;
+            };
+            auto wait_x1 = [&]() -> uint32_t {
+                const uint32_t s = s1;
+                ok = mbar_wait_w(&sh.x1ok[s], p1, a.err, abort_flag, ERR_WAIT_FULL | (87 << 4));
+                if (++s1 == C::N1) {
+                    s1 = 0;
+                    p1 ^= 1;
+                }
+                return s;
             };
             for (int n = 0; vote(begin_piece(n)); ++n) {
                 const int steps = uniform(sh.piece[n & 1].steps);
@@ -516,13 +575,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 const bool two = !kv || DP == 64;        // two S tiles
                 ok = mbar_wait_w(&sh.rfull, np & 1, a.err, abort_flag, ERR_WAIT_FULL | (88 << 4));
                 if (!ok) break;
-                uint32_t st = xs, x = wait_x(), xn = 0;  // stage and address of step u's tiles
+                uint32_t x0 = wait_x0(), x0n = 0;        // slots of step u and of step u + 1
                 if (!ok) break;
                 tc_fence_after();
-                mma_scores<T, DP>(tm + C::S, r0, x);
+                mma_scores<T, DP>(tm + C::S, r0, x0b + x0 * C::TILE);
                 umma_commit_w(&sh.sfull[0]);
-                mma_scores<T, DP>(tm + C::DPC, r0 + C::TILE, x + C::TILE);
+                uint32_t x1 = wait_x1();
+                if (!ok) break;
+                tc_fence_after();
+                mma_scores<T, DP>(tm + C::DPC, r0 + C::TILE, x1b + x1 * C::TILE);
                 umma_commit_w(&sh.dpfull);
+                if (!kv) umma_commit_w(&sh.x1empty[x1]);
+                if (vote(steps == 1)) umma_commit_w(&sh.rempty);
                 for (int u = 0; vote(u < steps); ++u, ++c) {
                     const bool more = vote(u + 1 < steps), first = vote(u == 0);
                     const uint32_t sb = two && (u & 1) ? 1u : 0u, sn = two ? sb ^ 1u : 0u;
@@ -533,35 +597,42 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     }
                     if (more && two) {
                         // (its tile: P(u - 1), whose product was issued, or S(u - 1), which has been read)
-                        xn = wait_x();
+                        x0n = wait_x0();
                         if (!ok) break;
                         tc_fence_after();
-                        mma_scores<T, DP>(tm + C::S + sn * 128, r0, xn);
+                        mma_scores<T, DP>(tm + C::S + sn * 128, r0, x0b + x0n * C::TILE);
                         umma_commit_w(&sh.sfull[sn]);
                     }
                     ok = mbar_wait_w(&sh.pready[c & 1], (c >> 1) & 1, a.err, abort_flag, ERR_WAIT_ACC | (89 << 4));
                     if (!ok) break;
-                    tc_fence_after();
-                    if (kv) mma_values<T, DP, 32>(tm + C::ACC0, tm + C::S + sb * 128, x + C::TILE, !first);
+                    if (kv) {
+                        tc_fence_after();
+                        mma_values<T, DP, 32>(tm + C::ACC0, tm + C::S + sb * 128, x1b + x1 * C::TILE, !first);
+                        umma_commit_w(&sh.x1empty[x1]);
+                    }
                     if (more && !two) {
-                        xn = wait_x();
+                        x0n = wait_x0();
                         if (!ok) break;
                         tc_fence_after();
-                        mma_scores<T, DP>(tm + C::S, r0, xn);
+                        mma_scores<T, DP>(tm + C::S, r0, x0b + x0n * C::TILE);
                         umma_commit_w(&sh.sfull[0]);
+                    }
+                    if (more) {
+                        x1 = wait_x1();
+                        if (!ok) break;
                     }
                     ok = mbar_wait_w(&sh.dsready, c & 1, a.err, abort_flag, ERR_WAIT_ACC | (90 << 4));
                     if (!ok) break;
                     tc_fence_after();
-                    mma_values<T, DP, 32>(tm + C::ACC1, tm + C::DPC, x, !first);
-                    umma_commit_w(&sh.xempty[st]);
+                    mma_values<T, DP, 32>(tm + C::ACC1, tm + C::DPC, x0b + x0 * C::TILE, !first);
                     if (more) {
-                        mma_scores<T, DP>(tm + C::DPC, r0 + C::TILE, xn + C::TILE);
+                        mma_scores<T, DP>(tm + C::DPC, r0 + C::TILE, x1b + x1 * C::TILE);
                         umma_commit_w(&sh.dpfull);
+                        if (!kv) umma_commit_w(&sh.x1empty[x1]);
                     }
-                    if (vote(u + 2 == steps || steps == 1)) umma_commit_w(&sh.rempty);    // no more products with R
-                    x = xn;
-                    if (++st == C::ST) st = 0;
+                    umma_commit_w(&sh.x0empty[x0]);
+                    if (vote(u + 2 == steps)) umma_commit_w(&sh.rempty);      // no more products with R
+                    x0 = x0n;
                 }
                 if (!ok) break;
                 umma_commit_w(&sh.fin);
