@@ -23,8 +23,9 @@
 
 namespace dn8 {
 
-// ---- delta and the logarithms in units of log2, head by head -------------------------------------
-// work: lse2 [Hq][Tq] (+inf where the row sees nothing: its P = 2^(s - inf) = 0), then delta [Hq][Tq].
+// ---- delta and the logarithms, head by head -------------------------------------
+// work: -lse2 [Hq][Tq] (-inf where the row sees nothing: its P = 2^(s - inf) = 0), then -delta scale
+// [Hq][Tq]: so that P = 2^(S c + w0) and dS = P (dP scale + w1), two fused operations on pairs.
 // LANES (8 or 16) threads per row of up to 64 or 128 elements; 32 rows of one head per block.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(32 * LANES) attn_bwd_prep_kernel(const dn8_attention_bwd_args a) {
@@ -44,8 +45,8 @@ __global__ void __launch_bounds__(32 * LANES) attn_bwd_prep_kernel(const dn8_att
     if (row < a.Tq && threadIdx.x % LANES == 0) {
         const float lse = a.lse[row * a.Hq + h];
         float* w = static_cast<float*>(a.work) + h * a.Tq + row;
-        w[0] = lse == -INFINITY ? INFINITY : lse * ATT_LOG2E;
-        w[a.Hq * a.Tq] = lse == -INFINITY ? 0.0f : s;
+        w[0] = lse == -INFINITY ? -INFINITY : -lse * ATT_LOG2E;
+        w[a.Hq * a.Tq] = lse == -INFINITY ? 0.0f : -s * a.scale;
     }
 }
 
@@ -62,7 +63,6 @@ template <int DP> struct BwdCfg {
     // TMEM columns: dP, then S (one or two tiles), then the sums at the end
     static constexpr uint32_t DPC = 0, S = 128, ACC1 = 512 - DP, ACC0 = 512 - 2 * DP;
 };
-constexpr int AB_POLY = 3;                    // of 8 pairs of exponentials, those taken by polynomial
 // S tiles: the sums are dv (ACC0) and dk (ACC1), or dq (ACC1)
 template <int DP> DN8_DEV constexpr int s_tiles(bool kv) { return kv && DP == 128 ? 1 : 2; }
 
@@ -96,7 +96,7 @@ struct BwdShared {
     uint32_t words[2][4];                     // of even and odd steps, as the statistics
     uint32_t tmem;
     int abort;
-    alignas(16) float lse2[2][AT_TILE], delta[2][AT_TILE];
+    alignas(16) float w0[2][AT_TILE], w1[2][AT_TILE];      // the statistics of a step's queries
 };
 
 // The 16 row warps on one piece: warp w has the TMEM lanes (resident rows) 32 (w % 4) .. and the columns
@@ -116,11 +116,11 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
     const bool inside = r < (KV ? pc.seq.nk : pc.seq.nq);
     // KV: the key may be seen at all; dq: the row's statistics
     const bool keep = KV && inside && (a.keep == nullptr || a.keep[pc.seq.k0 + r] != 0);
-    float row_lse = INFINITY, row_delta = 0.0f;
+    float row_w0 = -INFINITY, row_w1 = 0.0f;
     if (!KV && inside) {
         const float* w = static_cast<const float*>(a.work) + pc.h * a.Tq + pc.seq.q0 + r;
-        row_lse = w[0];
-        row_delta = w[a.Hq * a.Tq];
+        row_w0 = w[0];
+        row_w1 = w[a.Hq * a.Tq];
     }
     bool ok = true;
     const int steps = pc.steps, turn = pc.turn, hic = pc.hic, loc = pc.loc, skc = pc.skc;
@@ -138,7 +138,7 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
             const int off = pc.seq.nk - pc.seq.nq;
             if (KV) {
                 // columns are queries: seen from j - right - off on, up to j + left - off (first tokens: by all).
-                // Queries behind the end are zero rows with lse2 = inf.
+                // Queries behind the end are zero rows with w0 = -inf.
                 const int lo = r - right - off - c0, hi = r < a.sinks ? ATT_FAR : r + left - off - c0;
                 word = keep ? bits_from(lo, quarter) & bits_upto(hi, quarter) : 0u;
             } else {
@@ -161,18 +161,19 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.pready[c & 1]);
         }
+        // (a part of the exponentials by polynomial, to spare the special function units, was slower: the row
+        // warps' issue slots are the scarcer of the two)
         const float2 sc2 = f2_pack(sc, sc);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float2 l = f2_pack(-row_lse, -row_lse);
-            if (KV) {
-                l = *reinterpret_cast<const float2*>(sh.lse2[sx] + quarter * 32 + 2 * e);
-                l = f2_pack(-l.x, -l.y);
-            }
-            const float2 x = ex2_pair<AB_POLY>(
-                f2_fma(f2_pack(__uint_as_float(pr[2 * e]), __uint_as_float(pr[2 * e + 1])), sc2, l), e);
-            pr[2 * e] = __float_as_uint(x.x);
-            pr[2 * e + 1] = __float_as_uint(x.y);
+        for (int e = 0; e < 32; e += 4) {
+            float4 w = make_float4(row_w0, row_w0, row_w0, row_w0);
+            if (KV) w = *reinterpret_cast<const float4*>(sh.w0[sx] + quarter * 32 + e);
+            const float2 x = f2_fma(f2_pack(__uint_as_float(pr[e]), __uint_as_float(pr[e + 1])), sc2, f2_pack(w.x, w.y));
+            const float2 y = f2_fma(f2_pack(__uint_as_float(pr[e + 2]), __uint_as_float(pr[e + 3])), sc2, f2_pack(w.z, w.w));
+            pr[e] = __float_as_uint(ex2(x.x));
+            pr[e + 1] = __float_as_uint(ex2(x.y));
+            pr[e + 2] = __float_as_uint(ex2(y.x));
+            pr[e + 3] = __float_as_uint(ex2(y.y));
         }
         if (masked)
 #pragma unroll
@@ -198,24 +199,17 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
         if (masked)
 #pragma unroll
             for (int e = 0; e < 32; ++e) dp[e] = (word >> e) & 1u ? dp[e] : 0u;
-        if (KV) {
-            const float4* d4 = reinterpret_cast<const float4*>(sh.delta[sx] + quarter * 32);
+        const float2 scale2 = f2_pack(a.scale, a.scale);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float4 d = d4[e];
-                const float de[4] = {d.x, d.y, d.z, d.w};
-                float ds[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    ds[x] = __uint_as_float(pr[4 * e + x]) * ((__uint_as_float(dp[4 * e + x]) - de[x]) * a.scale);
-                pk[2 * e] = pack2(T(), ds[0], ds[1]);
-                pk[2 * e + 1] = pack2(T(), ds[2], ds[3]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                pk[e] = pack2(T(), __uint_as_float(pr[2 * e]) * ((__uint_as_float(dp[2 * e]) - row_delta) * a.scale),
-                              __uint_as_float(pr[2 * e + 1]) * ((__uint_as_float(dp[2 * e + 1]) - row_delta) * a.scale));
+        for (int e = 0; e < 32; e += 4) {
+            float4 w = make_float4(row_w1, row_w1, row_w1, row_w1);
+            if (KV) w = *reinterpret_cast<const float4*>(sh.w1[sx] + quarter * 32 + e);
+            const float2 x = f2_fma(f2_pack(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), scale2, f2_pack(w.x, w.y));
+            const float2 y = f2_fma(f2_pack(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3])), scale2, f2_pack(w.z, w.w));
+            const float2 u2 = __fmul2_rn(x, f2_pack(__uint_as_float(pr[e]), __uint_as_float(pr[e + 1])));
+            const float2 v2 = __fmul2_rn(y, f2_pack(__uint_as_float(pr[e + 2]), __uint_as_float(pr[e + 3])));
+            pk[e / 2] = pack2(T(), u2.x, u2.y);
+            pk[e / 2 + 1] = pack2(T(), v2.x, v2.y);
         }
         tmem_st16(tp, pk);
         tmem_wait_st(pk);
@@ -240,7 +234,7 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
     T* dst = KV ? (quarter < 2 ? static_cast<T*>(a.dv) + at * a.dv_stride_t + pc.h * a.dv_stride_h
                                : static_cast<T*>(a.dk) + at * a.dk_stride_t + pc.h * a.dk_stride_h)
                 : static_cast<T*>(a.dq) + at * a.dq_stride_t + pc.h * a.dq_stride_h;
-    const bool zero = steps == 0 || (!KV && row_lse == INFINITY);
+    const bool zero = steps == 0 || (!KV && row_w0 == -INFINITY);
 #pragma unroll 1
     for (int k = 0; k < COLS; k += 16) {
         uint32_t o[16] = {};
@@ -334,7 +328,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         if (lane == 0) mbar_arrive(&sh.pread);
         return sh.piece[n & 1].seq.b >= 0;
     };
-    griddep_wait();                                      // delta and lse2
+    griddep_wait();                                      // the statistics
 
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AB_REGS_OTHER));
@@ -483,7 +477,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const int x = tile * AT_TILE + w * 32 + lane;
-                        l2[w] = INFINITY;
+                        l2[w] = -INFINITY;
                         de[w] = 0.0f;
                         live[w] = true;
                         if (kv && x < nq) {
@@ -509,10 +503,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     if (!ok) break;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        word[w] = __ballot_sync(0xffffffffu, kv ? l2[w] != INFINITY : live[w]);
+                        word[w] = __ballot_sync(0xffffffffu, kv ? l2[w] != -INFINITY : live[w]);
                         if (kv) {
-                            sh.lse2[sx][w * 32 + lane] = l2[w];
-                            sh.delta[sx][w * 32 + lane] = de[w];
+                            sh.w0[sx][w * 32 + lane] = l2[w];
+                            sh.w1[sx][w * 32 + lane] = de[w];
                         } else if (lane == w) {
                             sh.words[sx][w] = word[w];
                         }

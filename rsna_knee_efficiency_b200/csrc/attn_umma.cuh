@@ -143,30 +143,6 @@ DN8_DEV float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^x of a pair without the special function unit (16 results per clock and SM, the bound of a softmax at D =
-// 64): x = n + f with n the nearest integer (read off the sum with 1.5 2^23), 2^f on [-1/2, 1/2] by the
-// degree-4 polynomial of least relative error (Remez exchange; 2.7e-6 = 2^-18.5 with fp32 coefficients),
-// and n added to the exponent. x below -126 gives 2^-126, which a 16-bit weight rounds to 0 (bf16: to
-// 1.2e-38) like the weight it stands for.
-DN8_DEV float2 ex2_poly(float2 x) {
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
-    const float2 magic = f2_pack(12582912.0f, 12582912.0f), minus = f2_pack(-12582912.0f, -12582912.0f);
-    const float2 t = __fadd2_rn(x, magic), n = __fadd2_rn(t, minus);
-    const float2 f = __fadd2_rn(x, f2_pack(-n.x, -n.y));
-    float2 p = f2_fma(f, f2_pack(0.009570102207362652f, 0.009570102207362652f), f2_pack(0.05591785907745361f, 0.05591785907745361f));
-    p = f2_fma(p, f, f2_pack(0.240247443318367f, 0.240247443318367f));
-    p = f2_fma(p, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
-    p = f2_fma(p, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
-    return f2_pack(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                   __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-// Pair k of a row's: which of the two ways takes its exponentials. POLY of every 8 pairs go by polynomial.
-template <int POLY> DN8_DEV float2 ex2_pair(float2 x, int k) {
-    if ((k * POLY) % 8 < POLY) return ex2_poly(x);
-    return f2_pack(ex2(x.x), ex2(x.y));
-}
-
 // Bits [lo, hi] of a row of 128, word w.
 DN8_DEV uint32_t bits_from(int lo, int w) {
     const int k = lo - 32 * w;
