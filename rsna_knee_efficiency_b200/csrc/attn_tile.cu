@@ -13,11 +13,13 @@
 // A CTA takes one piece after the other (ask_for_block): the loads and first scores of the next piece run
 // while the threads still write the last one's output.
 //
-// Warps 0-7 and 8-15: softmax of tile 0 and 1, two threads per row (64 scores each), then the output. Eight
-// warps with 128 scores a thread took 1.3 times as long: two warps per scheduler leave it idle two cycles of
-// three, waiting for their own last instruction. Warp 16: tcgen05 issue. Warp 17: TMA. Warp 18: rows of V that
-// nobody may see (behind the sequence, keep = 0) are zeroed in shared memory before the product, since
-// 0 * NaN is not 0 (their scores are replaced, so K may hold anything). Warp 19: which piece comes next.
+// Warps 0-7 and 8-15: softmax of tile 0 and 1, a warp per 16 rows and four threads per row, so that a row's
+// maximum takes two shuffles (32 scores of two rows a thread; one thread per row left the schedulers idle
+// two cycles of three, two threads of different warps per row had to meet in shared memory for every
+// tile). Warps 16 and 19: tcgen05 issue, one per query tile: an issue is some 25 instructions with its waits,
+// and one warp for both tiles was late for each by the other's. Warp 17: TMA. Warp 18: which piece comes
+// next, and rows of V that nobody may see (behind the sequence, keep = 0): they are zeroed in shared memory
+// before the product, since 0 * NaN is not 0 (their scores are replaced, so K may hold anything).
 #include "attn_umma.cuh"
 
 namespace dn8 {
@@ -35,18 +37,17 @@ template <int DP> struct TileCfg {
     static constexpr uint32_t S0 = 0, O0 = 256;
 };
 
-DN8_DEV bool has_tile(const KeyTiles& k, int t) {
-    return k.count > 0 && (t < k.first || (t >= k.start && t < k.start + k.count - k.first));
-}
-// Named barrier of two warps
+// Named barrier of the two warps that share 32 TMEM lanes
 DN8_DEV void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 DN8_DEV void pair_arrive(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
 
 struct TilePiece {
     Sequence seq;                                     // seq.b = -2: no more pieces
     int h, i0;                                        // query head, first query row
-    KeyTiles all, own[2];                             // key tiles of the piece and of each query tile
-    DN8_DEV bool uses(int g, int t) const { return has_tile(own[g], t); }
+    KeyTiles all, own[2];                             // key tiles of the piece, and of each query tile
+    // Query tile g's own are the piece's tiles u < lead[g] and from[g] <= u < to[g]. A tile whose first key is above
+    // hic[g], or below loc[g] but above skc, or (with a key mask) every tile, needs a mask.
+    int lead[2], from[2], to[2], hic[2], loc[2], skc;
 };
 
 struct TileShared {
@@ -57,7 +58,7 @@ struct TileShared {
     uint64_t pfilled, pread;
     TilePiece piece[2];                               // of even and odd number
     uint32_t words[3][4];
-    float part[2][2][AT_TILE];                        // [tile][half of the columns][row]
+    float stat[2][2][AT_TILE];                        // [tile][sum, reference][row]
     uint32_t tmem;
     int abort;
 };
@@ -80,12 +81,12 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     if (threadIdx.x == 512) {
         mbar_init(&sh.answered, 1);
         mbar_init(&sh.qfull, 1);
-        mbar_init(&sh.qempty, 1);
+        mbar_init(&sh.qempty, 2);
         for (int s = 0; s < 3; ++s) {
             mbar_init(&sh.kfull[s], 1);
-            mbar_init(&sh.kempty[s], 1);
+            mbar_init(&sh.kempty[s], 2);
             mbar_init(&sh.vfull[s], 1);
-            mbar_init(&sh.vempty[s], 1);
+            mbar_init(&sh.vempty[s], 2);
             mbar_init(&sh.vok[s], 1);
         }
         for (int g = 0; g < 2; ++g) {
@@ -107,7 +108,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
     const int left = a.left < 0 ? ATT_FAR : a.left, right = a.right < 0 ? ATT_FAR : a.right;
 
     // Piece n of this CTA: sh.piece[n % 2], from the moment it is filled until every warp has begun with the
-    // next one. Every warp but the last calls this for n = 0, 1, ... when it begins; false: there is
+    // next one. Every warp but 18 calls this for n = 0, 1, ... when it begins; false: there is
     // none (or a wait gave up).
     auto begin_piece = [&](int n) -> bool {
         if (!mbar_wait_w(&sh.pfilled, n & 1, a.err, abort_flag, ERR_WAIT_FULL | (63 << 4))) return false;
@@ -117,49 +118,114 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
 
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AF_REGS_OTHER));
-        if (warp == 19) {
-            // ---------------- pieces ----------------
-            int block = blockIdx.x, asked = 0;
+        if (warp == 18) {
+            // ---------------- pieces, and masked rows of V ----------------
+            int block = blockIdx.x, asked = 0, vc = 0;
             TilePiece pc;
-            for (int n = 0;;) {
-                pc.seq.b = -2;
-                if (block >= 0) {
+            // Looks block after block up until one holds a piece: false after the last.
+            auto look = [&]() -> bool {
+                while (block >= 0) {
                     pc.seq = find_block<false>(a, block / a.Hq, 1, 2 * AT_TILE);
                     pc.h = block % a.Hq;
+                    if (pc.seq.b >= 0) return true;   // (the bound on the blocks may be too high)
+                    if (lane == 0) {
+                        fence_async_smem();           // the last answer has been read
+                        mbar_expect_tx(&sh.answered, 16);
+                        ask_for_block(sh.answer, &sh.answered);
+                    }
+                    if (!mbar_wait_w(&sh.answered, asked & 1, a.err, abort_flag, ERR_WAIT_FULL | (61 << 4))) return false;
+                    ++asked;
+                    block = answered_block(sh.answer);
+                    __syncwarp();
                 }
-                if (pc.seq.b >= 0) {
-                    const int off = pc.seq.nk - pc.seq.nq;
+                return false;
+            };
+            auto publish = [&](int n, bool there) {
+                if (!there) {
+                    pc.seq.b = -2;
+                } else {
+                    const int nq = pc.seq.nq, nk = pc.seq.nk, off = nk - nq;
                     // last blocks first: with an open left side they are the longest
-                    pc.i0 = ((pc.seq.nq - 1) / (2 * AT_TILE) - pc.seq.blk) * 2 * AT_TILE;
-                    const int end = min(pc.i0 + 2 * AT_TILE, pc.seq.nq);
-                    pc.all = key_tiles(pc.i0 + off, end - 1 + off, pc.seq.nk, left, right, a.sinks, AT_TILE);
+                    pc.i0 = ((nq - 1) / (2 * AT_TILE) - pc.seq.blk) * 2 * AT_TILE;
+                    const int end = min(pc.i0 + 2 * AT_TILE, nq);
+                    pc.all = key_tiles(pc.i0 + off, end - 1 + off, nk, left, right, a.sinks, AT_TILE);
+                    pc.skc = a.sinks - AT_TILE;
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
-                        const int r0 = pc.i0 + g * AT_TILE;
-                        pc.own[g] = key_tiles(r0 + off, min(r0 + AT_TILE, end) - 1 + off, pc.seq.nk, left, right, a.sinks,
-                                              AT_TILE);
-                        if (r0 >= end) pc.own[g].count = 0;
+                        const int p0 = pc.i0 + g * AT_TILE + off, p1 = min(pc.i0 + (g + 1) * AT_TILE, end) - 1 + off;
+                        KeyTiles& own = pc.own[g];
+                        own = key_tiles(p0, p1, nk, left, right, a.sinks, AT_TILE);
+                        if (p0 > p1) own.count = 0;
+                        // (the piece's tiles are 0 .. first - 1 and start ..; a query tile's own are among them)
+                        pc.lead[g] = own.count > 0 ? own.first : 0;
+                        pc.from[g] = own.start < pc.all.first ? own.start : pc.all.first + own.start - pc.all.start;
+                        pc.to[g] = own.count > 0 ? pc.from[g] + own.count - own.first : 0;
+                        pc.hic[g] = min(nk - 1, p0 + right) - (AT_TILE - 1);
+                        pc.loc[g] = p1 - left;
                     }
-                }
-                if (pc.seq.b != -1) {                 // (-1: the bound on the blocks was too high)
-                    if (lane == 0) {
-                        sh.piece[n & 1] = pc;
-                        mbar_arrive(&sh.pfilled);
-                    }
-                    if (pc.seq.b == -2) break;
-                    // (the softmax warps read a piece when they start on it: one is known ahead, no more)
-                    if (!mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (62 << 4))) break;
-                    ++n;
                 }
                 if (lane == 0) {
-                    fence_async_smem();               // the last answer has been read
-                    mbar_expect_tx(&sh.answered, 16);
-                    ask_for_block(sh.answer, &sh.answered);
+                    sh.piece[n & 1] = pc;
+                    mbar_arrive(&sh.pfilled);
                 }
-                if (!mbar_wait_w(&sh.answered, asked & 1, a.err, abort_flag, ERR_WAIT_FULL | (61 << 4))) break;
-                ++asked;
-                block = answered_block(sh.answer);
                 __syncwarp();
+            };
+            publish(0, look());
+            bool ok = true;
+            for (int n = 0; pc.seq.b >= 0; ++n) {
+                const int count = pc.all.count, nk = pc.seq.nk, k0 = pc.seq.k0;
+                const KeyTiles all = pc.all;
+                for (int u = 0; u < max(count, 1); ++u) {
+                    if (u < count) {
+                        const int t = all.tile(u), vs = vc % C::VST;
+                        const bool fix = a.keep != nullptr || (t + 1) * AT_TILE > nk;
+                        uint32_t word[4];
+                        if (fix)
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                const int j = t * AT_TILE + w * 32 + lane;
+                                word[w] = __ballot_sync(0xffffffffu, j < nk && (a.keep == nullptr || a.keep[k0 + j] != 0));
+                            }
+                        ok = mbar_wait_w(&sh.vfull[vs], (vc / C::VST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (66 << 4));
+                        if (!ok) break;
+                        if (fix) {
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                if (lane == w) sh.words[vs][w] = word[w];
+                                if (!((word[w] >> lane) & 1u))
+#pragma unroll
+                                    for (int b = 0; b < DP / 64; ++b) {
+                                        uint4* row =
+                                            reinterpret_cast<uint4*>(sv + vs * C::TILE + b * AT_BLOCK + (w * 32 + lane) * 128);
+#pragma unroll
+                                        for (int c = 0; c < 8; ++c) row[c] = make_uint4(0u, 0u, 0u, 0u);
+                                    }
+                            }
+                            fence_async_smem();
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.vok[vs]);
+                        ++vc;
+                    }
+                    if (u == 0) {
+                        // The next piece, once every warp has begun with this one (the softmax warps do so last: one
+                        // piece is known ahead, no more). The first tile's product does not wait for it.
+                        ok = mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (62 << 4));
+                        if (!ok) break;
+                        if (lane == 0) {
+                            fence_async_smem();
+                            mbar_expect_tx(&sh.answered, 16);
+                            ask_for_block(sh.answer, &sh.answered);
+                        }
+                        ok = mbar_wait_w(&sh.answered, asked & 1, a.err, abort_flag, ERR_WAIT_FULL | (61 << 4));
+                        if (!ok) break;
+                        ++asked;
+                        block = answered_block(sh.answer);
+                        __syncwarp();
+                        publish(n + 1, look());
+                    }
+                }
+                if (!ok) break;
             }
         } else if (warp == 17) {
             // ---------------- TMA ----------------
@@ -191,112 +257,52 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 ++nq;
                 __syncwarp();
             }
-        } else if (warp == 18) {
-            // ---------------- masked rows of V ----------------
-            int vc = 0;
-            bool ok = true;
-            for (int n = 0; ok && begin_piece(n); ++n) {
-                const TilePiece& pc = sh.piece[n & 1];
-                for (int u = 0; u < pc.all.count; ++u, ++vc) {
-                    const int t = pc.all.tile(u), vs = vc % C::VST;
-                    const bool fix = a.keep != nullptr || (t + 1) * AT_TILE > pc.seq.nk;
-                    uint32_t word[4];
-                    if (fix)
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const int j = t * AT_TILE + w * 32 + lane;
-                            word[w] = __ballot_sync(0xffffffffu,
-                                                    j < pc.seq.nk && (a.keep == nullptr || a.keep[pc.seq.k0 + j] != 0));
-                        }
-                    ok = mbar_wait_w(&sh.vfull[vs], (vc / C::VST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (66 << 4));
-                    if (!ok) break;
-                    if (fix) {
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            if (lane == w) sh.words[vs][w] = word[w];
-                            if (!((word[w] >> lane) & 1u))
-#pragma unroll
-                                for (int b = 0; b < DP / 64; ++b) {
-                                    uint4* row =
-                                        reinterpret_cast<uint4*>(sv + vs * C::TILE + b * AT_BLOCK + (w * 32 + lane) * 128);
-#pragma unroll
-                                    for (int c = 0; c < 8; ++c) row[c] = make_uint4(0u, 0u, 0u, 0u);
-                                }
-                        }
-                        fence_async_smem();
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.vok[vs]);
-                }
-            }
         } else {
             // ---------------- tcgen05 issue (every value and branch uniform, see attn_umma.cuh) ----------------
-            const uint32_t q0 = uniform(smem_u32(sq)), k0 = uniform(smem_u32(sk)), v0 = uniform(smem_u32(sv));
-            const uint32_t tm = uniform(tmem);
-            uint32_t ks = 0, kp = 0, vs = 0, vp = 0, pp = 0, qp = 0;      // stages; phases, pfull's and oempty's by bit g
-            uint32_t op = 3;
+            // warp 16: query tile 0, warp 19: query tile 1
+            const uint32_t g = vote(warp == 19) ? 1u : 0u;
+            const uint32_t q0 = uniform(smem_u32(sq) + g * C::TILE), k0 = uniform(smem_u32(sk)), v0 = uniform(smem_u32(sv));
+            const uint32_t ts = uniform(tmem + C::S0 + g * 128), to = uniform(tmem + C::O0 + g * DP);
+            uint32_t ks = 0, kp = 0, vs = 0, vp = 0, pp = 0, qp = 0, op = 1;      // stages and phases
             for (int n = 0; vote(begin_piece(n)); ++n) {
-                KeyTiles all, own0, own1;
-                {
-                    const TilePiece& pc = sh.piece[n & 1];
-                    all.first = uniform(pc.all.first), all.start = uniform(pc.all.start), all.count = uniform(pc.all.count);
-                    own0.first = uniform(pc.own[0].first), own0.start = uniform(pc.own[0].start);
-                    own0.count = uniform(pc.own[0].count);
-                    own1.first = uniform(pc.own[1].first), own1.start = uniform(pc.own[1].start);
-                    own1.count = uniform(pc.own[1].count);
-                }
-                if (vote(all.count == 0)) continue;
-                if (!mbar_wait_w(&sh.qfull, qp, a.err, abort_flag, ERR_WAIT_FULL | (67 << 4))) break;
+                const TilePiece& pc = sh.piece[n & 1];
+                const int count = uniform(pc.all.count), lead = uniform(pc.lead[g]), from = uniform(pc.from[g]),
+                          to_ = uniform(pc.to[g]);
+                if (vote(count == 0)) continue;
+                bool ok = mbar_wait_w(&sh.qfull, qp, a.err, abort_flag, ERR_WAIT_FULL | (67 << 4)), begun = false, had = false;
+                if (!ok) break;
                 qp ^= 1;
-                bool begun0 = false, begun1 = false, had0 = false, had1 = false, ok = true;
-                for (int u = 0; vote(u <= all.count); ++u) {
-                    const bool more = vote(u < all.count);
-                    const int t = all.tile(u);
-                    const bool now0 = vote(more && has_tile(own0, t)), now1 = vote(more && has_tile(own1, t));
+                for (int u = 0; vote(u <= count); ++u) {
+                    const bool more = vote(u < count), now = vote(more && (u < lead || (u >= from && u < to_)));
+                    // (a tile that this query tile does not use is waited for all the same before it is released: the
+                    // release counts for the phase that follows its load)
                     if (more) {
                         ok = mbar_wait_w(&sh.kfull[ks], kp, a.err, abort_flag, ERR_WAIT_FULL | (68 << 4));
                         if (!ok) break;
                     }
                     if (vote(u > 0)) {
-                        ok = mbar_wait_w(&sh.vfull[vs], vp, a.err, abort_flag, ERR_WAIT_FULL | (69 << 4)) &&
-                             mbar_wait_w(&sh.vok[vs], vp, a.err, abort_flag, ERR_WAIT_FULL | (70 << 4));
+                        ok = mbar_wait_w(&sh.vok[vs], vp, a.err, abort_flag, ERR_WAIT_FULL | (70 << 4));
                         if (!ok) break;
-                    }
-                    const uint32_t kt = k0 + ks * C::TILE, vt = v0 + vs * C::TILE;
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        bool& begun = g ? begun1 : begun0;
-                        if (g ? had1 : had0) {
-                            ok = mbar_wait_w(&sh.pfull[g], (pp >> g) & 1, a.err, abort_flag, ERR_WAIT_ACC | (71 << 4));
+                        if (had) {
+                            ok = mbar_wait_w(&sh.pfull[g], pp, a.err, abort_flag, ERR_WAIT_ACC | (71 << 4));
                             if (!ok) break;
-                            pp ^= 1u << g;
+                            pp ^= 1;
                             if (!begun) {             // the last piece's output has been read
-                                ok = mbar_wait_w(&sh.oempty[g], (op >> g) & 1, a.err, abort_flag, ERR_WAIT_ACC | (59 << 4));
+                                ok = mbar_wait_w(&sh.oempty[g], op, a.err, abort_flag, ERR_WAIT_ACC | (59 << 4));
                                 if (!ok) break;
-                                op ^= 1u << g;
+                                op ^= 1;
                             }
                             tc_fence_after();
-                            mma_values<T, DP, 64>(tm + C::O0 + g * DP, tm + C::S0 + g * 128, vt, begun);
+                            mma_values<T, DP, 128>(to, ts, v0 + vs * C::TILE, begun);
                             begun = true;
                         }
-                        if (g ? now1 : now0) {
-                            // (S lies over P: the product that reads P was issued before)
-                            tc_fence_after();
-                            mma_scores<T, DP>(tm + C::S0 + g * 128, q0 + g * C::TILE, kt);
-                            umma_commit_w(&sh.sfull[g]);
-                        }
                     }
-                    if (!ok) break;
-                    had0 = now0;
-                    had1 = now1;
-                    if (more) {
-                        umma_commit_w(&sh.kempty[ks]);
-                        if (++ks == C::KST) {
-                            ks = 0;
-                            kp ^= 1;
-                        }
+                    if (now) {
+                        // (S lies over P: the product that reads P was issued before)
+                        tc_fence_after();
+                        mma_scores<T, DP>(ts, q0, k0 + ks * C::TILE);
+                        umma_commit_w(&sh.sfull[g]);
                     }
-                    if (vote(u + 1 == all.count)) umma_commit_w(&sh.qempty);
                     if (vote(u > 0)) {
                         umma_commit_w(&sh.vempty[vs]);
                         if (++vs == C::VST) {
@@ -304,148 +310,185 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                             vp ^= 1;
                         }
                     }
+                    if (more) {
+                        umma_commit_w(&sh.kempty[ks]);
+                        if (++ks == C::KST) {
+                            ks = 0;
+                            kp ^= 1;
+                        }
+                    }
+                    if (vote(u + 1 == count)) umma_commit_w(&sh.qempty);
+                    had = now;
                 }
                 if (!ok) break;
-                if (begun0) umma_commit_w(&sh.ofull[0]);
-                if (begun1) umma_commit_w(&sh.ofull[1]);
+                if (begun) umma_commit_w(&sh.ofull[g]);
             }
             __syncwarp();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AF_REGS_SOFTMAX));
-        // ---------------- softmax: two threads per row ----------------
-        const int g = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
-        const uint32_t quad = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + C::S0 + g * 128 + half * 64 + quad, to = tmem + C::O0 + g * DP + half * (DP / 2) + quad;
-        float* mine = &sh.part[g][half][row];
-        const float* other = &sh.part[g][half ^ 1][row];
-        const int pair = 1 + g * 4 + (warp & 3);      // named barrier of the two warps that share rows
+        // ---------------- softmax: a warp per 16 rows, four threads per row ----------------
+        const int g = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+        const int row = quad * 32 + half * 16 + (lane >> 2);           // of the query tile; the other one is row + 8
+        const uint32_t lanes = static_cast<uint32_t>(quad * 32 + half * 16) << 16;
+        const uint32_t ts = tmem + C::S0 + g * 128 + lanes, to = tmem + C::O0 + g * DP + lanes;
+        const int pair = 1 + g * 4 + quad;
         const float sc = a.scale * ATT_LOG2E;
         int ns = 0, no = 0, vc0 = 0;                  // scores and outputs so far; V tiles before this piece
         bool ok = true;
         for (int np = 0; ok && begin_piece(np); ++np) {
             const TilePiece& pc = sh.piece[np & 1];
-            float m = -INFINITY, l = 0.0f;            // reference (times sc), and this half's sum
-            int n = 0;
-            for (int u = 0; u < pc.all.count; ++u) {
-                const int t = pc.all.tile(u), j0 = t * AT_TILE, vs = (vc0 + u) % C::VST;
-                if (!pc.uses(g, t)) continue;
-                // positions of the tile's first and last row: does every row see every key?
-                const int nk = pc.seq.nk, last = j0 + AT_TILE - 1, pa = pc.i0 + g * AT_TILE + nk - pc.seq.nq;
-                const bool masked = a.keep != nullptr || last > min(nk - 1, pa + right) ||
-                                    (j0 < min(pa + AT_TILE, nk) - 1 - left && last >= a.sinks);
-                uint32_t word[2];
-                if (masked) {
-                    const int hi = min(nk - 1, pa + row + right) - j0, lo = pa + row - left - j0;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        word[c] = bits_upto(hi, 2 * half + c) &
-                                  (bits_from(lo, 2 * half + c) | bits_upto(a.sinks - 1 - j0, 2 * half + c));
-                }
+            const int tiles = pc.own[g].count, turn = pc.own[g].first - 1, hic = pc.hic[g], loc = pc.loc[g], skc = pc.skc;
+            int t = pc.own[g].tile(0);
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};      // references (times sc), this thread's sums
+            for (int n = 0; n < tiles; ++n) {
+                const int j0 = t * AT_TILE;
+                const bool masked = a.keep != nullptr || j0 > hic || (j0 < loc && j0 > skc);
+                t = t == turn ? pc.own[g].start : t + 1;
                 ok = mbar_wait_w(&sh.sfull[g], ns & 1, a.err, abort_flag, ERR_WAIT_ACC | (73 << 4));
                 if (!ok) break;
                 ++ns;
                 tc_fence_after();
                 uint32_t r[2][32];
-                tmem_ld32(ts, r[0]);
-                tmem_ld32(ts + 32, r[1]);
-                if (a.keep != nullptr) {
-                    // (after S: its issue has waited for the V tiles before this one, so the phase is not mistaken)
-                    ok = mbar_wait_w(&sh.vok[vs], ((vc0 + u) / C::VST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (72 << 4));
+                tmem_ld16x256_8(ts, r[0]);
+                tmem_ld16x256_8(ts + 64, r[1]);
+                if (masked) {
+                    int vs = 0;
+                    if (a.keep != nullptr) {
+                        // (after S: its issue has waited for the V tiles before this one, so the phase is not mistaken)
+                        const int u = vc0 + (n < pc.lead[g] ? n : pc.from[g] + n - pc.lead[g]);
+                        vs = u % C::VST;
+                        ok = mbar_wait_w(&sh.vok[vs], (u / C::VST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (72 << 4));
+                    }
+                    tmem_wait_ld(r[0]);
+                    reg_bind(r[1]);
+                    if (!ok) break;
+                    const int nk = pc.seq.nk, p0 = pc.i0 + g * AT_TILE + row + nk - pc.seq.nq;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) word[c] &= sh.words[vs][2 * half + c];
+                    for (int h = 0; h < 2; ++h) {
+                        const int p = p0 + 8 * h, hi = min(nk - 1, p + right) - j0, lo = p - left - j0;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t word = bits_upto(hi, w) & (bits_from(lo, w) | bits_upto(a.sinks - 1 - j0, w));
+                            if (a.keep != nullptr) word &= sh.words[vs][w];
+                            word >>= 2 * (lane & 3);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    uint32_t& x = r[w >> 1][4 * (4 * (w & 1) + k) + 2 * h + e];
+                                    x = (word >> (8 * k + e)) & 1u ? x : 0xFF800000u;          // -inf
+                                }
+                        }
+                    }
+                } else {
+                    tmem_wait_ld(r[0]);
+                    reg_bind(r[1]);
                 }
-                tmem_wait_ld(r[0]);
-                reg_bind(r[1]);
-                if (!ok) break;
-                if (masked)
+                float mx[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) r[c][e] = (word[c] >> e) & 1u ? r[c][e] : 0xFF800000u;   // -inf
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // four chains, not one of 64
+                        for (int h = 0; h < 2; ++h)
+                            mx[h][c] = fmaxf(fmaxf(mx[h][c], __uint_as_float(r[c][4 * k + 2 * h])),
+                                             __uint_as_float(r[c][4 * k + 2 * h + 1]));
+                float top[2];
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        m4[c] = fmaxf(fmaxf(m4[c], __uint_as_float(r[c >> 1][e + 2 * (c & 1)])),
-                                      __uint_as_float(r[c >> 1][e + 2 * (c & 1) + 1]));
-                float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                *mine = mx;
-                pair_sync(pair);
-                if (*abort_flag) {
-                    ok = false;
-                    break;
+                for (int h = 0; h < 2; ++h) {
+                    top[h] = fmaxf(mx[h][0], mx[h][1]);
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)) * sc;
                 }
-                mx = fmaxf(mx, *other) * sc;
-                if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
-                    const float mn = fmaxf(m, mx);
-                    const float f = ex2(m - (mn == -INFINITY ? 0.0f : mn));
-                    m = mn;
-                    l *= f;
+                if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
+                    float f[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float mn = fmaxf(m[h], top[h]);
+                        f[h] = ex2(m[h] - (mn == -INFINITY ? 0.0f : mn));
+                        m[h] = mn;
+                        l[h] *= f[h];
+                    }
                     if (n > 0) {
                         // S complete: so is the product before it, and the next one waits for P
 #pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
                             uint32_t o[16];
-                            tmem_ld16(to + 16 * c, o);
+                            tmem_ld16x256_4(to + 32 * c, o);
                             tmem_wait_ld(o);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st16(to + 16 * c, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f[(e >> 1) & 1]);
+                            tmem_st16x256_4(to + 32 * c, o);
                             tmem_wait_st(o);
                         }
                     }
                 }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const float2 sc2 = f2_pack(sc, sc), mr2 = f2_pack(-ref, -ref);
-                float2 s2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+                const float2 sc2 = f2_pack(sc, sc);
+                float2 mr2[2], s2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float ref = m[h] == -INFINITY ? 0.0f : -m[h];
+                    mr2[h] = f2_pack(ref, ref);
+                }
                 uint32_t pk[2][16];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        float2 x = f2_fma(f2_pack(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), sc2, mr2);
+                        float2 x = f2_fma(f2_pack(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), sc2,
+                                          mr2[e & 1]);
                         x.x = ex2(x.x);
                         x.y = ex2(x.y);
                         s2[e & 1] = __fadd2_rn(s2[e & 1], x);
                         // the weights are rounded to the values' type, the type of the matrix instruction
                         pk[c][e] = pack2(T(), x.x, x.y);
                     }
-                    tmem_st16(ts + 16 * c, pk[c]);
+                    tmem_st16x128_8(ts + 32 * c, pk[c]);
                 }
-                l += (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y);
+                l[0] += s2[0].x + s2[0].y;
+                l[1] += s2[1].x + s2[1].y;
                 tmem_wait_st(pk[0]);
                 tmem_wait_st(pk[1]);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.pfull[g]);
-                ++n;
             }
             if (!ok) break;
             vc0 += pc.all.count;
-            if (n > 0) {
-                // the two halves' sums (the barrier before has been passed by both: part is free)
+            // The output: a row per thread, the two warps of these 32 rows half of the elements each. Sums and
+            // references change hands through shared memory (a warp writes here again only after a tile that its
+            // partner has taken part in).
+            float ls = 0.0f, ms = -INFINITY;
+            if (tiles > 0) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                    if ((lane & 3) == 0) {
+                        sh.stat[g][0][row + 8 * h] = l[h];
+                        sh.stat[g][1][row + 8 * h] = m[h];
+                    }
+                }
                 pair_sync(pair);
-                *mine = l;
-                pair_sync(pair);
-                l = half == 0 ? l + *other : *other + l;
-                pair_sync(pair);
+                ls = sh.stat[g][0][quad * 32 + lane];
+                ms = sh.stat[g][1][quad * 32 + lane];
                 ok = mbar_wait_w(&sh.ofull[g], no & 1, a.err, abort_flag, ERR_WAIT_ACC | (74 << 4));
                 if (!ok || *abort_flag) break;
                 ++no;
                 tc_fence_after();
             }
-            const int i = pc.i0 + g * AT_TILE + row, h = pc.h;
+            const int i = pc.i0 + g * AT_TILE + quad * 32 + lane, h = pc.h;
             const int64_t at = pc.seq.q0 + i;
             const bool live = i < pc.seq.nq;
             T* out = static_cast<T*>(a.out) + at * a.o_stride_t + static_cast<int64_t>(h) * a.o_stride_h;
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const uint32_t tq = tmem + C::O0 + g * DP + half * (DP / 2) + (static_cast<uint32_t>(quad * 32) << 16);
+            const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
 #pragma unroll 1
             for (int c = 0; c < DP / 32; ++c) {
                 uint32_t o[16] = {};
-                if (n > 0) {
-                    tmem_ld16(to + 16 * c, o);
+                if (tiles > 0) {
+                    tmem_ld16(tq + 16 * c, o);
                     tmem_wait_ld(o);
                 }
                 const int d = half * (DP / 2) + 16 * c;
@@ -453,17 +496,17 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 for (int e = 0; e < 16; e += 8) {
                     float v[8];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) v[x] = l > 0.0f ? __uint_as_float(o[e + x]) * inv : 0.0f;
+                    for (int x = 0; x < 8; ++x) v[x] = ls > 0.0f ? __uint_as_float(o[e + x]) * inv : 0.0f;
                     if (live && d + e < a.D) store_f32(out + d + e, v);
                 }
             }
-            if (n > 0) {                              // O has been read: the next piece may use it
+            if (tiles > 0) {                          // O has been read: the next piece may use it
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.oempty[g]);
             }
             if (live && half == 0 && a.lse != nullptr)
-                a.lse[at * a.Hq + h] = l > 0.0f ? (m + __log2f(l)) * ATT_LN2 : -INFINITY;
+                a.lse[at * a.Hq + h] = ls > 0.0f ? (ms + __log2f(ls)) * ATT_LN2 : -INFINITY;
         }
         // A warp that gave up arrives once more, so that its partner's barrier completes; the partner then
         // sees the abort flag and leaves too.

@@ -81,12 +81,45 @@ template <typename T, int DP> DN8_DEV void mma_scores(uint32_t d, uint32_t a, ui
 }
 // D[128 x DP] (+)= A B, A [128 x 128] in TMEM, B a tile of 128 rows. A lies over the fp32 tile it was made
 // from: each PART columns of it in the first PART / 2 TMEM columns of their own, so that the threads that
-// read a part write over nothing else (PART = 64 or 32).
+// read a part write over nothing else (PART = 32), or all in the first 64 TMEM columns (PART = 128: threads
+// that have whole rows).
 template <typename T, int DP, int PART> DN8_DEV void mma_values(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-        umma_f16_ts4<PART == 64 ? 16 : 32>(d, a + 64 * k, desc_cols(b, 4 * k), idesc_f16<T>(AT_TILE, DP, true),
-                                           accumulate || k > 0);
+        umma_f16_ts4<PART == 128 ? 16 : 32>(d, a + (PART == 128 ? 32 : 64) * k, desc_cols(b, 4 * k),
+                                            idesc_f16<T>(AT_TILE, DP, true), accumulate || k > 0);
+}
+
+// Four threads per row: 16 rows x 64 columns of fp32. Thread t's registers 4k .. 4k + 3 are (row t / 4, columns
+// 8k + 2 (t % 4) and the next) and the same columns of row t / 4 + 8.
+#define DN8_R8(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), \
+                  "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+DN8_DEV void tmem_ld16x256_8(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : DN8_R8(0), DN8_R8(8), DN8_R8(16), DN8_R8(24) : "r"(taddr) : "memory");
+}
+DN8_DEV void tmem_ld16x256_4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : DN8_R8(0), DN8_R8(8) : "r"(taddr) : "memory");
+}
+#undef DN8_R8
+DN8_DEV void tmem_st16x256_4(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+// 16 rows x 32 columns of packed words: registers 2k, 2k + 1 are column 4k + t % 4 of rows t / 4 and t / 4 + 8.
+DN8_DEV void tmem_st16x128_8(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
 }
 
 // One row per thread: 16 packed words (32 elements of 16 bits) to columns taddr ..
