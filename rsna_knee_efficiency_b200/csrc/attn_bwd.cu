@@ -51,7 +51,10 @@ __global__ void __launch_bounds__(32 * LANES) attn_bwd_prep_kernel(const dn8_att
 }
 
 // ---- the two walks -----------------------------------------------------------------------------
-constexpr int AB_THREADS = 640;             // warps 0-15: rows; 16: tcgen05 issue; 17: TMA; 18: masked rows; 19: pieces
+// Warps 0-15: rows; 16: tcgen05 issue; 17: TMA; 18: statistics and masked rows of the streamed tiles; 19: which
+// piece comes next, asked for AB_AHEAD steps before the end of a piece (asked for at its start, a piece waits
+// behind a long one while others run out of work).
+constexpr int AB_THREADS = 640, AB_AHEAD = 4;
 // The launch gives every thread 96 registers: 16 x 32 x 104 + 4 x 32 x 64 = 20 x 32 x 96.
 constexpr int AB_REGS_ROWS = 104, AB_REGS_OTHER = 64;
 template <int DP> struct BwdCfg {
@@ -87,7 +90,7 @@ struct BwdPiece {
 };
 struct BwdShared {
     uint64_t answer[2];
-    uint64_t answered, pfilled, pread, rfull, rempty, fin, aempty, dpfull, dsready;
+    uint64_t answered, pfilled, pread, near, rfull, rempty, fin, aempty, dpfull, dsready;
     // (of even and odd steps: the rows may be done with S(u + 1), where there are two S tiles, before the
     // issuing warp, held up by its own queue, has looked for S(u))
     uint64_t pready[2];
@@ -291,6 +294,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         mbar_init(&sh.answered, 1);
         mbar_init(&sh.pfilled, 1);
         mbar_init(&sh.pread, 19);
+        mbar_init(&sh.near, 1);
         mbar_init(&sh.rfull, 1);
         mbar_init(&sh.rempty, 1);
         mbar_init(&sh.fin, 1);
@@ -408,8 +412,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                         mbar_arrive(&sh.pfilled);
                     }
                     if (pc.seq.b == -2) break;
-                    // (the row warps begin a piece last: one is known ahead, no more)
-                    if (!mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (92 << 4))) break;
+                    // (every warp has begun with it: one piece is known ahead, no more)
+                    if (!mbar_wait_w(&sh.near, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (99 << 4)) ||
+                        !mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (92 << 4)))
+                        break;
                     ++n;
                 }
                 if (lane == 0) {
@@ -495,7 +501,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     }
                 };
                 if (steps > 0) fetch();
+                if (steps == 0 && lane == 0) mbar_arrive(&sh.near);
                 for (int u = 0; u < steps; ++u, ++c) {
+                    if (u == max(0, steps - AB_AHEAD) && lane == 0) mbar_arrive(&sh.near);
                     const uint32_t s0 = c % C::N0, s1 = c % C::N1, sx = c & 1;
                     uint32_t word[4];
                     // (the step before the last has been read)

@@ -28,6 +28,10 @@ constexpr int AF_THREADS = 640;
 // The launch gives every thread 96 registers; the softmax warps take some of the others':
 // 16 x 32 x 104 + 4 x 32 x 64 = 20 x 32 x 96.
 constexpr int AF_REGS_SOFTMAX = 104, AF_REGS_OTHER = 64;
+// How many tiles before the end of a piece the next one is asked for: time enough to hide the question and the
+// first loads. Asked for at the start, a piece waits behind a long one while others run out of work: four
+// sequences of 6144, causal, took 364 us instead of 317.
+constexpr int AF_AHEAD = 4;
 
 template <int DP> struct TileCfg {
     static constexpr int KST = DP == 64 ? 3 : 2, VST = DP == 64 ? 3 : 2;      // stages of K and V
@@ -175,6 +179,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             for (int n = 0; pc.seq.b >= 0; ++n) {
                 const int count = pc.all.count, nk = pc.seq.nk, k0 = pc.seq.k0;
                 const KeyTiles all = pc.all;
+                const int ask_at = max(0, count - AF_AHEAD);
                 for (int u = 0; u < max(count, 1); ++u) {
                     if (u < count) {
                         const int t = all.tile(u), vs = vc % C::VST;
@@ -207,9 +212,9 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                         if (lane == 0) mbar_arrive(&sh.vok[vs]);
                         ++vc;
                     }
-                    if (u == 0) {
-                        // The next piece, once every warp has begun with this one (the softmax warps do so last: one
-                        // piece is known ahead, no more). The first tile's product does not wait for it.
+                    if (u == ask_at) {
+                        // The next piece, once every warp has begun with this one. (This tile's product does not wait for
+                        // it.)
                         ok = mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (62 << 4));
                         if (!ok) break;
                         if (lane == 0) {
@@ -343,7 +348,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};      // references (times sc), this thread's sums
             for (int n = 0; n < tiles; ++n) {
                 const int j0 = t * AT_TILE;
-                const bool masked = a.keep != nullptr || j0 > hic || (j0 < loc && j0 > skc);
+                const bool ranged = j0 > hic || (j0 < loc && j0 > skc), masked = a.keep != nullptr || ranged;
                 t = t == turn ? pc.own[g].start : t + 1;
                 ok = mbar_wait_w(&sh.sfull[g], ns & 1, a.err, abort_flag, ERR_WAIT_ACC | (73 << 4));
                 if (!ok) break;
@@ -353,24 +358,27 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 tmem_ld16x256_8(ts, r[0]);
                 tmem_ld16x256_8(ts + 64, r[1]);
                 if (masked) {
-                    int vs = 0;
+                    uint32_t keep[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
                     if (a.keep != nullptr) {
                         // (after S: its issue has waited for the V tiles before this one, so the phase is not mistaken)
-                        const int u = vc0 + (n < pc.lead[g] ? n : pc.from[g] + n - pc.lead[g]);
-                        vs = u % C::VST;
+                        const int u = vc0 + (n < pc.lead[g] ? n : pc.from[g] + n - pc.lead[g]), vs = u % C::VST;
                         ok = mbar_wait_w(&sh.vok[vs], (u / C::VST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (72 << 4));
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) keep[w] = sh.words[vs][w];
                     }
                     tmem_wait_ld(r[0]);
                     reg_bind(r[1]);
                     if (!ok) break;
                     const int nk = pc.seq.nk, p0 = pc.i0 + g * AT_TILE + row + nk - pc.seq.nq;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int p = p0 + 8 * h, hi = min(nk - 1, p + right) - j0, lo = p - left - j0;
+                    for (int w = 0; w < 4; ++w)
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            uint32_t word = bits_upto(hi, w) & (bits_from(lo, w) | bits_upto(a.sinks - 1 - j0, w));
-                            if (a.keep != nullptr) word &= sh.words[vs][w];
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t word = keep[w];
+                            if (ranged) {
+                                const int p = p0 + 8 * h, hi = min(nk - 1, p + right) - j0, lo = p - left - j0;
+                                word &= bits_upto(hi, w) & (bits_from(lo, w) | bits_upto(a.sinks - 1 - j0, w));
+                            }
                             word >>= 2 * (lane & 3);
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
@@ -380,7 +388,6 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                                     x = (word >> (8 * k + e)) & 1u ? x : 0xFF800000u;          // -inf
                                 }
                         }
-                    }
                 } else {
                     tmem_wait_ld(r[0]);
                     reg_bind(r[1]);
@@ -438,6 +445,8 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                     for (int e = 0; e < 16; ++e) {
                         float2 x = f2_fma(f2_pack(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), sc2,
                                           mr2[e & 1]);
+                        // (some of them by polynomial, to spare the special function units, cost the schedulers as
+                        // much as it spared)
                         x.x = ex2(x.x);
                         x.y = ex2(x.y);
                         s2[e & 1] = __fadd2_rn(s2[e & 1], x);
