@@ -176,15 +176,13 @@ DN8_DEV float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Bits [lo, hi] of a row of 128, word w.
+// Bits lo .. and .. hi of a row of 128, word w. (shl.b32 gives 0 for counts of 32 and more.)
 DN8_DEV uint32_t bits_from(int lo, int w) {
-    const int k = lo - 32 * w;
-    return k <= 0 ? 0xFFFFFFFFu : k >= 32 ? 0u : 0xFFFFFFFFu << k;
+    uint32_t r;
+    asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(0xFFFFFFFFu), "r"(max(lo - 32 * w, 0)));
+    return r;
 }
-DN8_DEV uint32_t bits_upto(int hi, int w) {
-    const int k = hi - 32 * w;
-    return k < 0 ? 0u : k >= 31 ? 0xFFFFFFFFu : (2u << k) - 1u;
-}
+DN8_DEV uint32_t bits_upto(int hi, int w) { return ~bits_from(hi + 1, w); }
 
 // 3-D map over [rows][heads][D] with token / head strides (elements): box 64 elements x 1 head x `box_rows`
 // rows. Elements behind D and rows behind the tensor arrive as zeros.
