@@ -40,10 +40,36 @@ template <> DN8_DEV void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)
 // Where a share's partial results are kept: [row block][key head][share] of (16 rows x (maximum, sum)) and
 // 16 x DP outputs, relative to the row's maximum (in units of log2).
 struct RowsPlan {
-    int blocks, splits;
+    int blocks, splits;      // row blocks (a bound) and shares there is room for
+    int slots;               // CTAs per key head that the GPU holds at a time
     float* ml;
     float* o;
 };
+
+// Shares of a row block's key axis. Lengths are known to the GPU alone, so each CTA adds them up: with as many
+// shares in all as there are slots, every share about as long, the CTAs run side by side and end together.
+// (Shares by the average length left the longest of ragged caches alone at the end; several waves of short
+// shares cost a start and an end each: 16 x 12288 keys, 8 heads, 74 us in one wave, 79 in two, 90 in five.)
+DN8_DEV int seen_keys(const dn8_attention_args& a, int nq, int nk) {      // that some row of a sequence sees, at most
+    if (a.left < 0 || a.right < 0) return nk;
+    return min(nk, min(a.left, nk) + min(a.right, nk) + min(a.sinks, nk) + nq);
+}
+// Keys of all row blocks of a key head (one whole warp).
+DN8_DEV float all_keys(const dn8_attention_args& a) {
+    const int G = a.Hq / a.Hk, lane = threadIdx.x & 31;
+    float total = 0.0f;
+    for (int b = lane; b < a.B; b += 32) {
+        const Sequence s = sequence_of(a, b);
+        total += static_cast<float>((static_cast<int64_t>(s.nq) * G + AR_ROWS - 1) / AR_ROWS * seen_keys(a, s.nq, s.nk));
+    }
+    return warp_sum(total);
+}
+template <int KEYS> DN8_DEV int shares_of(const dn8_attention_args& a, const RowsPlan& plan, const Sequence& sq, float total) {
+    if (sq.b < 0) return 0;
+    if (plan.splits == 1) return 1;
+    const float share = fmaxf(total / static_cast<float>(plan.slots), 4.0f * AR_WARPS * KEYS);      // keys
+    return max(1, min(plan.splits, static_cast<int>(seen_keys(a, sq.nq, sq.nk) / share)));
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(AR_WARPS * 32, 2)
@@ -56,13 +82,17 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
     __shared__ Sequence s_seq;
     __shared__ uint64_t s_full[AR_WARPS][AR_STAGES];
     __shared__ int s_abort;
+    __shared__ float s_total;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.Hq / a.Hk, kvh = blockIdx.z;
     griddep_launch_dependents();
     if (warp == 0) {
         const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS);
         if (lane == 0) s_seq = f;
-    } else if (threadIdx.x == 32) {
+    } else if (warp == 1) {
+        const float t = plan.splits > 1 ? all_keys(a) : 0.0f;
+        if (lane == 0) s_total = t;
+    } else if (threadIdx.x == 64) {
         for (int w = 0; w < AR_WARPS; ++w)
             for (int k = 0; k < AR_STAGES; ++k) mbar_init(&s_full[w][k], 1);
         s_abort = 0;
@@ -70,14 +100,15 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
     }
     __syncthreads();
     const Sequence sq = s_seq;
-    if (sq.b < 0) return;
+    const int shares = shares_of<KEYS>(a, plan, sq, s_total);
+    if (static_cast<int>(blockIdx.y) >= shares) return;
     volatile int* abort_flag = &s_abort;
     const int r0 = sq.blk * AR_ROWS, nrows = min(AR_ROWS, sq.nq * G - r0);
     const int off = sq.nk - sq.nq;
     const int left = a.left < 0 ? ATT_FAR : a.left, right = a.right < 0 ? ATT_FAR : a.right;
     const int p0 = r0 / G + off, p1 = (r0 + nrows - 1) / G + off;      // first and last row's position
     const KeyTiles kt = key_tiles(p0, p1, sq.nk, left, right, a.sinks, KEYS);
-    const int workers = plan.splits * AR_WARPS, me = blockIdx.y * AR_WARPS + warp;
+    const int workers = shares * AR_WARPS, me = blockIdx.y * AR_WARPS + warp;
     uint8_t* ring = sm + warp * AR_STAGES * AR_STAGE;
 
     auto issue = [&](int t, int stage) {                 // (lane 0)
@@ -258,7 +289,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
             ov = fmaf(f, so[(w * AR_ROWS + r) * DP + d], ov);
             lv = fmaf(f, sml[(w * AR_ROWS + r) * 2 + 1], lv);
         }
-        if (plan.splits > 1) {
+        if (shares > 1) {
             plan.o[(slot * AR_ROWS + r) * DP + d] = ov;
             if (d == 0) {
                 plan.ml[(slot * AR_ROWS + r) * 2] = mm;
@@ -279,30 +310,35 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
 template <typename T, int DP>
 __global__ void __launch_bounds__(AR_ROWS * 32) attn_join_kernel(const dn8_attention_args a, const RowsPlan plan) {
     __shared__ Sequence s_seq;
+    __shared__ float s_total;
     const int G = a.Hq / a.Hk, kvh = blockIdx.y, r = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (r == 0) {
         const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS);
         if (lane == 0) s_seq = f;
+    } else if (r == 1) {
+        const float t = all_keys(a);
+        if (lane == 0) s_total = t;
     }
     __syncthreads();
     const Sequence sq = s_seq;
-    if (sq.b < 0 || sq.blk * AR_ROWS + r >= sq.nq * G) return;
+    const int shares = shares_of<AR_TILE_BYTES / (DP * 2)>(a, plan, sq, s_total);
+    if (shares <= 1 || sq.blk * AR_ROWS + r >= sq.nq * G) return;      // (one share: the output is written)
     const size_t slot = (static_cast<size_t>(blockIdx.x) * a.Hk + kvh) * plan.splits;
     griddep_wait();
     float mm = -INFINITY;
-    for (int s = lane; s < plan.splits; s += 32) mm = fmaxf(mm, plan.ml[((slot + s) * AR_ROWS + r) * 2]);
+    for (int s = lane; s < shares; s += 32) mm = fmaxf(mm, plan.ml[((slot + s) * AR_ROWS + r) * 2]);
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
     const float ref = mm == -INFINITY ? 0.0f : mm;
     float lv = 0.0f, ov[DP / 32] = {};
-    for (int s0 = 0; s0 < plan.splits; s0 += 32) {
+    for (int s0 = 0; s0 < shares; s0 += 32) {
         float w = 0.0f;
-        if (s0 + lane < plan.splits) {
+        if (s0 + lane < shares) {
             const float2 ml = *reinterpret_cast<const float2*>(plan.ml + ((slot + s0 + lane) * AR_ROWS + r) * 2);
             w = ex2(ml.x - ref);
             lv = fmaf(w, ml.y, lv);
         }
-        const int ns = min(32, plan.splits - s0);
+        const int ns = min(32, shares - s0);
 #pragma unroll 8
         for (int s = 0; s < ns; ++s) {
             float v[DP / 32];
@@ -326,20 +362,18 @@ namespace {
 
 int head_pad(int D) { return D <= 64 ? 64 : 128; }
 
-// Row blocks (a bound: every sequence may leave one block unfilled) and shares of the key axis: as many
-// as give every SM a few CTAs while a warp still has a handful of tiles of an average sequence.
+// Row blocks (a bound: every sequence may leave one block unfilled), and room for shares: four times what an
+// average sequence gets, for the longest ones.
 RowsPlan rows_plan(const dn8_attention_args& a, int sms) {
     RowsPlan p = {};
     const int64_t rows = a.Tq * (a.Hq / a.Hk);
     p.blocks = static_cast<int>(rows / AR_ROWS + (a.B < rows ? a.B : rows));
-    int64_t seen = a.Tk / a.B;
-    if (a.left >= 0 && a.right >= 0) {
-        const int64_t w = static_cast<int64_t>(a.left) + a.right + 1 + a.sinks + a.Tq / a.B;
-        if (w < seen) seen = w;
-    }
-    const int64_t tiles = seen * head_pad(a.D) * 2 / AR_TILE_BYTES;
-    int64_t s = 12ll * sms / (static_cast<int64_t>(p.blocks) * a.Hk);
+    p.slots = 2 * sms / a.Hk;                            // (two CTAs per SM, by their shared memory)
+    const int64_t real = a.B * ((rows / a.B + AR_ROWS - 1) / AR_ROWS);
+    int64_t s = 4ll * p.slots / real;
+    const int64_t tiles = a.Tk * head_pad(a.D) * 2 / AR_TILE_BYTES;
     if (s > tiles / (4 * AR_WARPS)) s = tiles / (4 * AR_WARPS);
+    if (p.slots < 2 * real) s = 1;
     p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
     return p;
 }

@@ -148,10 +148,15 @@ def _heads(call: str, name: str, t, shape, types, dev, out: bool = False) -> tup
     return st, sh
 
 
+# the handle of a device's current stream, without a Stream object around it where torch offers that (2 us)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _launch(what: str, fn, a, dev: torch.device, stream) -> None:
     """Calls `fn(a, stream)` with the tensors' device current."""
     if stream is None:
-        s = torch.cuda.current_stream(dev).cuda_stream
+        s = _current_stream(dev.index)
     else:
         if stream.device != dev:
             raise ValueError(f"{what}: the stream is not of {dev}")
@@ -213,8 +218,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
     _flat(c, "rstd", rstd, (M,), _F32, dev)
     if wt not in _TYPES:
         _refuse(c, "bias", bias, (C,), _ANY, dev, "contiguous")
-    a = nat.LayerNormArgs(_ptr(x), _ptr(res), _ptr(weight), _ptr(bias), _ptr(out), _ptr(sum), _ptr(mean), _ptr(rstd),
-                          M, xs, rs, ys, ss, C, _TYPES[t], _TYPES[out.dtype], _TYPES[wt], eps)
+    a = nat.LayerNormArgs(x.data_ptr(), _ptr(res), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(sum), _ptr(mean),
+                          _ptr(rstd), M, xs, rs, ys, ss, C, _TYPES[t], _TYPES[out.dtype], _TYPES[wt], eps)
     _launch("dn8_layer_norm", nat.lib().dn8_layer_norm, a, dev, stream)
 
 
@@ -253,6 +258,9 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     _launch("dn8_layer_norm_bwd", lib.dn8_layer_norm_bwd, a, dev, stream)
 
 
+_SECTIONS = nat.I32 * nat.DN8_ROPE_AXES
+
+
 def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, q_out: torch.Tensor, k_out: torch.Tensor | None,
          sections, base: float = 10000.0, per_axis: bool = False, interleaved: bool = False, inverse: bool = False,
          stream=None) -> None:
@@ -279,9 +287,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, q_out: torc
             raise ValueError(f"{c}: k [T, H, D] expected")
         Hk = k.shape[1]
         ks, ko = _heads(c, "k", k, (T, Hk, D), t, dev), _heads(c, "k_out", k_out, (T, Hk, D), t, dev, True)
-    a = nat.RopeArgs(_ptr(q), _ptr(k), _ptr(pos), _ptr(q_out), _ptr(k_out), T, *qs, *ks, *qo, *ko, Hq, Hk, D,
-                     _TYPES[q.dtype], axes, (nat.I32 * nat.DN8_ROPE_AXES)(*sections), per_axis, interleaved, inverse,
-                     base)
+    a = nat.RopeArgs(q.data_ptr(), _ptr(k), pos.data_ptr(), q_out.data_ptr(), _ptr(k_out), T, *qs, *ks, *qo, *ko, Hq, Hk,
+                     D, _TYPES[t[0]], axes, _SECTIONS(*sections), per_axis, interleaved, inverse, base)
     _launch("dn8_rope", nat.lib().dn8_rope, a, dev, stream)
 
 
@@ -328,8 +335,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tens
     c = "attention"
     dev, sq, sk, t, strides, mask = _packed(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale)
     os = _heads(c, "out", out, sq, t, dev, True)
-    a = nat.AttentionArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cu_q), _ptr(cu_k), _ptr(len_k),
-                          _ptr(keep), _ptr(err), None, sq[0], sk[0], *strides, *os, *mask)
+    a = nat.AttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), cu_q.data_ptr(),
+                          cu_k.data_ptr(), _ptr(len_k), _ptr(keep), _ptr(err), None, sq[0], sk[0], *strides, *os, *mask)
     lib = nat.lib()
     nbytes = _bytes_of(lib.dn8_attention_work, a, dev)
     if nbytes > 0:
