@@ -3,10 +3,11 @@
 // A piece of work = up to 256 query rows of one head of one sequence, as two tiles of 128 rows, over the key
 // tiles that some row of them sees. Per key tile and query tile:
 //   S = Q K^T        tcgen05 128 x 128 x D into TMEM,
-//   P = 2^(S c - m)  one thread per row reads S from TMEM; P goes back to TMEM in 16 bits, over S,
+//   P = 2^(S c - m)  the threads read S from TMEM; P goes back to TMEM in 16 bits,
 //   O += P V         tcgen05 128 x D x 128, P from TMEM, V as it lies in memory.
-// Two query tiles alternate: while the threads of one take the exponentials of their S, the tensor cores
-// work on the other. The reference m of a row is its running maximum at the time of the last
+// Two query tiles are worked on side by side. At D <= 64 P has TMEM columns of its own, so the next S is made as
+// soon as this one has been read, and the threads find it when they are done; above, P lies over S, and the
+// next S waits for the product that reads P. The reference m of a row is its running maximum at the time of the last
 // rescaling: O and the sum are rescaled only when the maximum has grown by more than 2^8 (then P <=
 // 256, far inside fp16 and fp32), so the accumulator rarely leaves TMEM.
 //
@@ -37,8 +38,9 @@ template <int DP> struct TileCfg {
     static constexpr int KST = DP == 64 ? 3 : 2, VST = DP == 64 ? 3 : 2;      // stages of K and V
     static constexpr uint32_t TILE = AT_TILE * DP * 2;
     static constexpr uint32_t SMEM = 1024 + TILE * (2 + KST + VST) + 3072;
-    // TMEM columns: S (and P) of the two tiles, O of the two tiles
-    static constexpr uint32_t S0 = 0, O0 = 256;
+    // TMEM columns: S of the two tiles, P (over S, or of its own), O
+    static constexpr bool OWN_P = DP == 64;
+    static constexpr uint32_t S0 = 0, P0 = OWN_P ? 256 : 0, PG = OWN_P ? 64 : 128, O0 = OWN_P ? 384 : 256;
 };
 
 // Named barrier of the two warps that share 32 TMEM lanes
@@ -58,7 +60,7 @@ struct TileShared {
     uint64_t answer[2];                               // (16-byte aligned: first)
     uint64_t answered, qfull, qempty;
     uint64_t kfull[3], kempty[3], vfull[3], vempty[3], vok[3];
-    uint64_t sfull[2], pfull[2], ofull[2], oempty[2];
+    uint64_t sfull[2], sread[2], pfull[2], ofull[2], oempty[2];
     uint64_t pfilled, pread;
     TilePiece piece[2];                               // of even and odd number
     uint32_t words[3][4];
@@ -95,6 +97,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         }
         for (int g = 0; g < 2; ++g) {
             mbar_init(&sh.sfull[g], 1);
+            mbar_init(&sh.sread[g], 8);
             mbar_init(&sh.pfull[g], 8);
             mbar_init(&sh.ofull[g], 1);
             mbar_init(&sh.oempty[g], 8);
@@ -267,8 +270,9 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             // warp 16: query tile 0, warp 19: query tile 1
             const uint32_t g = vote(warp == 19) ? 1u : 0u;
             const uint32_t q0 = uniform(smem_u32(sq) + g * C::TILE), k0 = uniform(smem_u32(sk)), v0 = uniform(smem_u32(sv));
-            const uint32_t ts = uniform(tmem + C::S0 + g * 128), to = uniform(tmem + C::O0 + g * DP);
-            uint32_t ks = 0, kp = 0, vs = 0, vp = 0, pp = 0, qp = 0, op = 1;      // stages and phases
+            const uint32_t ts = uniform(tmem + C::S0 + g * 128), tp = uniform(tmem + C::P0 + g * C::PG);
+            const uint32_t to = uniform(tmem + C::O0 + g * DP);
+            uint32_t ks = 0, kp = 0, vs = 0, vp = 0, pp = 0, qp = 0, op = 1, rp = 1;      // stages and phases
             for (int n = 0; vote(begin_piece(n)); ++n) {
                 const TilePiece& pc = sh.piece[n & 1];
                 const int count = uniform(pc.all.count), lead = uniform(pc.lead[g]), from = uniform(pc.from[g]),
@@ -277,12 +281,33 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 bool ok = mbar_wait_w(&sh.qfull, qp, a.err, abort_flag, ERR_WAIT_FULL | (67 << 4)), begun = false, had = false;
                 if (!ok) break;
                 qp ^= 1;
+                // The next scores: of key tile u, and its release. (A tile that this query tile does not use is waited
+                // for all the same before it is released: the release counts for the phase that follows its load.)
+                auto scores = [&](int u, bool now) {
+                    if (now) {
+                        // (S is free: read, or P over it multiplied)
+                        if (C::OWN_P) {
+                            ok = mbar_wait_w(&sh.sread[g], rp, a.err, abort_flag, ERR_WAIT_ACC | (55 << 4));
+                            if (!ok) return;
+                            rp ^= 1;
+                        }
+                        tc_fence_after();
+                        mma_scores<T, DP>(ts, q0, k0 + ks * C::TILE);
+                        umma_commit_w(&sh.sfull[g]);
+                    }
+                    umma_commit_w(&sh.kempty[ks]);
+                    if (++ks == C::KST) {
+                        ks = 0;
+                        kp ^= 1;
+                    }
+                    if (vote(u + 1 == count)) umma_commit_w(&sh.qempty);
+                };
                 for (int u = 0; vote(u <= count); ++u) {
                     const bool more = vote(u < count), now = vote(more && (u < lead || (u >= from && u < to_)));
-                    // (a tile that this query tile does not use is waited for all the same before it is released: the
-                    // release counts for the phase that follows its load)
                     if (more) {
                         ok = mbar_wait_w(&sh.kfull[ks], kp, a.err, abort_flag, ERR_WAIT_FULL | (68 << 4));
+                        if (!ok) break;
+                        if (C::OWN_P) scores(u, now);
                         if (!ok) break;
                     }
                     if (vote(u > 0)) {
@@ -298,16 +323,12 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                                 op ^= 1;
                             }
                             tc_fence_after();
-                            mma_values<T, DP, 128>(to, ts, v0 + vs * C::TILE, begun);
+                            mma_values<T, DP, 128>(to, tp, v0 + vs * C::TILE, begun);
+                            if (C::OWN_P) umma_commit_w(&sh.ofull[g]);
                             begun = true;
                         }
                     }
-                    if (now) {
-                        // (S lies over P: the product that reads P was issued before)
-                        tc_fence_after();
-                        mma_scores<T, DP>(ts, q0, k0 + ks * C::TILE);
-                        umma_commit_w(&sh.sfull[g]);
-                    }
+                    if (!C::OWN_P && more) scores(u, now);
                     if (vote(u > 0)) {
                         umma_commit_w(&sh.vempty[vs]);
                         if (++vs == C::VST) {
@@ -315,18 +336,10 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                             vp ^= 1;
                         }
                     }
-                    if (more) {
-                        umma_commit_w(&sh.kempty[ks]);
-                        if (++ks == C::KST) {
-                            ks = 0;
-                            kp ^= 1;
-                        }
-                    }
-                    if (vote(u + 1 == count)) umma_commit_w(&sh.qempty);
                     had = now;
                 }
                 if (!ok) break;
-                if (begun) umma_commit_w(&sh.ofull[g]);
+                if (!C::OWN_P && begun) umma_commit_w(&sh.ofull[g]);
             }
             __syncwarp();
         }
@@ -336,7 +349,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         const int g = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
         const int row = quad * 32 + half * 16 + (lane >> 2);           // of the query tile; the other one is row + 8
         const uint32_t lanes = static_cast<uint32_t>(quad * 32 + half * 16) << 16;
-        const uint32_t ts = tmem + C::S0 + g * 128 + lanes, to = tmem + C::O0 + g * DP + lanes;
+        const uint32_t ts = tmem + C::S0 + g * 128 + lanes, tp = tmem + C::P0 + g * C::PG + lanes, to = tmem + C::O0 + g * DP + lanes;
         const int pair = 1 + g * 4 + quad;
         const float sc = a.scale * ATT_LOG2E;
         int ns = 0, no = 0, vc0 = 0;                  // scores and outputs so far; V tiles before this piece
@@ -360,7 +373,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 if (masked) {
                     uint32_t keep[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
                     if (a.keep != nullptr) {
-                        // (after S: its issue has waited for the V tiles before this one, so the phase is not mistaken)
+                        // (after S: its issue has waited for the V tiles VST before, so the phase is not mistaken)
                         const int u = vc0 + (n < pc.lead[g] ? n : pc.from[g] + n - pc.lead[g]), vs = u % C::VST;
                         ok = mbar_wait_w(&sh.vok[vs], (u / C::VST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (72 << 4));
 #pragma unroll
@@ -392,6 +405,11 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                     tmem_wait_ld(r[0]);
                     reg_bind(r[1]);
                 }
+                if (C::OWN_P) {                       // S is in registers: the next one may come
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.sread[g]);
+                }
                 float mx[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
@@ -408,6 +426,12 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)) * sc;
                 }
+                if (C::OWN_P && n > 0) {              // the product before is done with P, and O may be rescaled
+                    ok = mbar_wait_w(&sh.ofull[g], no & 1, a.err, abort_flag, ERR_WAIT_ACC | (56 << 4));
+                    if (!ok) break;
+                    ++no;
+                    tc_fence_after();
+                }
                 if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
                     float f[2];
 #pragma unroll
@@ -418,7 +442,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                         l[h] *= f[h];
                     }
                     if (n > 0) {
-                        // S complete: so is the product before it, and the next one waits for P
+                        // (with P over S: S complete, so is the product before it; the next one waits for P)
 #pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
                             uint32_t o[16];
@@ -453,7 +477,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                         // the weights are rounded to the values' type, the type of the matrix instruction
                         pk[c][e] = pack2(T(), x.x, x.y);
                     }
-                    tmem_st16x128_8(ts + 32 * c, pk[c]);
+                    tmem_st16x128_8(tp + 32 * c, pk[c]);
                 }
                 l[0] += s2[0].x + s2[0].y;
                 l[1] += s2[1].x + s2[1].y;
