@@ -37,38 +37,36 @@ template <> DN8_DEV void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Where a share's partial results are kept: [row block][key head][share] of (16 rows x (maximum, sum)) and
-// 16 x DP outputs, relative to the row's maximum (in units of log2).
+// Shares of a row block's key axis. Lengths are known to the GPU alone, so each CTA adds them up: every row block
+// is cut into as many whole parts of 1 / slots of all keys as it holds, and the CTAs are numbered block by
+// block, share by share, so that they run side by side and end together, however ragged the caches are.
+// (Several waves of short shares cost a start and an end each: 16 x 12288 keys, 8 heads, 74 us in one wave, 79 in
+// two, 90 in five.)
 struct RowsPlan {
-    int blocks, splits;      // row blocks (a bound) and shares there is room for
-    int slots;               // CTAs per key head that the GPU holds at a time
-    float* ml;
-    float* o;
+    int units;               // CTAs per key head, a bound: row blocks and shares
+    int slots;               // CTAs per key head that the GPU holds at a time, or 0: nothing is cut
+    float* ml;               // [key head][unit][16] (maximum in units of log2, sum)
+    float* o;                // [key head][unit][16][DP], relative to the maximum
 };
-
-// Shares of a row block's key axis. Lengths are known to the GPU alone, so each CTA adds them up: with as many
-// shares in all as there are slots, every share about as long, the CTAs run side by side and end together.
-// (Shares by the average length left the longest of ragged caches alone at the end; several waves of short
-// shares cost a start and an end each: 16 x 12288 keys, 8 heads, 74 us in one wave, 79 in two, 90 in five.)
-DN8_DEV int seen_keys(const dn8_attention_args& a, int nq, int nk) {      // that some row of a sequence sees, at most
-    if (a.left < 0 || a.right < 0) return nk;
-    return min(nk, min(a.left, nk) + min(a.right, nk) + min(a.sinks, nk) + nq);
-}
-// Keys of all row blocks of a key head (one whole warp).
-DN8_DEV float all_keys(const dn8_attention_args& a) {
-    const int G = a.Hq / a.Hk, lane = threadIdx.x & 31;
-    float total = 0.0f;
-    for (int b = lane; b < a.B; b += 32) {
-        const Sequence s = sequence_of(a, b);
-        total += static_cast<float>((static_cast<int64_t>(s.nq) * G + AR_ROWS - 1) / AR_ROWS * seen_keys(a, s.nq, s.nk));
+struct RowsShares {
+    const dn8_attention_args& a;
+    float part;              // keys
+    DN8_DEV int operator()(int nq, int nk) const {
+        return part > 0.0f ? max(1, static_cast<int>(seen_keys(a, nq, nk) / part)) : 1;
     }
-    return warp_sum(total);
-}
-template <int KEYS> DN8_DEV int shares_of(const dn8_attention_args& a, const RowsPlan& plan, const Sequence& sq, float total) {
-    if (sq.b < 0) return 0;
-    if (plan.splits == 1) return 1;
-    const float share = fmaxf(total / static_cast<float>(plan.slots), 4.0f * AR_WARPS * KEYS);      // keys
-    return max(1, min(plan.splits, static_cast<int>(seen_keys(a, sq.nq, sq.nk) / share)));
+};
+template <int KEYS> DN8_DEV RowsShares rows_shares(const dn8_attention_args& a, const RowsPlan& plan) {
+    RowsShares s = {a, 0.0f};                            // (one whole warp)
+    if (plan.slots == 0) return s;
+    const int G = a.Hq / a.Hk;
+    float total = 0.0f;
+    for (int b = threadIdx.x & 31; b < a.B; b += 32) {
+        const Sequence q = sequence_of(a, b);
+        total += static_cast<float>((static_cast<int64_t>(q.nq) * G + AR_ROWS - 1) / AR_ROWS) *
+                 static_cast<float>(seen_keys(a, q.nq, q.nk));
+    }
+    s.part = fmaxf(warp_sum(total) / static_cast<float>(plan.slots), 4.0f * AR_WARPS * KEYS);
+    return s;
 }
 
 template <typename T, int DP>
@@ -81,18 +79,18 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     __shared__ Sequence s_seq;
     __shared__ uint64_t s_full[AR_WARPS][AR_STAGES];
-    __shared__ int s_abort;
-    __shared__ float s_total;
+    __shared__ int s_abort, s_shares;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = a.Hq / a.Hk, kvh = blockIdx.z;
+    const int G = a.Hq / a.Hk, kvh = blockIdx.y;
     griddep_launch_dependents();
     if (warp == 0) {
-        const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS);
-        if (lane == 0) s_seq = f;
-    } else if (warp == 1) {
-        const float t = plan.splits > 1 ? all_keys(a) : 0.0f;
-        if (lane == 0) s_total = t;
-    } else if (threadIdx.x == 64) {
+        const RowsShares cuts = rows_shares<KEYS>(a, plan);
+        const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS, cuts);
+        if (lane == 0) {
+            s_seq = f;
+            s_shares = f.b < 0 ? 1 : cuts(f.nq, f.nk);
+        }
+    } else if (threadIdx.x == 32) {
         for (int w = 0; w < AR_WARPS; ++w)
             for (int k = 0; k < AR_STAGES; ++k) mbar_init(&s_full[w][k], 1);
         s_abort = 0;
@@ -100,15 +98,15 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
     }
     __syncthreads();
     const Sequence sq = s_seq;
-    const int shares = shares_of<KEYS>(a, plan, sq, s_total);
-    if (static_cast<int>(blockIdx.y) >= shares) return;
+    if (sq.b < 0) return;
+    const int shares = s_shares, share = sq.blk % shares;
     volatile int* abort_flag = &s_abort;
-    const int r0 = sq.blk * AR_ROWS, nrows = min(AR_ROWS, sq.nq * G - r0);
+    const int r0 = sq.blk / shares * AR_ROWS, nrows = min(AR_ROWS, sq.nq * G - r0);
     const int off = sq.nk - sq.nq;
     const int left = a.left < 0 ? ATT_FAR : a.left, right = a.right < 0 ? ATT_FAR : a.right;
     const int p0 = r0 / G + off, p1 = (r0 + nrows - 1) / G + off;      // first and last row's position
     const KeyTiles kt = key_tiles(p0, p1, sq.nk, left, right, a.sinks, KEYS);
-    const int workers = shares * AR_WARPS, me = blockIdx.y * AR_WARPS + warp;
+    const int workers = shares * AR_WARPS, me = share * AR_WARPS + warp;
     uint8_t* ring = sm + warp * AR_STAGES * AR_STAGE;
 
     auto issue = [&](int t, int stage) {                 // (lane 0)
@@ -275,7 +273,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
         }
     }
     __syncthreads();
-    const size_t slot = (static_cast<size_t>(blockIdx.x) * a.Hk + kvh) * plan.splits + blockIdx.y;
+    const size_t slot = static_cast<size_t>(kvh) * plan.units + blockIdx.x;
     for (int k = threadIdx.x; k < nrows * DP; k += AR_WARPS * 32) {
         const int r = k / DP, d = k % DP;
         float mm = -INFINITY;
@@ -310,20 +308,25 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
 template <typename T, int DP>
 __global__ void __launch_bounds__(AR_ROWS * 32) attn_join_kernel(const dn8_attention_args a, const RowsPlan plan) {
     __shared__ Sequence s_seq;
-    __shared__ float s_total;
+    __shared__ int s_shares;
     const int G = a.Hq / a.Hk, kvh = blockIdx.y, r = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (r == 0) {
-        const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS);
-        if (lane == 0) s_seq = f;
-    } else if (r == 1) {
-        const float t = all_keys(a);
-        if (lane == 0) s_total = t;
+        const auto cuts = rows_shares<AR_TILE_BYTES / (DP * 2)>(a, plan);
+        const Sequence f = find_block<false>(a, blockIdx.x, G, AR_ROWS, cuts);
+        if (lane == 0) {
+            s_seq = f;
+            s_shares = f.b < 0 ? 1 : cuts(f.nq, f.nk);
+        }
     }
     __syncthreads();
     const Sequence sq = s_seq;
-    const int shares = shares_of<AR_TILE_BYTES / (DP * 2)>(a, plan, sq, s_total);
-    if (shares <= 1 || sq.blk * AR_ROWS + r >= sq.nq * G) return;      // (one share: the output is written)
-    const size_t slot = (static_cast<size_t>(blockIdx.x) * a.Hk + kvh) * plan.splits;
+    // (one share: the output is written)
+    if (sq.b < 0 || s_shares <= 1 || sq.blk % s_shares != 0) return;
+    const int rr = sq.blk / s_shares * AR_ROWS + r;
+    if (rr >= sq.nq * G) return;
+    // (offsets that go back and forth may ask for more shares than there is room for)
+    const int shares = min(s_shares, plan.units - static_cast<int>(blockIdx.x));
+    const size_t slot = static_cast<size_t>(kvh) * plan.units + blockIdx.x;
     griddep_wait();
     float mm = -INFINITY;
     for (int s = lane; s < shares; s += 32) mm = fmaxf(mm, plan.ml[((slot + s) * AR_ROWS + r) * 2]);
@@ -349,7 +352,6 @@ __global__ void __launch_bounds__(AR_ROWS * 32) attn_join_kernel(const dn8_atten
         }
     }
     lv = warp_sum(lv);
-    const int rr = sq.blk * AR_ROWS + r;
     const int64_t row = sq.q0 + rr / G;
     const int h = kvh * G + rr % G;
 #pragma unroll
@@ -362,24 +364,23 @@ namespace {
 
 int head_pad(int D) { return D <= 64 ? 64 : 128; }
 
-// Row blocks (a bound: every sequence may leave one block unfilled), and room for shares: four times what an
-// average sequence gets, for the longest ones.
+// Row blocks (a bound: every sequence may leave one block unfilled), and shares: the sum of max(1, keys / part) is
+// at most blocks + slots (and one for the rounding of the sums). Many row blocks fill the GPU uncut.
 RowsPlan rows_plan(const dn8_attention_args& a, int sms) {
     RowsPlan p = {};
     const int64_t rows = a.Tq * (a.Hq / a.Hk);
-    p.blocks = static_cast<int>(rows / AR_ROWS + (a.B < rows ? a.B : rows));
-    p.slots = 2 * sms / a.Hk;                            // (two CTAs per SM, by their shared memory)
-    const int64_t real = a.B * ((rows / a.B + AR_ROWS - 1) / AR_ROWS);
-    int64_t s = 4ll * p.slots / real;
-    const int64_t tiles = a.Tk * head_pad(a.D) * 2 / AR_TILE_BYTES;
-    if (s > tiles / (4 * AR_WARPS)) s = tiles / (4 * AR_WARPS);
-    if (p.slots < 2 * real) s = 1;
-    p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+    const int64_t blocks = rows / AR_ROWS + (a.B < rows ? a.B : rows);
+    const int64_t slots = 2 * sms / a.Hk;                // (two CTAs per SM, by their shared memory)
+    p.units = static_cast<int>(blocks);
+    if (slots > 0 && blocks < 4 * slots && a.Tk * head_pad(a.D) * 2 / AR_TILE_BYTES >= 8 * AR_WARPS) {
+        p.slots = static_cast<int>(slots);
+        p.units = static_cast<int>(blocks + slots + 1);
+    }
     return p;
 }
 size_t rows_work(const dn8_attention_args& a, const RowsPlan& p) {
-    if (p.splits == 1) return 0;
-    return static_cast<size_t>(p.blocks) * a.Hk * p.splits * AR_ROWS * (head_pad(a.D) + 2) * sizeof(float);
+    if (p.slots == 0) return 0;
+    return static_cast<size_t>(p.units) * a.Hk * AR_ROWS * (head_pad(a.D) + 2) * sizeof(float);
 }
 
 template <typename T, int DP> cudaError_t rows_go(const dn8_attention_args& a, RowsPlan p, cudaStream_t st) {
@@ -396,26 +397,34 @@ template <typename T, int DP> cudaError_t rows_go(const dn8_attention_args& a, R
         if (e == cudaSuccess) e = make_head_map(&mv, a.v, a.type, a.Tk, a.Hk, a.D, a.v_stride_t, a.v_stride_h, keys);
         if (e != cudaSuccess) return e;
     }
-    if (p.splits > 1) {
+    if (p.slots > 0) {
         p.o = static_cast<float*>(a.work);
-        p.ml = p.o + static_cast<size_t>(p.blocks) * a.Hk * p.splits * AR_ROWS * DP;
+        p.ml = p.o + static_cast<size_t>(p.units) * a.Hk * AR_ROWS * DP;
     }
-    e = launch_pdl(false, attn_rows_kernel<T, DP>, dim3(p.blocks, p.splits, a.Hk), dim3(AR_WARPS * 32), smem, st, mk, mv,
-                   a, p);
-    if (e != cudaSuccess || p.splits == 1) return e;
-    return launch_pdl(true, attn_join_kernel<T, DP>, dim3(p.blocks, a.Hk), dim3(AR_ROWS * 32), 0, st, a, p);
+    e = launch_pdl(false, attn_rows_kernel<T, DP>, dim3(p.units, a.Hk), dim3(AR_WARPS * 32), smem, st, mk, mv, a, p);
+    if (e != cudaSuccess || p.slots == 0) return e;
+    return launch_pdl(true, attn_join_kernel<T, DP>, dim3(p.units, a.Hk), dim3(AR_ROWS * 32), 0, st, a, p);
 }
 
 }  // namespace
 
-// Few rows per sequence and key head: the row kernel, which packs the heads of a group and splits the
-// key axis. Otherwise 128-row tiles on the tensor cores (attn_tile.cu).
-static bool few_rows(const dn8_attention_args& a) { return a.Tq * (a.Hq / a.Hk) <= 32ll * a.B; }
+// Few rows per sequence and key head: the row kernel, which packs the heads of a group. Otherwise 128-row tiles on
+// the tensor cores (attn_tile.cu). A tile costs about as much however few of its rows are used, a block of 16 rows
+// reads all keys again (from L2) and pays a start and an end: up to 32 rows the row kernel, above that where
+// the keys are many. 16 heads in groups of 4, D = 64, row kernel and tiles: 48 rows over 24 x 2000 keys 35 and 74
+// us, over 64 x 500 52 and 62; 128 rows over 8 x 6000 51 and 77, over 24 x 2000 72 and 74, over 64 x 500 72 and 63;
+// 256 rows over 8 x 6000 90 and 78. 8 heads, 48 rows over 200 x 200 keys: 168 and 74.
+static bool few_rows(const dn8_attention_args& a) {
+    const int64_t rows = a.Tq * (a.Hq / a.Hk);
+    return rows <= 32ll * a.B || (rows <= 128ll * a.B && a.Tk >= 8 * rows);
+}
 
-size_t attention_work(const dn8_attention_args& a, int sms) { return few_rows(a) ? rows_work(a, rows_plan(a, sms)) : 0; }
+size_t attention_work(const dn8_attention_args& a, int sms) {
+    return few_rows(a) ? rows_work(a, rows_plan(a, sms)) : attention_tile_work(a, sms);
+}
 
 cudaError_t launch_attention(const dn8_attention_args& a, int sms, cudaStream_t st) {
-    if (!few_rows(a)) return launch_attention_tile(a, st);
+    if (!few_rows(a)) return launch_attention_tile(a, sms, st);
     const RowsPlan p = rows_plan(a, sms);
     if (a.type == DN8_F16) return head_pad(a.D) == 64 ? rows_go<__half, 64>(a, p, st) : rows_go<__half, 128>(a, p, st);
     return head_pad(a.D) == 64 ? rows_go<__nv_bfloat16, 64>(a, p, st) : rows_go<__nv_bfloat16, 128>(a, p, st);

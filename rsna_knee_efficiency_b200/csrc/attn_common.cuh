@@ -42,8 +42,13 @@ template <typename A> DN8_DEV Sequence sequence_of(const A& a, int b) {
 }
 
 // Block `unit` of the batch when every sequence is cut into ceil(len mul / per) blocks, len being its
-// queries (KEYS = false) or its keys. Called by one whole warp.
-template <bool KEYS, typename A> DN8_DEV Sequence find_block(const A& a, int unit, int mul, int per) {
+// queries (KEYS = false) or its keys, and every block into shares(queries, keys): blk then counts shares. Called
+// by one whole warp.
+struct OneShare {
+    DN8_DEV int operator()(int, int) const { return 1; }
+};
+template <bool KEYS, typename A, typename S = OneShare>
+DN8_DEV Sequence find_block(const A& a, int unit, int mul, int per, S shares = S()) {
     constexpr int BATCH = 4;                  // 32 sequences each, their offsets loaded together
     const int lane = threadIdx.x & 31;
     int run = 0;
@@ -66,7 +71,7 @@ template <bool KEYS, typename A> DN8_DEV Sequence find_block(const A& a, int uni
             const int nq = checked_len(q0[x], q1[x], a.Tq, a.err);
             int nk = checked_len(k0[x], k1[x], a.Tk, a.err);
             if (a.len_k != nullptr) nk = checked_len(0, kn[x], nk, a.err);
-            const int mine = static_cast<int>((static_cast<int64_t>(KEYS ? nk : nq) * mul + per - 1) / per);
+            const int mine = static_cast<int>((static_cast<int64_t>(KEYS ? nk : nq) * mul + per - 1) / per) * shares(nq, nk);
             int incl = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -92,15 +97,26 @@ template <bool KEYS, typename A> DN8_DEV Sequence find_block(const A& a, int uni
 // Key tiles of TILE keys that queries at positions p0 .. p1 see some key of: the tiles of the first
 // tokens, then those of the window. tile(t) for t = 0 .. count - 1.
 struct KeyTiles {
-    int first;         // tiles 0 .. first - 1: first tokens
+    int base, first;   // tiles base .. base + first - 1: first tokens (base = 0 unless cut)
     int start;         // then start, start + 1, ...
     int count;
-    DN8_DEV int tile(int t) const { return t < first ? t : start + t - first; }
+    DN8_DEV int tile(int t) const { return t < first ? base + t : start + t - first; }
+    DN8_DEV void cut(int b, int e) {                           // keep tile(b) .. tile(e - 1)
+        base += min(b, first);
+        start += max(0, b - first);
+        first = max(0, min(e, first) - b);
+        count = max(0, e - b);
+    }
 };
+// Keys that one of `rows` neighbouring queries sees, at most.
+template <typename A> DN8_DEV int seen_keys(const A& a, int rows, int nk) {
+    if (a.left < 0 || a.right < 0) return nk;
+    return min(nk, min(a.left, nk) + min(a.right, nk) + min(a.sinks, nk) + rows);
+}
 DN8_DEV KeyTiles key_tiles(int p0, int p1, int nk, int left, int right, int sinks, int tile) {
     const int hi = min(nk - 1, p1 + right), lo = max(0, p0 - left);
     KeyTiles k;
-    k.first = k.start = k.count = 0;
+    k.base = k.first = k.start = k.count = 0;
     if (hi < 0) return k;
     const int s = min(sinks, hi + 1);                          // first tokens that may be seen
     k.start = lo / tile;

@@ -33,6 +33,7 @@ constexpr int AF_REGS_SOFTMAX = 104, AF_REGS_OTHER = 64;
 // first loads. Asked for at the start, a piece waits behind a long one while others run out of work: four
 // sequences of 6144, causal, took 364 us instead of 317.
 constexpr int AF_AHEAD = 4;
+constexpr float AF_SHARE = 4.0f;                      // key tiles of a share, at least
 
 template <int DP> struct TileCfg {
     static constexpr int KST = DP == 64 ? 3 : 2, VST = DP == 64 ? 3 : 2;      // stages of K and V
@@ -50,11 +51,43 @@ DN8_DEV void pair_arrive(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) :
 struct TilePiece {
     Sequence seq;                                     // seq.b = -2: no more pieces
     int h, i0;                                        // query head, first query row
+    int share;                                        // where a share's results go, or -1: straight to the output
     KeyTiles all, own[2];                             // key tiles of the piece, and of each query tile
     // Query tile g's own are the piece's tiles u < lead[g] and from[g] <= u < to[g]. A tile whose first key is above
     // hic[g], or below loc[g] but above skc, or (with a key mask) every tile, needs a mask.
     int lead[2], from[2], to[2], hic[2], loc[2], skc;
 };
+
+// Shares of a piece's key tiles. Where the rows make fewer pieces than half the SMs (a few heads, or some hundreds
+// of queries over long caches), a piece whose walk is longer than an SM's part of all of them is cut. The
+// lengths are known to the GPU alone, so each CTA adds them up: pieces times the tiles that a piece sees at
+// most. A piece gets as many shares as whole parts fit into its sequence's, so all shares run side by side.
+// Uncut and cut, us: one head, 5627 queries and keys, D = 80, 178 and 60; two heads, 1905, D = 128, window of
+// 1450, 51 and 42; four heads, 4096, D = 64, 66 and 56; 64 queries of 4 heads over 20000 keys 113 and 30. A call whose
+// pieces turn out not to be cut pays 8 us for this and the join (12 heads, 4096: 105 and 114).
+struct TilePlan {
+    int sms;                                          // 0: nothing is cut
+    int units;                                        // pieces and shares, per head (a bound)
+    float* o;                                         // [share][256][DP], relative to the reference
+    float2* ml;                                       // [share][256] (reference, sum)
+    int4* rec;                                        // [share] first row, rows (0: not a piece's first share), shares
+};
+struct TileShares {
+    const dn8_attention_args& a;
+    float inv;                                        // 1 / tiles of a part, or 0: nothing is cut
+    DN8_DEV int tiles(int nq, int nk) const { return (seen_keys(a, min(nq, 2 * AT_TILE), nk) + AT_TILE - 1) / AT_TILE; }
+    DN8_DEV int operator()(int nq, int nk) const { return max(1, static_cast<int>(tiles(nq, nk) * inv)); }
+};
+DN8_DEV TileShares tile_shares(const dn8_attention_args& a, const TilePlan& plan) {      // (one whole warp)
+    TileShares s = {a, 0.0f};
+    float total = 0.0f;
+    for (int b = threadIdx.x & 31; b < a.B; b += 32) {
+        const Sequence q = sequence_of(a, b);
+        total += static_cast<float>((q.nq + 2 * AT_TILE - 1) / (2 * AT_TILE)) * static_cast<float>(s.tiles(q.nq, q.nk));
+    }
+    s.inv = fminf(static_cast<float>(plan.sms) / (warp_sum(total) * static_cast<float>(a.Hq)), 1.0f / AF_SHARE);
+    return s;
+}
 
 struct TileShared {
     uint64_t answer[2];                               // (16-byte aligned: first)
@@ -69,10 +102,10 @@ struct TileShared {
     int abort;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool CUT>
 __global__ void __launch_bounds__(AF_THREADS, 1)
 attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                 const __grid_constant__ CUtensorMap mv, const dn8_attention_args a) {
+                 const __grid_constant__ CUtensorMap mv, const dn8_attention_args a, const TilePlan plan) {
     using C = TileCfg<DP>;
     static_assert(sizeof(TileShared) <= 3072, "shared state");
     extern __shared__ uint8_t smem_raw[];
@@ -123,16 +156,30 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         return sh.piece[n & 1].seq.b >= 0;
     };
 
+    if (CUT) griddep_launch_dependents();
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AF_REGS_OTHER));
         if (warp == 18) {
             // ---------------- pieces, and masked rows of V ----------------
             int block = blockIdx.x, asked = 0, vc = 0;
+            const TileShares shares = CUT ? tile_shares(a, plan) : TileShares{a, 0.0f};
             TilePiece pc;
             // Looks block after block up until one holds a piece: false after the last.
             auto look = [&]() -> bool {
                 while (block >= 0) {
-                    pc.seq = find_block<false>(a, block / a.Hq, 1, 2 * AT_TILE);
+                    if (CUT) {
+                        pc.seq = find_block<false>(a, block / a.Hq, 1, 2 * AT_TILE, shares);
+                        pc.share = block;
+                        // (behind the last piece there are some 148 blocks with nothing to do: one of them ends this CTA's
+                        // search, blocks that were not asked for start by themselves. Each one more held V up for
+                        // 2 us.)
+                        if (pc.seq.b < 0) {
+                            if (lane == 0) plan.rec[block] = make_int4(0, 0, 0, 0);
+                            return false;
+                        }
+                    } else {
+                        pc.seq = find_block<false>(a, block / a.Hq, 1, 2 * AT_TILE);
+                    }
                     pc.h = block % a.Hq;
                     if (pc.seq.b >= 0) return true;   // (the bound on the blocks may be too high)
                     if (lane == 0) {
@@ -152,21 +199,41 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                     pc.seq.b = -2;
                 } else {
                     const int nq = pc.seq.nq, nk = pc.seq.nk, off = nk - nq;
+                    const int cuts = CUT ? shares(nq, nk) : 1, nth = cuts == 1 ? pc.seq.blk : pc.seq.blk / cuts;
+                    const int mine = pc.seq.blk - nth * cuts;
                     // last blocks first: with an open left side they are the longest
-                    pc.i0 = ((nq - 1) / (2 * AT_TILE) - pc.seq.blk) * 2 * AT_TILE;
+                    pc.i0 = ((nq - 1) / (2 * AT_TILE) - nth) * 2 * AT_TILE;
                     const int end = min(pc.i0 + 2 * AT_TILE, nq);
-                    pc.all = key_tiles(pc.i0 + off, end - 1 + off, nk, left, right, a.sinks, AT_TILE);
+                    const KeyTiles whole = key_tiles(pc.i0 + off, end - 1 + off, nk, left, right, a.sinks, AT_TILE);
+                    pc.all = whole;
+                    int u0 = 0, n_ = whole.count;     // this share's of the piece's tiles: n_ from u0 on
+                    if (CUT) {
+                        const bool first = cuts > 1 && mine == 0;
+                        if (lane == 0) plan.rec[pc.share] = make_int4(pc.seq.q0 + pc.i0, first ? end - pc.i0 : 0, cuts, 0);
+                        if (cuts > 1) {
+                            // (tiles < 2^21, and at most one share per SM)
+                            u0 = mine * whole.count / cuts;
+                            n_ = (mine + 1) * whole.count / cuts - u0;
+                            pc.all.cut(u0, u0 + n_);
+                        } else {
+                            pc.share = -1;
+                        }
+                    }
                     pc.skc = a.sinks - AT_TILE;
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
                         const int p0 = pc.i0 + g * AT_TILE + off, p1 = min(pc.i0 + (g + 1) * AT_TILE, end) - 1 + off;
-                        KeyTiles& own = pc.own[g];
-                        own = key_tiles(p0, p1, nk, left, right, a.sinks, AT_TILE);
-                        if (p0 > p1) own.count = 0;
-                        // (the piece's tiles are 0 .. first - 1 and start ..; a query tile's own are among them)
-                        pc.lead[g] = own.count > 0 ? own.first : 0;
-                        pc.from[g] = own.start < pc.all.first ? own.start : pc.all.first + own.start - pc.all.start;
-                        pc.to[g] = own.count > 0 ? pc.from[g] + own.count - own.first : 0;
+                        KeyTiles own = key_tiles(p0, p1, nk, left, right, a.sinks, AT_TILE);
+                        if (p0 > p1) own.first = own.count = 0;
+                        // (a query tile's own are among the piece's)
+                        const int from = own.count > 0 ? whole.first + own.start - whole.start : 0;
+                        pc.lead[g] = max(0, min(own.first - u0, n_));
+                        pc.from[g] = max(0, min(from - u0, n_));
+                        pc.to[g] = max(0, min(from + own.count - own.first - u0, n_));
+                        pc.own[g].base = pc.all.base;
+                        pc.own[g].first = pc.lead[g];
+                        pc.own[g].start = pc.all.tile(pc.from[g]);
+                        pc.own[g].count = pc.lead[g] + max(0, pc.to[g] - pc.from[g]);
                         pc.hic[g] = min(nk - 1, p0 + right) - (AT_TILE - 1);
                         pc.loc[g] = p1 - left;
                     }
@@ -356,7 +423,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         bool ok = true;
         for (int np = 0; ok && begin_piece(np); ++np) {
             const TilePiece& pc = sh.piece[np & 1];
-            const int tiles = pc.own[g].count, turn = pc.own[g].first - 1, hic = pc.hic[g], loc = pc.loc[g], skc = pc.skc;
+            const int tiles = pc.own[g].count, turn = pc.own[g].base + pc.own[g].first - 1, hic = pc.hic[g], loc = pc.loc[g], skc = pc.skc;
             int t = pc.own[g].tile(0);
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};      // references (times sc), this thread's sums
             for (int n = 0; n < tiles; ++n) {
@@ -517,6 +584,8 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             T* out = static_cast<T*>(a.out) + at * a.o_stride_t + static_cast<int64_t>(h) * a.o_stride_h;
             const uint32_t tq = tmem + C::O0 + g * DP + half * (DP / 2) + (static_cast<uint32_t>(quad * 32) << 16);
             const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
+            const bool cut = CUT && pc.share >= 0;
+            const int64_t slot = static_cast<int64_t>(pc.share) * 2 * AT_TILE + g * AT_TILE + quad * 32 + lane;
 #pragma unroll 1
             for (int c = 0; c < DP / 32; ++c) {
                 uint32_t o[16] = {};
@@ -525,6 +594,12 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                     tmem_wait_ld(o);
                 }
                 const int d = half * (DP / 2) + 16 * c;
+                if (cut) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (live) *reinterpret_cast<uint4*>(plan.o + slot * DP + d + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 16; e += 8) {
                     float v[8];
@@ -538,7 +613,8 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.oempty[g]);
             }
-            if (live && half == 0 && a.lse != nullptr)
+            if (cut && live && half == 0) plan.ml[slot] = make_float2(ms, ls);
+            if (!cut && live && half == 0 && a.lse != nullptr)
                 a.lse[at * a.Hq + h] = ls > 0.0f ? (ms + __log2f(ls)) * ATT_LN2 : -INFINITY;
         }
         // A warp that gave up arrives once more, so that its partner's barrier completes; the partner then
@@ -551,6 +627,99 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         tc_fence_after();
         tmem_free(tmem, 512);
     }
+}
+
+// Adds the shares of the cut pieces: weights 2^(m_s - max m), 32 shares at a time, then a warp's lanes hold DP / 32
+// elements each. Every warp reads the records and takes one row in `step` of those that they name (a block per
+// piece and some rows spent 20 us on 11520 blocks with nothing to do, where 192 pieces had not been cut).
+constexpr int AF_JOIN_WARPS = 16;
+template <typename T, int DP>
+DN8_DEV void join_row(const dn8_attention_args& a, const TilePlan& plan, int block, int cuts, int64_t row, int r) {
+    const int lane = threadIdx.x & 31, h = block % a.Hq;
+    // (share s of the same piece and head: block + s Hq)
+    auto slot = [&](int s) { return (static_cast<int64_t>(block) + static_cast<int64_t>(s) * a.Hq) * (2 * AT_TILE) + r; };
+    float mm = -INFINITY, lv = 0.0f, ov[DP / 32] = {};
+    for (int s = lane; s < cuts; s += 32) mm = fmaxf(mm, plan.ml[slot(s)].x);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    for (int s0 = 0; s0 < cuts; s0 += 32) {
+        float w = 0.0f;
+        if (s0 + lane < cuts) {
+            const float2 ml = plan.ml[slot(s0 + lane)];
+            w = ex2(ml.x - ref);
+            lv = fmaf(w, ml.y, lv);
+        }
+        const int ns = min(32, cuts - s0);
+#pragma unroll 8
+        for (int s = 0; s < ns; ++s) {
+            float v[DP / 32];
+            load_f32(plan.o + slot(s0 + s) * DP + lane * (DP / 32), v);
+            const float ws = __shfl_sync(0xffffffffu, w, s);
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e) ov[e] = fmaf(ws, v[e], ov[e]);
+        }
+    }
+    lv = warp_sum(lv);
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) ov[e] = lv > 0.0f ? ov[e] / lv : 0.0f;
+    if (lane * (DP / 32) < a.D)
+        store_f32(static_cast<T*>(a.out) + row * a.o_stride_t + h * a.o_stride_h + lane * (DP / 32), ov);
+    if (lane == 0 && a.lse != nullptr) a.lse[row * a.Hq + h] = lv > 0.0f ? (mm + log2f(lv)) * ATT_LN2 : -INFINITY;
+}
+template <typename T, int DP>
+__global__ void __launch_bounds__(AF_JOIN_WARPS * 32) attn_tile_join_kernel(const dn8_attention_args a, const TilePlan plan) {
+    constexpr int BATCH = 4;                          // 32 records each, loaded together
+    const int lane = threadIdx.x & 31, blocks = plan.units * a.Hq, step = gridDim.x * AF_JOIN_WARPS;
+    int next = blockIdx.x * AF_JOIN_WARPS + (threadIdx.x >> 5), run = 0;
+    griddep_wait();
+    for (int base = 0; base < blocks; base += 32 * BATCH) {
+        int4 rec[BATCH];
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+            const int block = base + 32 * x + lane;
+            rec[x] = block < blocks ? plan.rec[block] : make_int4(0, 0, 0, 0);
+            // (offsets that go back and forth may ask for more shares than there is room for, and a kernel that gave
+            // up leaves records behind that say nothing: rows and shares are kept inside the tensors)
+            rec[x].z = min(rec[x].z, (blocks - 1 - block) / a.Hq + 1);
+            if (rec[x].x < 0 || rec[x].y < 0 || rec[x].y > 2 * AT_TILE || static_cast<int64_t>(rec[x].x) + rec[x].y > a.Tq)
+                rec[x].y = 0;
+        }
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+            int incl = rec[x].y;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const int total = __shfl_sync(0xffffffffu, incl, 31);
+            for (; next < run + total; next += step) {
+                const int src = __ffs(__ballot_sync(0xffffffffu, next < run + incl)) - 1;
+                const int r = next - run - __shfl_sync(0xffffffffu, incl - rec[x].y, src);
+                const int64_t row = static_cast<int64_t>(__shfl_sync(0xffffffffu, rec[x].x, src)) + r;
+                join_row<T, DP>(a, plan, base + 32 * x + src, __shfl_sync(0xffffffffu, rec[x].z, src), row, r);
+            }
+            run += total;
+        }
+    }
+}
+
+// (a bound on the pieces: every sequence may leave one unfilled)
+static int64_t tile_pieces(const dn8_attention_args& a) { return a.Tq / (2 * AT_TILE) + (a.B < a.Tq ? a.B : a.Tq); }
+static TilePlan tile_plan(const dn8_attention_args& a, int sms) {
+    TilePlan p = {};
+    const int64_t pieces = tile_pieces(a);
+    if (a.Tq * a.Hq < sms * AT_TILE && pieces * a.Hq < 2ll * sms && a.Tk >= 2 * AF_SHARE * AT_TILE) {
+        p.sms = sms;
+        // sum of max(1, tiles / part) <= pieces + sms / Hq (and one for the rounding of the sums)
+        p.units = static_cast<int>(pieces) + sms / a.Hq + 1;
+    }
+    return p;
+}
+size_t attention_tile_work(const dn8_attention_args& a, int sms) {
+    return static_cast<size_t>(tile_plan(a, sms).units) * a.Hq * 2 * AT_TILE * ((a.D <= 64 ? 64 : 128) + 2) * sizeof(float) +
+           static_cast<size_t>(tile_plan(a, sms).units) * a.Hq * sizeof(int4);
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -580,24 +749,30 @@ cudaError_t make_head_map(CUtensorMap* map, const void* base, int type, int64_t 
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <typename T, int DP> static cudaError_t tile_go(const dn8_attention_args& a, cudaStream_t st) {
+template <typename T, int DP> static cudaError_t tile_go(const dn8_attention_args& a, int sms, cudaStream_t st) {
     CUtensorMap mq = {}, mk = {}, mv = {};
     cudaError_t e = make_head_map(&mq, a.q, a.type, a.Tq, a.Hq, a.D, a.q_stride_t, a.q_stride_h);
     if (e == cudaSuccess && a.Tk > 0) e = make_head_map(&mk, a.k, a.type, a.Tk, a.Hk, a.D, a.k_stride_t, a.k_stride_h);
     if (e == cudaSuccess && a.Tk > 0) e = make_head_map(&mv, a.v, a.type, a.Tk, a.Hk, a.D, a.v_stride_t, a.v_stride_h);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(attn_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileCfg<DP>::SMEM);
+    TilePlan plan = tile_plan(a, sms);
+    const auto kernel = plan.sms > 0 ? attn_tile_kernel<T, DP, true> : attn_tile_kernel<T, DP, false>;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileCfg<DP>::SMEM);
     if (e != cudaSuccess) return e;
-    // a bound on the blocks: every sequence may leave one unfilled
-    const int64_t blocks = (a.Tq / (2 * AT_TILE) + (a.B < a.Tq ? a.B : a.Tq)) * a.Hq;
+    const int64_t blocks = (plan.sms > 0 ? plan.units : tile_pieces(a)) * a.Hq;
     if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-    return launch_pdl(false, attn_tile_kernel<T, DP>, dim3(static_cast<unsigned>(blocks)), dim3(AF_THREADS),
-                      TileCfg<DP>::SMEM, st, mq, mk, mv, a);
+    plan.o = static_cast<float*>(a.work);
+    plan.ml = reinterpret_cast<float2*>(plan.o + blocks * 2 * AT_TILE * DP);
+    plan.rec = reinterpret_cast<int4*>(plan.ml + blocks * 2 * AT_TILE);
+    e = launch_pdl(false, kernel, dim3(static_cast<unsigned>(blocks)), dim3(AF_THREADS), TileCfg<DP>::SMEM,
+                   st, mq, mk, mv, a, plan);
+    if (e != cudaSuccess || plan.sms == 0) return e;
+    return launch_pdl(true, attn_tile_join_kernel<T, DP>, dim3(2 * sms), dim3(AF_JOIN_WARPS * 32), 0, st, a, plan);
 }
 
-cudaError_t launch_attention_tile(const dn8_attention_args& a, cudaStream_t st) {
-    if (a.type == DN8_F16) return a.D <= 64 ? tile_go<__half, 64>(a, st) : tile_go<__half, 128>(a, st);
-    return a.D <= 64 ? tile_go<__nv_bfloat16, 64>(a, st) : tile_go<__nv_bfloat16, 128>(a, st);
+cudaError_t launch_attention_tile(const dn8_attention_args& a, int sms, cudaStream_t st) {
+    if (a.type == DN8_F16) return a.D <= 64 ? tile_go<__half, 64>(a, sms, st) : tile_go<__half, 128>(a, sms, st);
+    return a.D <= 64 ? tile_go<__nv_bfloat16, 64>(a, sms, st) : tile_go<__nv_bfloat16, 128>(a, sms, st);
 }
 
 }  // namespace dn8

@@ -69,7 +69,8 @@ cudaError_t launch_layer_norm_bwd(const dn8_layer_norm_bwd_args& a, cudaStream_t
 size_t layer_norm_bwd_work(int C);
 cudaError_t launch_rope(const dn8_rope_args& a, int sms, cudaStream_t st);
 cudaError_t launch_attention(const dn8_attention_args& a, int sms, cudaStream_t st);
-cudaError_t launch_attention_tile(const dn8_attention_args& a, cudaStream_t st);
+cudaError_t launch_attention_tile(const dn8_attention_args& a, int sms, cudaStream_t st);
+size_t attention_tile_work(const dn8_attention_args& a, int sms);
 size_t attention_work(const dn8_attention_args& a, int sms);
 cudaError_t launch_attention_bwd(const dn8_attention_bwd_args& a, int sms, cudaStream_t st);
 size_t attention_bwd_work(const dn8_attention_bwd_args& a, int sms);

@@ -366,7 +366,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                              _ptr(cu_q), _ptr(cu_k), _ptr(len_k), _ptr(keep), _ptr(err), None, sq[0], sk[0], *gs,
                              *strides, *os, *outs, *mask)
     lib = nat.lib()
-    nbytes = lib.dn8_attention_bwd_work(a)
+    nbytes = _bytes_of(lib.dn8_attention_bwd_work, a, dev)
     if nbytes > 0:
         work = _workspace(c, nbytes, work, dev, stream)
         a.work = work.data_ptr()
