@@ -69,11 +69,44 @@ template <int DP> struct BwdCfg {
 // S tiles: the sums are dv (ACC0) and dk (ACC1), or dq (ACC1)
 template <int DP> DN8_DEV constexpr int s_tiles(bool kv) { return kv && DP == 128 ? 1 : 2; }
 
-// Shares of the walks over the first tokens' key tiles (shares = 1: none are cut).
+// Shares of the walks over key tiles (dk, dv). Under a window, those over the first tokens' tiles are cut
+// (split_blocks > 0). Where the keys make few pieces and a key head has several query heads, every walk longer than
+// two thirds of an SM's part of all steps is (sms > 0): the lengths are known to the GPU alone, so each CTA adds
+// them up. A step of dk, dv counts KV_STEP steps of dq (five products, not three). Uncut and cut, us: 3022 tokens,
+// 8 heads in groups of 4, D = 80, left of 479: 220 and 134 (147 in parts of an SM's whole share); 719 tokens, D = 128,
+// the same heads: 64 and 43. Walks of dq are never the longest there, and short walks are not cut: 900 tokens, 4
+// heads of their own, D = 128, took 30 us uncut and 49 cut.
 struct BwdPlan {
-    int kv_blocks, split_blocks, tiles, shares;
-    float* part;                              // [sequence][tile][key head][share][dv, dk][128][DP]
+    int kv_blocks, split_blocks, tiles, shares, sms;
+    int blocks, records;                      // blocks in all; those that may be shares
+    float* part;                              // [block][dv, dk][128][DP]
+    int4* rec;                                // [block] first key row; rows (0: not a piece's first share) + 256 head;
+                                              // shares; blocks from one share to the next
 };
+constexpr float KV_STEP = 1.5f, AB_SHARE = 8.0f;      // AB_SHARE: steps of a share, at least
+constexpr float AB_PARTS = 1.5f;              // parts per SM
+// Tiles of 128 that the rows of a tile meet on an axis of n, the first tokens aside (n < 2^28).
+template <typename A> DN8_DEV int met_tiles(const A& a, int n) {
+    const int met = a.left < 0 || a.right < 0 ? n : min(n, min(a.left, n) + min(a.right, n) + AT_TILE);
+    return (met + AT_TILE - 1) / AT_TILE;
+}
+struct BwdShares {
+    const dn8_attention_bwd_args& a;
+    float inv;                                // 1 / steps of a part, or 0: nothing is cut
+    DN8_DEV int operator()(int nq, int) const { return max(1, __float2int_rn(met_tiles(a, nq) * (a.Hq / a.Hk) * inv)); }
+};
+DN8_DEV BwdShares bwd_shares(const dn8_attention_bwd_args& a, const BwdPlan& plan) {      // (one whole warp)
+    BwdShares s = {a, 0.0f};
+    if (plan.sms == 0) return s;
+    float total = 0.0f;
+    for (int b = threadIdx.x & 31; b < a.B; b += 32) {
+        const Sequence q = sequence_of(a, b);
+        total += KV_STEP * static_cast<float>((q.nk + AT_TILE - 1) / AT_TILE) * met_tiles(a, q.nq) +
+                 static_cast<float>((q.nq + AT_TILE - 1) / AT_TILE) * met_tiles(a, q.nk);
+    }
+    s.inv = fminf(AB_PARTS * KV_STEP * static_cast<float>(plan.sms) / (warp_sum(total) * static_cast<float>(a.Hq)), 1.0f / AB_SHARE);
+    return s;
+}
 
 struct BwdPiece {
     Sequence seq;                             // seq.b = -2: no more pieces
@@ -271,7 +304,7 @@ DN8_DEV bool bwd_rows(const dn8_attention_bwd_args& a, BwdShared& sh, const BwdP
     return true;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool CUT>
 __global__ void __launch_bounds__(AB_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
@@ -340,23 +373,30 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             // ---------------- pieces ----------------
             int block = blockIdx.x, asked = 0;
             BwdPiece pc;
+            const BwdShares shares = CUT ? bwd_shares(a, plan) : BwdShares{a, 0.0f};
             for (int n = 0;;) {
                 pc.seq.b = -2;
                 pc.steps = pc.tile0 = pc.hx = 0;
                 pc.turn = pc.back = pc.share = -1;
-                int begin = 0;                           // which share
+                int cuts = 1, mine = 0;                  // shares, and which one
                 if (block >= 0) {
                     pc.kv = block < plan.kv_blocks;
                     if (block < plan.split_blocks) {
                         // share s of the walk over tile t of sequence b and key head h: block = ((b tiles + t) Hk + h)
                         // shares + s
-                        const int s = block % plan.shares, x = block / plan.shares;
+                        const int x = block / plan.shares;
+                        cuts = plan.shares;
+                        mine = block - x * cuts;
                         pc.seq = sequence_of(a, x / a.Hk / plan.tiles);
                         pc.seq.blk = x / a.Hk % plan.tiles;
                         pc.h = x % a.Hk;
-                        pc.share = block;
                         if (pc.seq.blk * AT_TILE >= pc.seq.nk) pc.seq.b = -1;
-                        begin = s;
+                    } else if (CUT && pc.kv) {
+                        pc.seq = find_block<true>(a, block / a.Hk, 1, AT_TILE, shares);
+                        pc.h = block % a.Hk;
+                        if (pc.seq.b >= 0) cuts = shares(pc.seq.nq, pc.seq.nk);
+                        mine = pc.seq.blk % cuts;
+                        pc.seq.blk /= cuts;
                     } else if (pc.kv) {
                         const int x = block - plan.split_blocks;
                         pc.seq = find_block<true>(a, x / a.Hk, 1, AT_TILE);
@@ -366,6 +406,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                         const int x = block - plan.kv_blocks;
                         pc.seq = find_block<false>(a, x / a.Hq, 1, AT_TILE);
                         pc.h = x % a.Hq;
+                    }
+                    if (cuts > 1) pc.share = block;
+                    if (block < plan.records && lane == 0) {
+                        const int r0 = pc.seq.blk * AT_TILE;
+                        const bool first = pc.seq.b >= 0 && mine == 0 && cuts > 1;
+                        plan.rec[block] = make_int4(pc.seq.k0 + r0, (first ? min(AT_TILE, pc.seq.nk - r0) : 0) + 256 * pc.h, cuts,
+                                                    CUT ? a.Hk : 1);
                     }
                 }
                 if (pc.seq.b >= 0) {
@@ -378,10 +425,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                         const int hi = pc.r0 < a.sinks ? nq - 1 : min(nq - 1, jl + left - off);
                         const int first = lo / AT_TILE, per = lo <= hi ? hi / AT_TILE - first + 1 : 1;
                         pc.steps = lo <= hi ? per * G : 0;
-                        if (pc.share >= 0) {             // steps [s n / shares, (s + 1) n / shares)
-                            const int s = begin, n_ = pc.steps;
-                            begin = static_cast<int>(static_cast<int64_t>(s) * n_ / plan.shares);
-                            pc.steps = static_cast<int>(static_cast<int64_t>(s + 1) * n_ / plan.shares) - begin;
+                        int begin = 0;
+                        if (cuts > 1) {                  // steps [s n / shares, (s + 1) n / shares)
+                            const int n_ = pc.steps;
+                            begin = static_cast<int>(static_cast<int64_t>(mine) * n_ / cuts);
+                            pc.steps = static_cast<int>(static_cast<int64_t>(mine + 1) * n_ / cuts) - begin;
                         }
                         pc.tile0 = first + begin % per;
                         pc.hx = pc.h * G + begin / per;
@@ -660,34 +708,63 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     }
 }
 
-// dk, dv of the first tokens' key tiles: the shares' sums, in order. One block per 16 rows of a tile and key
-// head; thread: 4 elements of a row.
+// The sums of cut walks: the shares', in order. Every warp reads the records and takes one row in `step` of those
+// that they name; a lane holds DP / 32 elements.
+constexpr int AB_JOIN_WARPS = 16;
 template <typename T, int DP>
-__global__ void __launch_bounds__(16 * (DP / 4)) attn_bwd_join_kernel(const dn8_attention_bwd_args a, const BwdPlan plan) {
-    const int x = blockIdx.x / (AT_TILE / 16), h = x % a.Hk, tile = x / a.Hk % plan.tiles, b = x / a.Hk / plan.tiles;
-    const int row = blockIdx.x % (AT_TILE / 16) * 16 + threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
-    const int k0 = a.cu_k[b];
-    int nk = checked_len(k0, a.cu_k[b + 1], a.Tk, a.err);
-    if (a.len_k != nullptr) nk = checked_len(0, a.len_k[b], nk, a.err);
-    const int j = tile * AT_TILE + row;
+__global__ void __launch_bounds__(AB_JOIN_WARPS * 32) attn_bwd_join_kernel(const dn8_attention_bwd_args a, const BwdPlan plan) {
+    constexpr int BATCH = 4;                          // 32 records each, loaded together
+    const int lane = threadIdx.x & 31, step = gridDim.x * AB_JOIN_WARPS, d = lane * (DP / 32);
+    int next = blockIdx.x * AB_JOIN_WARPS + (threadIdx.x >> 5), run = 0;
     griddep_wait();
-    if (j >= nk || d >= a.D) return;
-    const int64_t at = static_cast<int64_t>(k0) + j;
+    for (int base = 0; base < plan.records; base += 32 * BATCH) {
+        int4 rec[BATCH];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int y = 0; y < plan.shares; ++y) {
-            const float4 v = *reinterpret_cast<const float4*>(
-                plan.part + (((static_cast<size_t>(x) * plan.shares + y) * 2 + k) * AT_TILE + row) * DP + d);
-            s[0] += v.x;
-            s[1] += v.y;
-            s[2] += v.z;
-            s[3] += v.w;
+        for (int x = 0; x < BATCH; ++x) {
+            const int block = base + 32 * x + lane;
+            rec[x] = block < plan.records ? plan.rec[block] : make_int4(0, 0, 0, 0);
         }
-        T* dst = k == 0 ? static_cast<T*>(a.dv) + at * a.dv_stride_t + h * a.dv_stride_h
-                        : static_cast<T*>(a.dk) + at * a.dk_stride_t + h * a.dk_stride_h;
-        store_f32(dst + d, s);
+#pragma unroll
+        for (int x = 0; x < BATCH; ++x) {
+            // (offsets that go back and forth may ask for more shares than there is room for, and a kernel that gave
+            // up leaves records behind that say nothing: rows and shares are kept inside the tensors)
+            const int4 c = rec[x];
+            const bool sound = c.x >= 0 && c.y >= 0 && (c.y & 255) <= AT_TILE && c.w >= 1 && (c.y >> 8) < a.Hk &&
+                               static_cast<int64_t>(c.x) + (c.y & 255) <= a.Tk;
+            const int mine = sound ? c.y & 255 : 0;
+            int incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const int total = __shfl_sync(0xffffffffu, incl, 31);
+            for (; next < run + total; next += step) {
+                const int src = __ffs(__ballot_sync(0xffffffffu, next < run + incl)) - 1;
+                const int r = next - run - __shfl_sync(0xffffffffu, incl - mine, src);
+                const int64_t row = static_cast<int64_t>(__shfl_sync(0xffffffffu, c.x, src)) + r;
+                const int from = __shfl_sync(0xffffffffu, c.w, src), h = __shfl_sync(0xffffffffu, c.y, src) >> 8;
+                const int block = base + 32 * x + src;
+                const int cuts = min(__shfl_sync(0xffffffffu, c.z, src), (plan.records - 1 - block) / from + 1);
+                const float* p = plan.part + (static_cast<size_t>(block) * 2 * AT_TILE + r) * DP + d;
+                float s[2][DP / 32] = {};
+#pragma unroll 4
+                for (int y = 0; y < cuts; ++y) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float v[DP / 32];
+                        load_f32(p + (static_cast<size_t>(y) * from * 2 + k) * AT_TILE * DP, v);
+#pragma unroll
+                        for (int e = 0; e < DP / 32; ++e) s[k][e] += v[e];
+                    }
+                }
+                if (d < a.D) {
+                    store_f32(static_cast<T*>(a.dv) + row * a.dv_stride_t + h * a.dv_stride_h + d, s[0]);
+                    store_f32(static_cast<T*>(a.dk) + row * a.dk_stride_t + h * a.dk_stride_h + d, s[1]);
+                }
+            }
+            run += total;
+        }
     }
 }
 
@@ -698,12 +775,17 @@ static BwdPlan bwd_plan(const dn8_attention_bwd_args& a, int sms) {
     BwdPlan p = {};
     p.shares = 1;
     p.tiles = 1;
-    if (a.left >= 0 && a.sinks > 0 && a.Tk > 0 && a.Tq > 0) {
-        const int64_t G = a.Hq / a.Hk;
+    // bounds on the tiles: every sequence may leave one unfilled
+    int64_t kt = a.Tk / AT_TILE + (a.B < a.Tk ? a.B : a.Tk), qt = a.Tq / AT_TILE + (a.B < a.Tq ? a.B : a.Tq);
+    const int64_t G = a.Hq / a.Hk, width = a.left < 0 || a.right < 0 ? a.Tq : static_cast<int64_t>(a.left) + a.right + AT_TILE;
+    if (G > 1 && 2 * a.Tk * a.Hk < sms * AT_TILE && G * (width < a.Tq ? width : a.Tq) >= 20 * AT_TILE && kt * a.Hk < 4ll * sms) {
+        // sum of max(1, steps / part), rounded, <= pieces + AB_PARTS sms / Hk (and one for the rounding of the sums)
+        p.sms = sms;
+        kt += static_cast<int64_t>(AB_PARTS * sms) / a.Hk + 1;
+    } else if (a.left >= 0 && a.sinks > 0 && a.Tk > 0 && a.Tq > 0) {
         const int64_t tiles = (static_cast<int64_t>(a.sinks < a.Tk ? a.sinks : a.Tk) + AT_TILE - 1) / AT_TILE;
         const int64_t all = G * (a.Tq / a.B / AT_TILE + 1);
-        const int64_t width = static_cast<int64_t>(a.left) + (a.right < 0 ? a.Tq / a.B : a.right) + AT_TILE;
-        const int64_t others = G * (width / AT_TILE + 1);
+        const int64_t others = G * ((static_cast<int64_t>(a.left) + (a.right < 0 ? a.Tq / a.B : a.right) + AT_TILE) / AT_TILE + 1);
         const int64_t walks = a.B * tiles * a.Hk;
         int64_t s = (all + others - 1) / others;
         const int64_t fill = (2ll * sms + walks - 1) / walks;
@@ -714,6 +796,14 @@ static BwdPlan bwd_plan(const dn8_attention_bwd_args& a, int sms) {
             p.split_blocks = static_cast<int>(walks * p.shares);
         }
     }
+    const int64_t kv = kt * a.Hk + p.split_blocks, all = kv + qt * a.Hq;
+    if (all > 0x7FFFFFFFll) {
+        p.blocks = -1;
+        return p;
+    }
+    p.kv_blocks = static_cast<int>(kv);
+    p.blocks = static_cast<int>(all);
+    p.records = p.sms > 0 ? p.kv_blocks : p.split_blocks;
     return p;
 }
 static size_t bwd_stat_bytes(const dn8_attention_bwd_args& a) {
@@ -722,7 +812,7 @@ static size_t bwd_stat_bytes(const dn8_attention_bwd_args& a) {
 
 size_t attention_bwd_work(const dn8_attention_bwd_args& a, int sms) {
     const int DP = a.D <= 64 ? 64 : 128;
-    return bwd_stat_bytes(a) + static_cast<size_t>(bwd_plan(a, sms).split_blocks) * 2 * AT_TILE * DP * sizeof(float);
+    return bwd_stat_bytes(a) + static_cast<size_t>(bwd_plan(a, sms).records) * (2 * AT_TILE * DP * sizeof(float) + sizeof(int4));
 }
 
 template <typename T, int DP> static cudaError_t bwd_go(const dn8_attention_bwd_args& a, int sms, cudaStream_t st) {
@@ -737,26 +827,22 @@ template <typename T, int DP> static cudaError_t bwd_go(const dn8_attention_bwd_
         if (e == cudaSuccess) e = make_head_map(&mv, a.v, a.type, a.Tk, a.Hk, a.D, a.v_stride_t, a.v_stride_h);
     }
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(attn_bwd_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdCfg<DP>::SMEM);
-    if (e != cudaSuccess) return e;
     BwdPlan plan = bwd_plan(a, sms);
-    // bounds on the tiles: every sequence may leave one unfilled
-    const int64_t kt = (a.Tk / AT_TILE + (a.B < a.Tk ? a.B : a.Tk)) * a.Hk + plan.split_blocks;
-    const int64_t qt = (a.Tq / AT_TILE + (a.B < a.Tq ? a.B : a.Tq)) * a.Hq;
-    if (kt + qt > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-    plan.kv_blocks = static_cast<int>(kt);
+    const auto kernel = plan.sms > 0 ? attn_bwd_kernel<T, DP, true> : attn_bwd_kernel<T, DP, false>;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdCfg<DP>::SMEM);
+    if (e != cudaSuccess) return e;
+    if (plan.blocks < 0) return cudaErrorInvalidValue;
     plan.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + bwd_stat_bytes(a));
+    plan.rec = reinterpret_cast<int4*>(plan.part + static_cast<size_t>(plan.records) * 2 * AT_TILE * DP);
     if (a.Tq > 0) {
         e = launch_pdl(false, attn_bwd_prep_kernel<T, DP / 8>, dim3(static_cast<unsigned>((a.Tq + 31) / 32), a.Hq),
                        dim3(32 * (DP / 8)), 0, st, a);
         if (e != cudaSuccess) return e;
     }
-    e = launch_pdl(a.Tq > 0, attn_bwd_kernel<T, DP>, dim3(static_cast<unsigned>(kt + qt)), dim3(AB_THREADS),
+    e = launch_pdl(a.Tq > 0, kernel, dim3(static_cast<unsigned>(plan.blocks)), dim3(AB_THREADS),
                    BwdCfg<DP>::SMEM, st, mq, mk, mv, mdo, a, plan);
-    if (e != cudaSuccess || plan.shares == 1) return e;
-    return launch_pdl(true, attn_bwd_join_kernel<T, DP>,
-                      dim3(static_cast<unsigned>(plan.split_blocks / plan.shares * (AT_TILE / 16))), dim3(16 * (DP / 4)), 0, st,
-                      a, plan);
+    if (e != cudaSuccess || plan.records == 0) return e;
+    return launch_pdl(true, attn_bwd_join_kernel<T, DP>, dim3(2 * sms), dim3(AB_JOIN_WARPS * 32), 0, st, a, plan);
 }
 
 cudaError_t launch_attention_bwd(const dn8_attention_bwd_args& a, int sms, cudaStream_t st) {
