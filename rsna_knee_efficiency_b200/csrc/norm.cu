@@ -15,8 +15,9 @@
 
 namespace dn8 {
 
-// Sum of one value per thread over a team of TPR threads; every thread gets the same sum. `red`
-// holds a float per warp and is free for the next call after the second barrier.
+// Sums of values per thread over a team of TPR threads; every thread gets the same ones. `red`, a float per value
+// and warp, is the team's, and free once the team has passed another barrier: two calls in a row use two of them.
+// (One barrier per sum, of the team alone, not two of the block: 27056 rows of 1848 fp32 with a residual 136 -> 120 us.)
 // Teams of less than a warp do not wait for one another.
 template <int TPR> DN8_DEV float lanes_sum(float v) {
     if (TPR >= 32) return warp_sum(v);
@@ -25,35 +26,36 @@ template <int TPR> DN8_DEV float lanes_sum(float v) {
     for (int k = TPR / 2; k > 0; k >>= 1) v += __shfl_xor_sync(mask, v, k);
     return v;
 }
+template <int TPR> DN8_DEV void team_barrier() {
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / TPR), "n"(TPR < 32 ? 32 : TPR) : "memory");
+}
 template <int TPR> DN8_DEV float team_sum(float v, float* red) {
     v = lanes_sum<TPR>(v);
     if (TPR <= 32) return v;
-    const int warp = threadIdx.x >> 5;
+    const int warp = (threadIdx.x % TPR) >> 5;
     if ((threadIdx.x & 31) == 0) red[warp] = v;
-    __syncthreads();
+    team_barrier<TPR>();
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < TPR / 32; ++w) s += red[w];
-    __syncthreads();
     return s;
 }
 template <int TPR> DN8_DEV void team_sum2(float& a, float& b, float* red) {
     a = lanes_sum<TPR>(a);
     b = lanes_sum<TPR>(b);
     if (TPR <= 32) return;
-    const int warp = (threadIdx.x % TPR) >> 5;               // `red` is the team's
+    const int warp = (threadIdx.x % TPR) >> 5;
     if ((threadIdx.x & 31) == 0) {
         red[warp] = a;
         red[TPR / 32 + warp] = b;
     }
-    __syncthreads();
+    team_barrier<TPR>();
     a = b = 0.0f;
 #pragma unroll
     for (int w = 0; w < TPR / 32; ++w) {
         a += red[w];
         b += red[TPR / 32 + w];
     }
-    __syncthreads();
 }
 
 // A team's rows are gridDim.x teams apart; the next row's loads are in flight while this one is reduced.
@@ -63,7 +65,7 @@ template <typename TX, typename TY, int VEC, int NV, int TPR>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR < 512 ? (VEC * NV <= 16 ? 8 : 4) : (VEC * NV <= 16 ? 2 : 1))
 ln_kernel(const dn8_layer_norm_args a) {
     constexpr int THREADS = TPR < 128 ? 128 : TPR, TEAMS = THREADS / TPR;
-    __shared__ float red[TPR < 32 ? 1 : TPR / 32];
+    __shared__ float red[2][TPR < 32 ? 1 : TPR / 32];
     extern __shared__ __align__(16) float wb[];              // [C] weights, [C] biases
     const int t = threadIdx.x % TPR, C = a.C;
     const int64_t step = static_cast<int64_t>(gridDim.x) * TEAMS;
@@ -128,7 +130,7 @@ ln_kernel(const dn8_layer_norm_args a) {
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s += h[k][e];
-        const float mu = team_sum<TPR>(s, red) / static_cast<float>(C);
+        const float mu = team_sum<TPR>(s, red[0]) / static_cast<float>(C);
         float q = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
@@ -138,7 +140,7 @@ ln_kernel(const dn8_layer_norm_args a) {
                     h[k][e] -= mu;
                     q = fmaf(h[k][e], h[k][e], q);
                 }
-        const float r = rsqrtf(team_sum<TPR>(q, red) / static_cast<float>(C) + a.eps);
+        const float r = rsqrtf(team_sum<TPR>(q, red[1]) / static_cast<float>(C) + a.eps);
         TY* y = static_cast<TY*>(a.y) + row * a.y_stride;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -163,7 +165,7 @@ ln_kernel(const dn8_layer_norm_args a) {
 // the variance and for the output.
 template <typename TX, typename TY>
 __global__ void __launch_bounds__(512) ln_long_kernel(const dn8_layer_norm_args a) {
-    __shared__ float red[16];
+    __shared__ float red[2][16];
     const int64_t row = blockIdx.x;
     const int C = a.C;
     const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
@@ -180,13 +182,13 @@ __global__ void __launch_bounds__(512) ln_long_kernel(const dn8_layer_norm_args 
         s += v;
     }
     const TX* h = res != nullptr ? sum : x;                  // a thread reads back its own columns
-    const float mu = team_sum<512>(s, red) / static_cast<float>(C);
+    const float mu = team_sum<512>(s, red[0]) / static_cast<float>(C);
     float q = 0.0f;
     for (int c = threadIdx.x; c < C; c += 512) {
         const float d = to_f32(h[c]) - mu;
         q = fmaf(d, d, q);
     }
-    const float r = rsqrtf(team_sum<512>(q, red) / static_cast<float>(C) + a.eps);
+    const float r = rsqrtf(team_sum<512>(q, red[1]) / static_cast<float>(C) + a.eps);
     TY* y = static_cast<TY*>(a.y) + row * a.y_stride;
     for (int c = threadIdx.x; c < C; c += 512) {
         float w[1] = {1.0f}, b[1] = {0.0f};
@@ -200,18 +202,36 @@ __global__ void __launch_bounds__(512) ln_long_kernel(const dn8_layer_norm_args 
     }
 }
 
-// Backward: persistent blocks of TEAMS teams; a thread keeps the same columns for every row, so the
-// sums of dy xh and dy over the block's rows stay in its registers. They are added over the teams in
-// shared memory and written as one row of the workspace [gridDim.x][2][C]; ln_cols_kernel adds the
-// rows in a fixed order (no atomics: the same bits every call).
+// BYTES from global to shared memory, asynchronously; wait_copies: all but the `n` last committed groups have come.
+template <int BYTES> DN8_DEV void copy_async(void* dst, const void* src) {
+    if (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+DN8_DEV void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+DN8_DEV void wait_copies(int n) {
+    if (n >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (n >= 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Backward: persistent blocks of TEAMS teams; a thread keeps the same columns for every row, so the sums of dy xh
+// and dy over the block's rows stay in its registers. Rows of 16-byte vectors come through a ring of `stages` rows
+// per team in shared memory: every thread copies and reads its own vectors, so nobody waits for anybody. (One
+// row ahead in registers is too little in flight: 23664 rows of 2016, fp32 and fp16, took 117 us and take 88; 98304 of
+// 512 bf16 with dsum 77 and 73, 5.5 TB/s; 20427 of 1064 fp16, bound by instructions, 50 and 53.) The sums are added
+// over the teams in shared memory and written as one row of the workspace [gridDim.x][2][C]; ln_cols_kernel adds
+// the rows in a fixed order (no atomics: the same bits every call).
 template <typename TX, typename TY, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1) ln_bwd_kernel(const dn8_layer_norm_bwd_args a) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1) ln_bwd_kernel(const dn8_layer_norm_bwd_args a,
+                                                                                                       int stages) {
     constexpr int THREADS = TPR < 256 ? 256 : TPR;
     constexpr int TEAMS = THREADS / TPR, CB = NV * VEC * TPR;      // columns a team covers
-    __shared__ float red[TEAMS][TPR < 32 ? 1 : 2 * TPR / 32];
+    __shared__ float red[TEAMS][2][TPR < 32 ? 1 : 2 * TPR / 32];
     __shared__ float part[TEAMS > 1 ? 2 * CB : 1];
     griddep_launch_dependents();
-    extern __shared__ __align__(16) float ws_[];             // [C] weights
+    extern __shared__ __align__(16) float ws_[];             // [C] weights, then the ring
     const int team = threadIdx.x / TPR, t = threadIdx.x % TPR, C = a.C;
     float dw[NV][VEC], db[NV][VEC];
 #pragma unroll
@@ -228,28 +248,49 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1) ln_b
     }
     __syncthreads();
     const float inv_c = 1.0f / static_cast<float>(C);
-    // every team of a block makes the same number of steps (the barriers of team_sum2); the next row's loads
-    // are in flight while this one is reduced
+    // (every team of a block makes the same number of steps)
     const int64_t step = static_cast<int64_t>(gridDim.x) * TEAMS;
+    constexpr bool RING = VEC > 1;
+    constexpr int SX = VEC * sizeof(TX), SY = VEC * sizeof(TY);
     Vec<TX, VEC> nx[NV], nd[NV];
     Vec<TY, VEC> ng[NV];
-    float nmu = 0.0f, nr = 0.0f;
-    auto fetch = [&](int64_t r) {
+    float nmu = 0.0f, nr = 0.0f;                             // mean and rstd: one row ahead
+    auto fetch_stats = [&](int64_t r) {
         if (r >= a.rows) return;
         nmu = a.mean[r];
         nr = a.rstd[r];
+    };
+    // a team's row in the ring: x, dy, dsum
+    const int row_bytes = C * static_cast<int>(2 * sizeof(TX) + sizeof(TY));
+    uint8_t* ring = reinterpret_cast<uint8_t*>(ws_ + C) + static_cast<size_t>(team) * stages * row_bytes;
+    auto fetch = [&](int64_t r, int stage) {
+        if (r < a.rows) {
+            uint8_t* slot = ring + stage * row_bytes;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (t + k * TPR) * VEC;
-            if (c < C) {
-                nx[k] = load_vec<TX, VEC>(static_cast<const TX*>(a.x) + r * a.x_stride + c);
-                ng[k] = load_vec<TY, VEC>(static_cast<const TY*>(a.dy) + r * a.dy_stride + c);
-                if (a.dsum != nullptr)
-                    nd[k] = load_vec<TX, VEC>(static_cast<const TX*>(a.dsum) + r * a.dsum_stride + c);
+            for (int k = 0; k < NV; ++k) {
+                const int c = (t + k * TPR) * VEC;
+                if (c < C) {
+                    const TX* x = static_cast<const TX*>(a.x) + r * a.x_stride + c;
+                    const TY* dy = static_cast<const TY*>(a.dy) + r * a.dy_stride + c;
+                    const TX* ds = a.dsum != nullptr ? static_cast<const TX*>(a.dsum) + r * a.dsum_stride + c : nullptr;
+                    if constexpr (RING) {
+                        copy_async<SX>(slot + c * sizeof(TX), x);
+                        copy_async<SY>(slot + C * sizeof(TX) + c * sizeof(TY), dy);
+                        if (ds != nullptr) copy_async<SX>(slot + C * (sizeof(TX) + sizeof(TY)) + c * sizeof(TX), ds);
+                    } else {
+                        nx[k] = load_vec<TX, VEC>(x);
+                        ng[k] = load_vec<TY, VEC>(dy);
+                        if (ds != nullptr) nd[k] = load_vec<TX, VEC>(ds);
+                    }
+                }
             }
         }
+        if (RING) commit_copies();
     };
-    fetch(static_cast<int64_t>(blockIdx.x) * TEAMS + team);
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
+    for (int s = 0; s < stages; ++s) fetch(row0 + s * step, s);
+    fetch_stats(row0);
+    int stage = 0, odd = 0;
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * TEAMS; base < a.rows; base += step) {
         const int64_t row = base + team;
         const bool live = row < a.rows;
@@ -257,12 +298,22 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1) ln_b
         Vec<TX, VEC> d[NV];
         float s1 = 0.0f, s2 = 0.0f;
         const float mu = nmu, r = nr;
+        fetch_stats(row + step);
+        if (RING) wait_copies(stages - 1);
         if (live) {
+            const uint8_t* slot = ring + stage * row_bytes;
 #pragma unroll
             for (int k = 0; k < NV; ++k)
                 if ((t + k * TPR) * VEC < C) {
                     float w[VEC];
                     load_f32(ws_ + (t + k * TPR) * VEC, w);
+                    if (RING) {
+                        const int c = (t + k * TPR) * VEC;
+                        nx[k] = *reinterpret_cast<const Vec<TX, VEC>*>(slot + c * sizeof(TX));
+                        ng[k] = *reinterpret_cast<const Vec<TY, VEC>*>(slot + C * sizeof(TX) + c * sizeof(TY));
+                        if (a.dsum != nullptr)
+                            nd[k] = *reinterpret_cast<const Vec<TX, VEC>*>(slot + C * (sizeof(TX) + sizeof(TY)) + c * sizeof(TX));
+                    }
                     d[k] = nd[k];
                     nx[k].get(xh[k]);
                     ng[k].get(dy[k]);
@@ -277,8 +328,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR < 512 ? 2 : 1) ln_b
                     }
                 }
         }
-        fetch(row + step);
-        team_sum2<TPR>(s1, s2, red[team]);
+        fetch(row + stages * step, stage);
+        if (++stage == stages) stage = 0;
+        team_sum2<TPR>(s1, s2, red[team][odd]);
+        odd ^= 1;
         if (!live) continue;
         s1 *= inv_c;
         s2 *= inv_c;
@@ -454,11 +507,23 @@ cudaError_t ln_bwd_go(const dn8_layer_norm_bwd_args& a, cudaStream_t st, int* nr
     const int64_t want = (a.rows + teams - 1) / teams;
     const int grid = static_cast<int>(want < LN_COLS_ROWS ? want : LN_COLS_ROWS);
     *nrows = grid;
-    const size_t smem = static_cast<size_t>(a.C) * sizeof(float);
-    if (a.C <= 8 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 8>, dim3(grid), dim3(256), smem, st, a);
-    if (a.C <= 32 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 32>, dim3(grid), dim3(256), smem, st, a);
-    if (a.C <= 128 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 128>, dim3(grid), dim3(256), smem, st, a);
-    if (a.C <= 512 * per) return launch_pdl(false, ln_bwd_kernel<TX, TY, VEC, NV, 512>, dim3(grid), dim3(512), smem, st, a);
+    if (a.C <= 512 * per) {
+        // Stages: four rows per team, two or one where they would not leave room for two blocks per SM (teams of
+        // 512: for one)
+        const size_t most = a.C <= 128 * per ? 80 * 1024 : 180 * 1024;
+        const size_t rows = static_cast<size_t>(teams) * a.C * (2 * sizeof(TX) + sizeof(TY));
+        const int stages = VEC == 1 ? 1 : 4 * rows <= most ? 4 : 2 * rows <= most ? 2 : 1;
+        const size_t smem = static_cast<size_t>(a.C) * sizeof(float) + (VEC == 1 ? 0 : stages * rows);
+        const auto kernel = a.C <= 8 * per     ? ln_bwd_kernel<TX, TY, VEC, NV, 8>
+                            : a.C <= 32 * per  ? ln_bwd_kernel<TX, TY, VEC, NV, 32>
+                            : a.C <= 128 * per ? ln_bwd_kernel<TX, TY, VEC, NV, 128>
+                                               : ln_bwd_kernel<TX, TY, VEC, NV, 512>;
+        if (smem > 40 * 1024) {
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            if (e != cudaSuccess) return e;
+        }
+        return launch_pdl(false, kernel, dim3(grid), dim3(a.C <= 128 * per ? 256 : 512), smem, st, a, stages);
+    }
     if (a.work != nullptr) {
         const int slabs = static_cast<int>(a.rows < 32 ? 1 : a.rows / 32 < LN_COLS_ROWS ? a.rows / 32 : LN_COLS_ROWS);
         *nrows = slabs;
@@ -480,8 +545,8 @@ cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, int sms, cudaStream_
         using TY = decltype(ty);
         // 16-byte loads where every row allows them, single elements otherwise
         if (!vec) return ln_go<TX, TY, 1, 16>(a, sms, st);
-        if (sizeof(TX) == 4) return ln_go<TX, TY, 4, 4>(a, sms, st);
-        return ln_go<TX, TY, 8, 2>(a, sms, st);
+        if constexpr (sizeof(TX) == 4) return ln_go<TX, TY, 4, 4>(a, sms, st);
+        else return ln_go<TX, TY, 8, 2>(a, sms, st);
     });
 }
 
@@ -498,8 +563,8 @@ cudaError_t launch_layer_norm_bwd(const dn8_layer_norm_bwd_args& args, cudaStrea
         using TX = decltype(tx);
         using TY = decltype(ty);
         if (!vec) return ln_bwd_go<TX, TY, 1, 8>(a, st, &nrows);
-        if (sizeof(TX) == 4) return ln_bwd_go<TX, TY, 4, 4>(a, st, &nrows);
-        return ln_bwd_go<TX, TY, 8, 2>(a, st, &nrows);
+        if constexpr (sizeof(TX) == 4) return ln_bwd_go<TX, TY, 4, 4>(a, st, &nrows);
+        else return ln_bwd_go<TX, TY, 8, 2>(a, st, &nrows);
     });
     if (e != cudaSuccess || a.work == nullptr) return e;
     return launch_pdl(nrows > 0, ln_cols_kernel, dim3((2 * a.C + 31) / 32), dim3(1024), 0, st,
