@@ -23,6 +23,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -42,23 +43,27 @@ class _LayerNorm(torch.autograd.Function):
         mean, rstd = (torch.empty(x.shape[0], dtype=torch.float32, device=x.device) for _ in range(2))
         ops.layer_norm(x, weight, bias, out, eps, res, h, mean, rstd)
         ctx.save_for_backward(x if h is None else h, weight, mean, rstd)
-        ctx.has = (res is not None, bias is not None)
+        ctx.has = (res is not None, None if bias is None else bias.dtype)
         if h is None:
             return out
         return out, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dsum=None):
         h, weight, mean, rstd = ctx.saved_tensors
         dx = torch.empty_like(h, memory_format=torch.contiguous_format)
         dw = None if weight is None else torch.empty_like(weight)
-        db = torch.empty_like(weight) if ctx.has[1] else None
+        has_res, bias_type = ctx.has
+        db = None
+        if bias_type is not None:                            # (of the weight's type, fp32 without one)
+            db = torch.empty(h.shape[1], dtype=torch.float32 if weight is None else weight.dtype, device=h.device)
         ops.layer_norm_backward(dy.contiguous(), h, weight, mean, rstd, dx, dw, db,
                                 None if dsum is None else dsum.contiguous())
-        return dx, dw, db, None, None, dx if ctx.has[0] else None
+        return dx, dw, None if db is None else db.to(bias_type), None, None, dx if has_res else None
 
 
-def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, eps: float = 1e-5,
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float = 1e-5,
                dtype: torch.dtype | None = None, res: torch.Tensor | None = None):
     """`ops.layer_norm` of x [M, C] with a gradient; returns the output (of `dtype`, default x's), and with
     `res` (output, x + res)."""
@@ -76,6 +81,7 @@ class _Rope(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         pos, = ctx.saved_tensors
         dq, dk = dq.contiguous(), dk.contiguous()
@@ -98,15 +104,17 @@ class _Attention(torch.autograd.Function):
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.full(q.shape[:2], -torch.inf, dtype=torch.float32, device=q.device)
         ops.attention(q, k, v, out, cu_q, cu_k, lse=lse, **mask)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
-        ctx.mask = mask
+        # (keep and len_k among the saved tensors: autograd notices when they change before the backward pass)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k, mask.get("keep"), mask.get("len_k"))
+        ctx.mask = {n: x for n, x in mask.items() if n not in ("keep", "len_k")}
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, out, lse, cu_q, cu_k, keep, len_k = ctx.saved_tensors
         grads = [torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-        ops.attention_backward(dout.contiguous(), q, k, v, out, lse, *grads, cu_q, cu_k, **ctx.mask)
+        ops.attention_backward(dout.contiguous(), q, k, v, out, lse, *grads, cu_q, cu_k, keep=keep, len_k=len_k, **ctx.mask)
         return *grads, None, None, None
 
 
