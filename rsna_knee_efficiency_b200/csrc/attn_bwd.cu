@@ -18,7 +18,12 @@
 // while they take the exponentials of S(u + 1); else S(u + 1) is made while they work on dS(u).
 //
 // A CTA takes one piece (one walk) after the other (ask_for_block). Under a window, the first tokens' key
-// tile is seen by every query: its walk is cut into shares, whose sums attn_bwd_join_kernel adds.
+// tile is seen by every query: its walk is cut into shares, whose sums attn_bwd_join_kernel adds (and where heads are
+// few, every long walk of dk and dv).
+//
+// 2 x 8192 tokens, 16 heads, no mask: D = 64 2045 us (671 TFLOP/s of the 10 D per pair), D = 128 3440 us (800). Bound by no
+// single unit: at views of 6160 with windows of 512 to each side, D = 64, 422 us; 403 without the exponentials, 378
+// without the product of dS, 401 with half of the value products.
 #include "attn_umma.cuh"
 
 namespace dn8 {

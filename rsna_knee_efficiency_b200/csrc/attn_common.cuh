@@ -94,6 +94,54 @@ DN8_DEV Sequence find_block(const A& a, int unit, int mul, int per, S shares = S
     return s;
 }
 
+// The sequences of a batch of up to MOST as one warp keeps them in shared memory, which asks for block after block:
+// a look takes 0.1 us where find_block, which reads the offsets again, takes 1.6.
+struct SequenceTable {
+    static constexpr int MOST = 128;
+    int4 seq[MOST];    // q0, nq, k0, nk
+    int end[MOST];     // blocks of this sequence and those before it
+    template <typename A, typename S> DN8_DEV void fill(const A& a, int per, S shares) {
+        const int lane = threadIdx.x & 31;
+        int run = 0;
+#pragma unroll 1
+        for (int base = 0; base < a.B; base += 32) {
+            const int b = base + lane;
+            int incl = 0;
+            if (b < a.B) {
+                const Sequence s = sequence_of(a, b);
+                seq[b] = make_int4(s.q0, s.nq, s.k0, s.nk);
+                incl = (s.nq + per - 1) / per * shares(s.nq, s.nk);
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (b < a.B) end[b] = run + incl;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        __syncwarp();
+    }
+    DN8_DEV Sequence find(int B, int unit) const {
+        const int lane = threadIdx.x & 31;
+        Sequence s;
+        s.b = -1;
+        for (int base = 0; base < B && s.b < 0; base += 32) {
+            const unsigned hit = __ballot_sync(0xffffffffu, base + lane < B && unit < end[base + lane]);
+            if (hit) s.b = base + __ffs(hit) - 1;
+        }
+        if (s.b >= 0) {
+            const int4 v = seq[s.b];
+            s.q0 = v.x;
+            s.nq = v.y;
+            s.k0 = v.z;
+            s.nk = v.w;
+            s.blk = unit - (s.b > 0 ? end[s.b - 1] : 0);
+        }
+        return s;
+    }
+};
+
 // Key tiles of TILE keys that queries at positions p0 .. p1 see some key of: the tiles of the first
 // tokens, then those of the window. tile(t) for t = 0 .. count - 1.
 struct KeyTiles {

@@ -12,7 +12,13 @@
 // 256, far inside fp16 and fp32), so the accumulator rarely leaves TMEM.
 //
 // A CTA takes one piece after the other (ask_for_block): the loads and first scores of the next piece run
-// while the threads still write the last one's output.
+// while the threads still write the last one's output. A piece costs some 5 us beyond its tiles (1.4 us each at
+// D <= 64), so for short sequences the next one is asked for early and looked up in shared memory: 128 x 128
+// tokens, 16 heads, D = 64, 90 us with the question behind V and offsets from memory, 74.
+//
+// 2 x 8192 tokens, 16 heads, no mask: D = 64 658 us (835 TFLOP/s, bound by the special function units: the
+// exponentials alone take 0.7 of it, then by the latency of a tile's steps), D = 128 945 us (1163 TFLOP/s, 0.68 of
+// the measured matrix rate). Four views of 6144, causal, 8 heads, D = 128: 326 us.
 //
 // Warps 0-7 and 8-15: softmax of tile 0 and 1, a warp per 16 rows and four threads per row, so that a row's
 // maximum takes two shuffles (32 scores of two rows a thread; one thread per row left the schedulers idle
@@ -38,7 +44,7 @@ constexpr float AF_SHARE = 4.0f;                      // key tiles of a share, a
 template <int DP> struct TileCfg {
     static constexpr int KST = DP == 64 ? 3 : 2, VST = DP == 64 ? 3 : 2;      // stages of K and V
     static constexpr uint32_t TILE = AT_TILE * DP * 2;
-    static constexpr uint32_t SMEM = 1024 + TILE * (2 + KST + VST) + 3072;
+    static constexpr uint32_t SMEM = 1024 + TILE * (2 + KST + VST) + 6144;
     // TMEM columns: S of the two tiles, P (over S, or of its own), O
     static constexpr bool OWN_P = DP == 64;
     static constexpr uint32_t S0 = 0, P0 = OWN_P ? 256 : 0, PG = OWN_P ? 64 : 128, O0 = OWN_P ? 384 : 256;
@@ -98,6 +104,7 @@ struct TileShared {
     TilePiece piece[2];                               // of even and odd number
     uint32_t words[3][4];
     float stat[2][2][AT_TILE];                        // [tile][sum, reference][row]
+    SequenceTable table;
     uint32_t tmem;
     int abort;
 };
@@ -107,7 +114,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
 attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                  const __grid_constant__ CUtensorMap mv, const dn8_attention_args a, const TilePlan plan) {
     using C = TileCfg<DP>;
-    static_assert(sizeof(TileShared) <= 3072, "shared state");
+    static_assert(sizeof(TileShared) <= 6144, "shared state");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sq = smem;
@@ -163,12 +170,14 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             // ---------------- pieces, and masked rows of V ----------------
             int block = blockIdx.x, asked = 0, vc = 0;
             const TileShares shares = CUT ? tile_shares(a, plan) : TileShares{a, 0.0f};
+            const bool few = a.B <= SequenceTable::MOST;
+            if (few) sh.table.fill(a, 2 * AT_TILE, shares);
             TilePiece pc;
             // Looks block after block up until one holds a piece: false after the last.
             auto look = [&]() -> bool {
                 while (block >= 0) {
+                    pc.seq = few ? sh.table.find(a.B, block / a.Hq) : find_block<false>(a, block / a.Hq, 1, 2 * AT_TILE, shares);
                     if (CUT) {
-                        pc.seq = find_block<false>(a, block / a.Hq, 1, 2 * AT_TILE, shares);
                         pc.share = block;
                         // (behind the last piece there are some 148 blocks with nothing to do: one of them ends this CTA's
                         // search, blocks that were not asked for start by themselves. Each one more held V up for
@@ -177,8 +186,6 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                             if (lane == 0) plan.rec[block] = make_int4(0, 0, 0, 0);
                             return false;
                         }
-                    } else {
-                        pc.seq = find_block<false>(a, block / a.Hq, 1, 2 * AT_TILE);
                     }
                     pc.h = block % a.Hq;
                     if (pc.seq.b >= 0) return true;   // (the bound on the blocks may be too high)
@@ -244,6 +251,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 }
                 __syncwarp();
             };
+            pc.share = -1;
             publish(0, look());
             bool ok = true;
             for (int n = 0; pc.seq.b >= 0; ++n) {
@@ -251,6 +259,16 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                 const KeyTiles all = pc.all;
                 const int ask_at = max(0, count - AF_AHEAD);
                 for (int u = 0; u < max(count, 1); ++u) {
+                    if (u == ask_at) {
+                        // The next piece, asked for once every warp has begun with this one ...
+                        ok = mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (62 << 4));
+                        if (!ok) break;
+                        if (lane == 0) {
+                            fence_async_smem();
+                            mbar_expect_tx(&sh.answered, 16);
+                            ask_for_block(sh.answer, &sh.answered);
+                        }
+                    }
                     if (u < count) {
                         const int t = all.tile(u), vs = vc % C::VST;
                         const bool fix = a.keep != nullptr || (t + 1) * AT_TILE > nk;
@@ -283,21 +301,14 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                         ++vc;
                     }
                     if (u == ask_at) {
-                        // The next piece, once every warp has begun with this one. (This tile's product does not wait for
-                        // it.)
-                        ok = mbar_wait_w(&sh.pread, n & 1, a.err, abort_flag, ERR_WAIT_EMPTY | (62 << 4));
-                        if (!ok) break;
-                        if (lane == 0) {
-                            fence_async_smem();
-                            mbar_expect_tx(&sh.answered, 16);
-                            ask_for_block(sh.answer, &sh.answered);
-                        }
+                        // ... and looked up when this tile's V, whose product may be waiting, has been let go
                         ok = mbar_wait_w(&sh.answered, asked & 1, a.err, abort_flag, ERR_WAIT_FULL | (61 << 4));
                         if (!ok) break;
                         ++asked;
                         block = answered_block(sh.answer);
                         __syncwarp();
-                        publish(n + 1, look());
+                        const bool there = look();
+                        publish(n + 1, there);
                     }
                 }
                 if (!ok) break;

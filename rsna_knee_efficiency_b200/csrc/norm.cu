@@ -8,7 +8,8 @@
 // Both passes are bound by memory: a row is read once into registers (a team of 8, 32, 128 or 512
 // threads per row, so that a thread holds at most 32 values), the variance is summed from the
 // registers as squares of differences (no cancellation of E[x^2] - mu^2), and written once.
-// Statistics and sums are fp32. Narrow rows share a warp: 67678 rows of 31 bf16 took 52 us with a warp each and
+// Statistics and sums are fp32. 98304 rows of 512 bf16 with a residual (403 MB): 76 us, 5.3 TB/s of 6.5 for a copy.
+// Narrow rows share a warp: 67678 rows of 31 bf16 took 52 us with a warp each and
 // take 19 with eight threads each, 90000 of 64 (fp32 in, fp16 out) 40 and 17.
 #include "ctx_common.cuh"
 #include "dn8_kernels.h"
