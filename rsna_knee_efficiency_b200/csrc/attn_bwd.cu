@@ -67,7 +67,7 @@ template <int DP> struct BwdCfg {
     // for again at the next one's start (S), so where memory is short X0 has the third slot.
     static constexpr int N0 = 3, N1 = DP == 64 ? 3 : 2;
     static constexpr uint32_t TILE = AT_TILE * DP * 2;
-    static constexpr uint32_t SMEM = TILE * (2 + N0 + N1) + 3072;
+    static constexpr uint32_t STATE = 3 << 10, SMEM = TILE * (2 + N0 + N1) + STATE;
     // TMEM columns: dP, then S (one or two tiles), then the sums at the end
     static constexpr uint32_t DPC = 0, S = 128, ACC1 = 512 - DP, ACC0 = 512 - 2 * DP;
 };
@@ -315,7 +315,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
                 const dn8_attention_bwd_args a, const BwdPlan plan) {
     using C = BwdCfg<DP>;
-    static_assert(sizeof(BwdShared) <= 3072, "shared state");
+    static_assert(sizeof(BwdShared) <= C::STATE, "shared state");
     extern __shared__ __align__(1024) uint8_t smem[];    // (no static shared memory, so it starts aligned)
     uint8_t* sr = smem;                                  // R0, R1
     uint8_t* sx0 = smem + 2 * C::TILE;                   // slots of X0

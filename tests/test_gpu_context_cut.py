@@ -82,3 +82,31 @@ def test_cut_attention_offsets_that_go_back():
     grads = [torch.empty_like(t) for t in (q, k, v)]
     ops.attention_backward(q, q, k, v, out, lse, *grads, bad, bad, err=err)
     assert int(err) == 4
+
+
+def many(n, seed, most):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(0, most, (n,), generator=g).tolist()
+
+
+# batches around the number of sequences that a block keeps at hand, with a long one among the short ones
+MANY = [(many(128, 1, 90), None, 2, 1, 64, -1, -1), (many(129, 2, 90), None, 2, 2, 64, 30, 0), (many(300, 3, 70), None, 1, 1, 128, -1, 0),
+        (many(200, 4, 20) + [900], many(200, 5, 50) + [9000], 1, 1, 64, -1, -1), ([1] * 140, many(139, 6, 300) + [12000], 4, 1, 64, -1, 0),
+        ([700] + [0] * 150, [5000] + [3] * 150, 2, 1, 64, -1, -1)]
+
+
+@pytest.mark.parametrize("lens_q,lens_k,Hq,Hk,D,left,right", MANY, ids=[f"{len(m[0])}-{m[2]}.{m[3]}-d{m[4]}" for m in MANY])
+def test_many_sequences(lens_q, lens_k, Hq, Hk, D, left, right):
+    g, q, k, v, cq, ck, _, mask = attention_case(len(lens_q), lens_q, lens_k or lens_q, Hq, Hk, D, BF16, left, right, 0)
+    out, lse = run_attention(q, k, v, cq, ck, None, mask)
+    o, ls, to, tl = ref.attention(q, k, v, cq, ck, **mask)
+    ref.close(out, o, to, "out")
+    ref.close(lse, ls, tl, "lse")
+    dout = randn(g, *q.shape, dtype=BF16)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    grads = [torch.full_like(t, 7.0) for t in (q, k, v)]
+    ops.attention_backward(dout, q, k, v, out, lse, *grads, i32(cq), i32(ck), err=err, **mask)
+    assert int(err) == 0
+    want = ref.attention(q, k, v, cq, ck, dout=dout, out=out, lse=lse, **mask)
+    for a, w, tol, name in zip(grads, want[:3], want[3:], ("dq", "dk", "dv")):
+        ref.close(a, w, tol, name)
