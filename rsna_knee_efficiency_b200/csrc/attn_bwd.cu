@@ -24,6 +24,8 @@
 // 2 x 8192 tokens, 16 heads, no mask: D = 64 2045 us (671 TFLOP/s of the 10 D per pair), D = 128 3440 us (800). Bound by no
 // single unit: at views of 6160 with windows of 512 to each side, D = 64, 422 us; 403 without the exponentials, 378
 // without the product of dS, 401 with half of the value products.
+#include <type_traits>
+
 #include "attn_umma.cuh"
 
 namespace dn8 {
@@ -67,7 +69,9 @@ template <int DP> struct BwdCfg {
     // for again at the next one's start (S), so where memory is short X0 has the third slot.
     static constexpr int N0 = 3, N1 = DP == 64 ? 3 : 2;
     static constexpr uint32_t TILE = AT_TILE * DP * 2;
-    static constexpr uint32_t STATE = 3 << 10, SMEM = TILE * (2 + N0 + N1) + STATE;
+    // (the sequences by blocks of queries and of keys lie behind the state where there is room)
+    static constexpr bool TABLES = DP == 64;
+    static constexpr uint32_t STATE = 3 << 10, SMEM = TILE * (2 + N0 + N1) + STATE + (TABLES ? 2 * sizeof(SequenceTable) : 0);
     // TMEM columns: dP, then S (one or two tiles), then the sums at the end
     static constexpr uint32_t DPC = 0, S = 128, ACC1 = 512 - DP, ACC0 = 512 - 2 * DP;
 };
@@ -379,6 +383,25 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             int block = blockIdx.x, asked = 0;
             BwdPiece pc;
             const BwdShares shares = CUT ? bwd_shares(a, plan) : BwdShares{a, 0.0f};
+            // a block's sequence: from shared memory, from this warp's registers where that is full, or read again
+            const bool few = a.B <= (C::TABLES ? SequenceTable::MOST : SequenceLanes::MOST);
+            SequenceTable* table = reinterpret_cast<SequenceTable*>(reinterpret_cast<uint8_t*>(&sh) + C::STATE);
+            SequenceLanes seqs;
+            if (few && C::TABLES) {
+                table[0].fill<false>(a, AT_TILE, OneShare());
+                table[1].fill<true>(a, AT_TILE, shares);
+            } else if (few) {
+                seqs.fill(a, AT_TILE, shares);
+            }
+            auto tile_of = [&](auto keys, int unit) -> Sequence {
+                constexpr bool KEYS = decltype(keys)::value;
+                if (!few) {
+                    if constexpr (KEYS && CUT) return find_block<true>(a, unit, 1, AT_TILE, shares);
+                    else return find_block<KEYS>(a, unit, 1, AT_TILE);
+                }
+                if constexpr (C::TABLES) return table[KEYS].find(a.B, unit);
+                else return seqs.template find<KEYS>(unit);
+            };
             for (int n = 0;;) {
                 pc.seq.b = -2;
                 pc.steps = pc.tile0 = pc.hx = 0;
@@ -397,19 +420,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                         pc.h = x % a.Hk;
                         if (pc.seq.blk * AT_TILE >= pc.seq.nk) pc.seq.b = -1;
                     } else if (CUT && pc.kv) {
-                        pc.seq = find_block<true>(a, block / a.Hk, 1, AT_TILE, shares);
+                        pc.seq = tile_of(std::true_type(), block / a.Hk);
                         pc.h = block % a.Hk;
                         if (pc.seq.b >= 0) cuts = shares(pc.seq.nq, pc.seq.nk);
                         mine = pc.seq.blk % cuts;
                         pc.seq.blk /= cuts;
                     } else if (pc.kv) {
                         const int x = block - plan.split_blocks;
-                        pc.seq = find_block<true>(a, x / a.Hk, 1, AT_TILE);
+                        pc.seq = tile_of(std::true_type(), x / a.Hk);
                         pc.h = x % a.Hk;
                         if (plan.shares > 1 && pc.seq.blk < plan.tiles) pc.seq.b = -1;
                     } else {
                         const int x = block - plan.kv_blocks;
-                        pc.seq = find_block<false>(a, x / a.Hq, 1, AT_TILE);
+                        pc.seq = tile_of(std::false_type(), x / a.Hq);
                         pc.h = x % a.Hq;
                     }
                     if (cuts > 1) pc.share = block;

@@ -100,7 +100,7 @@ struct SequenceTable {
     static constexpr int MOST = 128;
     int4 seq[MOST];    // q0, nq, k0, nk
     int end[MOST];     // blocks of this sequence and those before it
-    template <typename A, typename S> DN8_DEV void fill(const A& a, int per, S shares) {
+    template <bool KEYS, typename A, typename S> DN8_DEV void fill(const A& a, int per, S shares) {
         const int lane = threadIdx.x & 31;
         int run = 0;
 #pragma unroll 1
@@ -110,7 +110,7 @@ struct SequenceTable {
             if (b < a.B) {
                 const Sequence s = sequence_of(a, b);
                 seq[b] = make_int4(s.q0, s.nq, s.k0, s.nk);
-                incl = (s.nq + per - 1) / per * shares(s.nq, s.nk);
+                incl = ((KEYS ? s.nk : s.nq) + per - 1) / per * shares(s.nq, s.nk);
             }
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -138,6 +138,48 @@ struct SequenceTable {
             s.nk = v.w;
             s.blk = unit - (s.b > 0 ? end[s.b - 1] : 0);
         }
+        return s;
+    }
+};
+
+// The same of up to 32 sequences in a warp's registers, where shared memory is full: lane b holds sequence b, its
+// blocks of queries and, cut into shares, of keys.
+struct SequenceLanes {
+    static constexpr int MOST = 32;
+    int q0, nq, k0, nk, q_end, k_end;
+    template <typename A, typename S> DN8_DEV void fill(const A& a, int per, S key_shares) {
+        const int lane = threadIdx.x & 31;
+        q0 = nq = k0 = nk = q_end = k_end = 0;
+        if (lane < a.B) {
+            const Sequence s = sequence_of(a, lane);
+            q0 = s.q0;
+            nq = s.nq;
+            k0 = s.k0;
+            nk = s.nk;
+            q_end = (nq + per - 1) / per;
+            k_end = (nk + per - 1) / per * key_shares(nq, nk);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, q_end, o), w = __shfl_up_sync(0xffffffffu, k_end, o);
+            if (lane >= o) {
+                q_end += v;
+                k_end += w;
+            }
+        }
+    }
+    template <bool KEYS> DN8_DEV Sequence find(int unit) const {
+        const int end = KEYS ? k_end : q_end;
+        const unsigned hit = __ballot_sync(0xffffffffu, unit < end);
+        Sequence s;
+        s.b = __ffs(hit) - 1;                                  // (-1: none)
+        const int b = max(s.b, 0);
+        s.q0 = __shfl_sync(0xffffffffu, q0, b);
+        s.nq = __shfl_sync(0xffffffffu, nq, b);
+        s.k0 = __shfl_sync(0xffffffffu, k0, b);
+        s.nk = __shfl_sync(0xffffffffu, nk, b);
+        const int before = __shfl_sync(0xffffffffu, end, max(b - 1, 0));
+        s.blk = unit - (b > 0 ? before : 0);
         return s;
     }
 };

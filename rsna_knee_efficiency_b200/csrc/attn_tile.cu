@@ -171,7 +171,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             int block = blockIdx.x, asked = 0, vc = 0;
             const TileShares shares = CUT ? tile_shares(a, plan) : TileShares{a, 0.0f};
             const bool few = a.B <= SequenceTable::MOST;
-            if (few) sh.table.fill(a, 2 * AT_TILE, shares);
+            if (few) sh.table.fill<false>(a, 2 * AT_TILE, shares);
             TilePiece pc;
             // Looks block after block up until one holds a piece: false after the last.
             auto look = [&]() -> bool {
