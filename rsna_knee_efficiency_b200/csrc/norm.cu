@@ -493,7 +493,8 @@ cudaError_t ln_go(const dn8_layer_norm_args& a, int sms, cudaStream_t st) {
     constexpr int per = VEC * NV;
     if (a.C <= 8 * per) return ln_team<TX, TY, VEC, NV, 8>(a, sms, st);
     if (a.C <= 32 * per) return ln_team<TX, TY, VEC, NV, 32>(a, sms, st);
-    if (a.C <= 64 * per) return ln_team<TX, TY, VEC, 2 * NV, 32>(a, sms, st);
+    // (32 single elements per thread keep too few warps at work)
+    if (VEC > 1 && a.C <= 64 * per) return ln_team<TX, TY, VEC, 2 * NV, 32>(a, sms, st);
     if (a.C <= 128 * per) return ln_team<TX, TY, VEC, NV, 128>(a, sms, st);
     if (a.C <= 256 * per) return ln_team<TX, TY, VEC, 2 * NV, 128>(a, sms, st);
     if (a.C <= 512 * per) return ln_team<TX, TY, VEC, NV, 512>(a, sms, st);
@@ -541,10 +542,19 @@ cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, int sms, cudaStream_
     const bool vec = a.C % 8 == 0 && vec_ok(a.w, 0, 4) && vec_ok(a.b, 0, 4) && vec_ok(a.x, a.x_stride, sx) &&
                      vec_ok(a.y, a.y_stride, sy) &&
                      (a.res == nullptr || (vec_ok(a.res, a.res_stride, sx) && vec_ok(a.sum, a.sum_stride, sx)));
+    // two elements of every row (and of weight and bias) at a time
+    auto pairs_of = [](const void* p, int64_t stride, int size) {
+        return reinterpret_cast<uintptr_t>(p) % (2 * size) == 0 && stride % 2 == 0;
+    };
+    const bool two = a.C % 2 == 0 && pairs_of(a.w, 0, 4) && pairs_of(a.b, 0, 4) && pairs_of(a.x, a.x_stride, sx) &&
+                     pairs_of(a.y, a.y_stride, sy) &&
+                     (a.res == nullptr || (pairs_of(a.res, a.res_stride, sx) && pairs_of(a.sum, a.sum_stride, sx)));
     return with_types(a.x_type, a.y_type, [&](auto tx, auto ty) {
         using TX = decltype(tx);
         using TY = decltype(ty);
-        // 16-byte loads where every row allows them, single elements otherwise
+        // 16-byte loads where every row allows them, pairs where C is even (40000 rows of 514 bf16 with a residual:
+        // 204 us in single elements, 45; 8000 of 2050 fp32 110 and 71), single elements otherwise
+        if (!vec && two) return ln_go<TX, TY, 2, 8>(a, sms, st);
         if (!vec) return ln_go<TX, TY, 1, 16>(a, sms, st);
         if constexpr (sizeof(TX) == 4) return ln_go<TX, TY, 4, 4>(a, sms, st);
         else return ln_go<TX, TY, 8, 2>(a, sms, st);

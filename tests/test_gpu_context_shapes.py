@@ -43,6 +43,24 @@ def test_narrow_layer_norm(M, C, t, to, res):
     assert all(torch.equal(p, q) for p, q in zip(again, (dx, dw, db)))
 
 
+@pytest.mark.parametrize("M,C,t,to", [(300, 2, BF16, BF16), (77, 514, F16, F16), (40, 2050, F32, F16), (9, 8194, F32, F32), (5, 18002, BF16, BF16),
+                                      (64, 130, F32, BF16), (33, 515, BF16, BF16), (21, 1537, F32, F32), (3, 4100, F16, F16)])
+@pytest.mark.parametrize("res", [False, True])
+@pytest.mark.parametrize("wt", [F32, F16])
+def test_layer_norm_by_pairs(M, C, t, to, res, wt):
+    g = gen(M * C + 1)
+    wide = randn(g, M, C + 3, dtype=t)               # rows an odd number of elements apart: single elements again
+    for x in (randn(g, M, C, dtype=t), wide[:, 1:C + 1], wide[:, 2:C + 2]):
+        r = randn(g, M, C, dtype=t) if res else None
+        w, b = (1 + 0.2 * randn(g, C)).to(wt), randn(g, C, dtype=wt)
+        y, s = torch.empty(M, C, dtype=to, device=DEV), torch.empty(M, C, dtype=t, device=DEV) if res else None
+        ops.layer_norm(x, w, b, y, 1e-5, r, s)
+        h, wy, _, _, tol, _, _ = ref.layer_norm(x, w, b, 1e-5, r)
+        ref.close(y, wy, tol + ref.u(to) * wy.abs() + ref.eta(to), "y")
+        if res:
+            assert torch.equal(s.double(), h)
+
+
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 @pytest.mark.parametrize("T,Hq,Hk,D,sec,per_axis", [
     (1, 1, 0, 8, (1,), False), (53, 8, 2, 64, (1, 30), True), (700, 4, 1, 32, (1, 11, 1, 2), True), (19, 3, 3, 80, (39,), False),
