@@ -10,7 +10,7 @@
 // registers as squares of differences (no cancellation of E[x^2] - mu^2), and written once.
 // Statistics and sums are fp32. 98304 rows of 512 bf16 with a residual (403 MB): 76 us, 5.3 TB/s of 6.5 for a copy.
 // Narrow rows share a warp: 67678 rows of 31 bf16 took 52 us with a warp each and
-// take 19 with eight threads each, 90000 of 64 (fp32 in, fp16 out) 40 and 17.
+// take 11 with eight threads each, 90000 of 64 (fp32 in, fp16 out) 40 and 17.
 #include "ctx_common.cuh"
 #include "dn8_kernels.h"
 
@@ -493,10 +493,10 @@ cudaError_t ln_go(const dn8_layer_norm_args& a, int sms, cudaStream_t st) {
     constexpr int per = VEC * NV;
     if (a.C <= 8 * per) return ln_team<TX, TY, VEC, NV, 8>(a, sms, st);
     if (a.C <= 32 * per) return ln_team<TX, TY, VEC, NV, 32>(a, sms, st);
-    // (32 single elements per thread keep too few warps at work)
+    // (more single elements per thread keep too few warps at work)
     if (VEC > 1 && a.C <= 64 * per) return ln_team<TX, TY, VEC, 2 * NV, 32>(a, sms, st);
     if (a.C <= 128 * per) return ln_team<TX, TY, VEC, NV, 128>(a, sms, st);
-    if (a.C <= 256 * per) return ln_team<TX, TY, VEC, 2 * NV, 128>(a, sms, st);
+    if (VEC > 1 && a.C <= 256 * per) return ln_team<TX, TY, VEC, 2 * NV, 128>(a, sms, st);
     if (a.C <= 512 * per) return ln_team<TX, TY, VEC, NV, 512>(a, sms, st);
     if (a.C <= 1024 * per) return ln_team<TX, TY, VEC, 2 * NV, 512>(a, sms, st);
     return launch_pdl(false, ln_long_kernel<TX, TY>, dim3(static_cast<unsigned>(a.rows)), dim3(512), 0, st, a);
@@ -553,9 +553,10 @@ cudaError_t launch_layer_norm(const dn8_layer_norm_args& a, int sms, cudaStream_
         using TX = decltype(tx);
         using TY = decltype(ty);
         // 16-byte loads where every row allows them, pairs where C is even (40000 rows of 514 bf16 with a residual:
-        // 204 us in single elements, 45; 8000 of 2050 fp32 110 and 71), single elements otherwise
-        if (!vec && two) return ln_go<TX, TY, 2, 8>(a, sms, st);
-        if (!vec) return ln_go<TX, TY, 1, 16>(a, sms, st);
+        // 45 us, 67 with half as many per thread; 8000 of 2050 fp32: 71, and 45), else single elements, eight per thread
+        // (40000 rows of 515: 88 us; with sixteen, 189)
+        if (!vec && two) return a.C <= 1024 ? ln_go<TX, TY, 2, 8>(a, sms, st) : ln_go<TX, TY, 2, 4>(a, sms, st);
+        if (!vec) return ln_go<TX, TY, 1, 8>(a, sms, st);
         if constexpr (sizeof(TX) == 4) return ln_go<TX, TY, 4, 4>(a, sms, st);
         else return ln_go<TX, TY, 8, 2>(a, sms, st);
     });
