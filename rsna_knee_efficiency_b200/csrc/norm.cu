@@ -520,7 +520,8 @@ cudaError_t ln_bwd_go(const dn8_layer_norm_bwd_args& a, cudaStream_t st, int* nr
                             : a.C <= 32 * per  ? ln_bwd_kernel<TX, TY, VEC, NV, 32>
                             : a.C <= 128 * per ? ln_bwd_kernel<TX, TY, VEC, NV, 128>
                                                : ln_bwd_kernel<TX, TY, VEC, NV, 512>;
-        if (smem > 40 * 1024) {
+        // (the default limit of 48 KB counts the static part too: up to 16.5 KB, the sums of teams of 128)
+        if (smem > 24 * 1024) {
             cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
             if (e != cudaSuccess) return e;
         }
