@@ -480,8 +480,10 @@ cudaError_t ln_team(const dn8_layer_norm_args& a, int sms, cudaStream_t st) {
     const int64_t want = (a.rows + TEAMS - 1) / TEAMS, most = static_cast<int64_t>(sms) * (1024 / THREADS);
     const size_t smem = static_cast<size_t>(a.C) * 2 * sizeof(float);
     if (smem > 40 * 1024) {
+        // (the most that any call of this instance asks for, not this call's own: another host thread with a
+        // narrower row may set the limit between here and the launch)
         cudaError_t e = cudaFuncSetAttribute(ln_kernel<TX, TY, VEC, NV, TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+                                             VEC * NV * TPR * 2 * static_cast<int>(sizeof(float)));
         if (e != cudaSuccess) return e;
     }
     return launch_pdl(false, ln_kernel<TX, TY, VEC, NV, TPR>, dim3(static_cast<unsigned>(want < most ? want : most)),
@@ -522,7 +524,11 @@ cudaError_t ln_bwd_go(const dn8_layer_norm_bwd_args& a, cudaStream_t st, int* nr
                                                : ln_bwd_kernel<TX, TY, VEC, NV, 512>;
         // (the default limit of 48 KB counts the static part too: up to 16.5 KB, the sums of teams of 128)
         if (smem > 24 * 1024) {
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            // (as in ln_team: the most that any call of the instance asks for)
+            const size_t cols = static_cast<size_t>(per) * (a.C <= 8 * per ? 8 : a.C <= 32 * per ? 32 : a.C <= 128 * per ? 128 : 512);
+            const size_t widest = teams * cols * (2 * sizeof(TX) + sizeof(TY));
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(cols * sizeof(float) + (widest > most ? widest : most)));
             if (e != cudaSuccess) return e;
         }
         return launch_pdl(false, kernel, dim3(grid), dim3(a.C <= 128 * per ? 256 : 512), smem, st, a, stages);

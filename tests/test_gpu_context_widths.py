@@ -5,12 +5,14 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
 import torch
 
 import context_ref as ref
+from rsna_knee_efficiency_b200 import _native as nat
 from rsna_knee_efficiency_b200 import ops
 from test_gpu_context_ops import BF16, DEV, F16, F32, gen, randn
 
@@ -56,3 +58,37 @@ def test_widths_in_a_process_of_its_own():
 @pytest.mark.parametrize("C", WIDTHS)
 def test_widths(C, t, to):
     both_directions(301, C, t, to)
+
+
+@pytest.mark.parametrize("direction,widths", [("forward", (5200, 8000)), ("backward", (1064, 1664))])
+def test_two_widths_from_several_host_threads(direction, widths):
+    """Widths of one kernel instance that ask for different amounts of shared memory, called from four host threads
+    at the C entry (which lets go of Python's lock): no call is refused for what another thread asks."""
+    lib, refused, go = nat.lib(), [], threading.Barrier(4, timeout=60)
+
+    def work(C):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            x, y = (torch.ones(8, C, dtype=BF16, device=DEV) for _ in range(2))
+            mean, rstd = torch.zeros(8, device=DEV), torch.ones(8, device=DEV)
+            if direction == "forward":
+                fn = lib.dn8_layer_norm
+                a = nat.LayerNormArgs(x=x.data_ptr(), y=y.data_ptr(), rows=8, x_stride=C, y_stride=C, C=C, eps=1e-5)
+            else:
+                fn = lib.dn8_layer_norm_bwd
+                a = nat.LayerNormBwdArgs(dy=x.data_ptr(), x=x.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr(),
+                                         dx=y.data_ptr(), rows=8, dy_stride=C, x_stride=C, dx_stride=C, C=C)
+            a.x_type = a.y_type = nat.DN8_BF16
+            s.synchronize()
+            go.wait()
+            refused.append(sum(fn(a, s.cuda_stream) != nat.DN8_OK for _ in range(20000)))
+            s.synchronize()
+    switch = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    threads = [threading.Thread(target=work, args=(C,)) for C in widths * 2]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    sys.setswitchinterval(switch)
+    assert refused == [0] * 4
