@@ -22,7 +22,10 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+// Reports a CUDA error and clears it: left behind, it would be raised by whoever asks for the last error next. (One
+// that ended the context stays.)
 int cuda_fail(cudaError_t e, const char* what) {
+    (void)cudaGetLastError();
     return fail(DN8_ECUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
 
