@@ -322,14 +322,17 @@ __global__ void __launch_bounds__(AR_ROWS * 32) attn_join_kernel(const dn8_atten
     }
     __syncthreads();
     const Sequence sq = s_seq;
-    // (one share: the output is written)
-    if (sq.b < 0 || s_shares <= 1 || sq.blk % s_shares != 0) return;
+    const bool idle = sq.b < 0 || s_shares <= 1 || sq.blk % s_shares != 0;      // (one share: the output is written)
+    // A block with nothing to add leaves without waiting, and its room goes to one that has (where all wait, a token
+    // over each of 8 caches takes 109 us, not 105). But the first one always waits: were all to leave (nothing is cut),
+    // this grid would be over, and what comes after it let go, while the row kernel still writes.
+    if (!idle || (blockIdx.x == 0 && blockIdx.y == 0)) griddep_wait();
+    if (idle) return;
     const int rr = sq.blk / s_shares * AR_ROWS + r;
     if (rr >= sq.nq * G) return;
     // (offsets that go back and forth may ask for more shares than there is room for)
     const int shares = min(s_shares, plan.units - static_cast<int>(blockIdx.x));
     const size_t slot = static_cast<size_t>(kvh) * plan.units + blockIdx.x;
-    griddep_wait();
     float mm = -INFINITY;
     for (int s = lane; s < shares; s += 32) mm = fmaxf(mm, plan.ml[((slot + s) * AR_ROWS + r) * 2]);
 #pragma unroll
