@@ -44,7 +44,7 @@ constexpr float AF_SHARE = 4.0f;                      // key tiles of a share, a
 template <int DP> struct TileCfg {
     static constexpr int KST = DP == 64 ? 3 : 2, VST = DP == 64 ? 3 : 2;      // stages of K and V
     static constexpr uint32_t TILE = AT_TILE * DP * 2;
-    static constexpr uint32_t SMEM = 1024 + TILE * (2 + KST + VST) + 6144;
+    static constexpr uint32_t SMEM = 1024 + TILE * (2 + KST + VST) + 8192;
     // TMEM columns: S of the two tiles, P (over S, or of its own), O
     static constexpr bool OWN_P = DP == 64;
     static constexpr uint32_t S0 = 0, P0 = OWN_P ? 256 : 0, PG = OWN_P ? 64 : 128, O0 = OWN_P ? 384 : 256;
@@ -103,7 +103,7 @@ struct TileShared {
     uint64_t pfilled, pread;
     TilePiece piece[2];                               // of even and odd number
     uint32_t words[3][4];
-    float stat[2][2][AT_TILE];                        // [tile][sum, reference][row]
+    float stat[2][2][2][AT_TILE];                     // [turn][tile][sum, reference][row]
     SequenceTable table;
     uint32_t tmem;
     int abort;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
 attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                  const __grid_constant__ CUtensorMap mv, const dn8_attention_args a, const TilePlan plan) {
     using C = TileCfg<DP>;
-    static_assert(sizeof(TileShared) <= 6144, "shared state");
+    static_assert(sizeof(TileShared) <= 8192, "shared state");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sq = smem;
@@ -431,6 +431,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
         const int pair = 1 + g * 4 + quad;
         const float sc = a.scale * ATT_LOG2E;
         int ns = 0, no = 0, vc0 = 0;                  // scores and outputs so far; V tiles before this piece
+        int hand = 0;                                // outputs handed over so far, odd or even
         bool ok = true;
         for (int np = 0; ok && begin_piece(np); ++np) {
             const TilePiece& pc = sh.piece[np & 1];
@@ -568,8 +569,9 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             if (!ok) break;
             vc0 += pc.all.count;
             // The output: a row per thread, the two warps of these 32 rows half of the elements each. Sums and
-            // references change hands through shared memory (a warp writes here again only after a tile that its
-            // partner has taken part in).
+            // references change hands through shared memory, by turns in two places: a warp writes to a place again
+            // only after the barrier of the turn between, which its partner reaches when it has read this one. (Key
+            // tiles do not keep the two together: a piece of one tile waits for nobody before its sums are written.)
             float ls = 0.0f, ms = -INFINITY;
             if (tiles > 0) {
 #pragma unroll
@@ -577,13 +579,14 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
                     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
                     if ((lane & 3) == 0) {
-                        sh.stat[g][0][row + 8 * h] = l[h];
-                        sh.stat[g][1][row + 8 * h] = m[h];
+                        sh.stat[hand][g][0][row + 8 * h] = l[h];
+                        sh.stat[hand][g][1][row + 8 * h] = m[h];
                     }
                 }
                 pair_sync(pair);
-                ls = sh.stat[g][0][quad * 32 + lane];
-                ms = sh.stat[g][1][quad * 32 + lane];
+                ls = sh.stat[hand][g][0][quad * 32 + lane];
+                ms = sh.stat[hand][g][1][quad * 32 + lane];
+                hand ^= 1;
                 ok = mbar_wait_w(&sh.ofull[g], no & 1, a.err, abort_flag, ERR_WAIT_ACC | (74 << 4));
                 if (!ok || *abort_flag) break;
                 ++no;
