@@ -271,8 +271,9 @@ int dn8_rope(const dn8_rope_args* a, dn8_stream stream);
  * Query i of nq stands at p = i + nk - nq and sees key j iff keep[j] (a byte per key row, not zero),
  * j <= p + right, and (j >= p - left or j < sinks); left or right = -1: no limit on that side.
  * out = softmax(scale q k) v over the visible keys, lse = log sum exp(scale q k) (natural). A query
- * that sees nothing: out = 0, lse = -inf. What masked keys hold, and rows of no sequence, is never
- * used; rows of no sequence are not written. Visible keys and values have to be finite. Query head h
+ * that sees nothing: out = 0, lse = -inf. What keys hold that no query of their sequence sees (by keep,
+ * len_k or the window), and rows of no sequence, is never used; rows of no sequence are not written.
+ * Keys and values that some query sees have to be finite. Query head h
  * reads key head h / (Hq / Hk). Scores, softmax and sums in fp32; the weights are rounded to `type`
  * for the second product.
  * Offsets are checked on the device: a sequence that leaves [0, Tq] or [0, Tk], or a len_k outside its

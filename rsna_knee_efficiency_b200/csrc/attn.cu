@@ -15,8 +15,8 @@ namespace dn8 {
 // per tile and left the memory half idle; a TMA tile takes one, and tests are made per tile.
 // One token of each of 8 streams over caches of 1 to 32768 (551 MB of keys and values), 32 heads on 8, D = 128: 103 us,
 // 5.3 TB/s, 0.82 of the copy rate; 4 queries over 16 x 12288 tokens, 8 heads, D = 64 (403 MB): 77 us, 5.2 TB/s.
-// Rows of values that no query may see (behind the sequence's end, or keep = 0) are zeroed in shared
-// memory, since 0 * NaN is not 0; their scores are replaced, so keys may hold anything.
+// Rows of values that no query of the sequence may see (behind its end, keep = 0, or before every window) are zeroed
+// in shared memory, since 0 * NaN is not 0; their scores are replaced, so keys may hold anything.
 constexpr int AR_WARPS = 4, AR_ROWS = 16, AR_STAGES = 3;
 constexpr uint32_t AR_TILE_BYTES = 4096, AR_STAGE = 2 * AR_TILE_BYTES;
 
@@ -144,10 +144,11 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__
                 qf[kk][half + 2 * c] = live && d < a.D ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
             }
     }
+    const uint32_t hidden = hidden_keys(a, sq.nq, sq.nk);
     auto kept = [&](int t) -> bool {                     // this lane's key of tile index t may be seen
         if (t >= kt.count || lane >= KEYS) return true;
         const int j = kt.tile(t) * KEYS + lane;
-        return j < sq.nk && (a.keep == nullptr || a.keep[sq.k0 + j] != 0);
+        return j < sq.nk && behind_hidden(a, j, hidden) && (a.keep == nullptr || a.keep[sq.k0 + j] != 0);
     };
     bool next_kept = kept(me);
 

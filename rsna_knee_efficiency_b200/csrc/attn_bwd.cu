@@ -552,6 +552,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 const BwdPiece& pc = sh.piece[n & 1];
                 const bool kv = pc.kv != 0;
                 const int steps = pc.steps, q0 = pc.seq.q0, nq = pc.seq.nq, nk = pc.seq.nk;
+                const uint32_t hidden = hidden_keys(a, nq, nk);
                 int tile = pc.tile0, hx = pc.hx;
                 float l2[4], de[4];
                 bool live[4];
@@ -567,7 +568,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                             l2[w] = ws[0];
                             de[w] = ws[a.Hq * a.Tq];
                         }
-                        if (!kv) live[w] = x < nk && (a.keep == nullptr || a.keep[pc.seq.k0 + x] != 0);
+                        if (!kv) live[w] = x < nk && behind_hidden(a, x, hidden) && (a.keep == nullptr || a.keep[pc.seq.k0 + x] != 0);
                     }
                     if (tile == pc.turn) {
                         tile = pc.back;

@@ -198,6 +198,14 @@ struct KeyTiles {
         count = max(0, e - b);
     }
 };
+// Keys sinks .. sinks + hidden_keys() - 1 of a sequence lie before every query's window (the first query stands at
+// nk - nq): nobody sees them, and they may hold anything, like those behind nk or with keep = 0.
+template <typename A> DN8_DEV uint32_t hidden_keys(const A& a, int nq, int nk) {
+    return a.left < 0 ? 0u : static_cast<uint32_t>(max(0, nk - nq - a.left - a.sinks));
+}
+template <typename A> DN8_DEV bool behind_hidden(const A& a, int j, uint32_t hidden) {
+    return static_cast<uint32_t>(j - a.sinks) >= hidden;
+}
 // Keys that one of `rows` neighbouring queries sees, at most.
 template <typename A> DN8_DEV int seen_keys(const A& a, int rows, int nk) {
     if (a.left < 0 || a.right < 0) return nk;

@@ -25,8 +25,8 @@
 // two cycles of three, two threads of different warps per row had to meet in shared memory for every
 // tile). Warps 16 and 19: tcgen05 issue, one per query tile: an issue is some 25 instructions with its waits,
 // and one warp for both tiles was late for each by the other's. Warp 17: TMA. Warp 18: which piece comes
-// next, and rows of V that nobody may see (behind the sequence, keep = 0): they are zeroed in shared memory
-// before the product, since 0 * NaN is not 0 (their scores are replaced, so K may hold anything).
+// next, and rows of V that nobody may see (behind the sequence, keep = 0, before every window): they are zeroed in
+// shared memory before the product, since 0 * NaN is not 0 (their scores are replaced, so K may hold anything).
 #include "attn_umma.cuh"
 
 namespace dn8 {
@@ -257,6 +257,7 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
             for (int n = 0; pc.seq.b >= 0; ++n) {
                 const int count = pc.all.count, nk = pc.seq.nk, k0 = pc.seq.k0;
                 const KeyTiles all = pc.all;
+                const uint32_t hidden = hidden_keys(a, pc.seq.nq, nk);
                 const int ask_at = max(0, count - AF_AHEAD);
                 for (int u = 0; u < max(count, 1); ++u) {
                     if (u == ask_at) {
@@ -271,13 +272,16 @@ attn_tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__
                     }
                     if (u < count) {
                         const int t = all.tile(u), vs = vc % C::VST;
-                        const bool fix = a.keep != nullptr || (t + 1) * AT_TILE > nk;
+                        const bool fix = a.keep != nullptr || (t + 1) * AT_TILE > nk ||
+                                         (hidden > 0 && t * AT_TILE < a.sinks + static_cast<int>(hidden) &&
+                                          (t + 1) * AT_TILE > a.sinks);
                         uint32_t word[4];
                         if (fix)
 #pragma unroll
                             for (int w = 0; w < 4; ++w) {
                                 const int j = t * AT_TILE + w * 32 + lane;
-                                word[w] = __ballot_sync(0xffffffffu, j < nk && (a.keep == nullptr || a.keep[k0 + j] != 0));
+                                word[w] = __ballot_sync(0xffffffffu, j < nk && behind_hidden(a, j, hidden) &&
+                                                                         (a.keep == nullptr || a.keep[k0 + j] != 0));
                             }
                         ok = mbar_wait_w(&sh.vfull[vs], (vc / C::VST) & 1, a.err, abort_flag, ERR_WAIT_FULL | (66 << 4));
                         if (!ok) break;

@@ -328,8 +328,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tens
     (bool or uint8 [Tk]), j <= p + right and (j >= p - left or j < sinks); -1: no limit. right = 0 is
     causal; a single new token per sequence over caches is nq = 1. out = softmax(scale q k) v; scale
     defaults to D^-1/2; lse [Tq, Hq] fp32 is kept for the backward pass. A query that sees nothing:
-    0 and -inf. Masked keys may hold anything (NaN included), visible ones must be finite. Rows of no
-    sequence are left as they are. Offsets are read on the device: a sequence outside the tensors
+    0 and -inf. Keys that no query of their sequence sees (by keep, len_k or the window) may hold anything
+    (NaN included), the others must be finite. Rows of no sequence are left as they are. Offsets are read on the device: a sequence outside the tensors
     counts as empty and sets `err` (int32 [1]). `work`: uint8 of `dn8_attention_work` bytes,
     allocated if needed and not given."""
     c = "attention"
