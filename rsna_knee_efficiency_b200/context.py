@@ -25,6 +25,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
+from . import _native as nat
 from . import ops
 
 
@@ -119,7 +120,8 @@ class _Attention(torch.autograd.Function):
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor, **mask):
-    """`ops.attention` with a gradient; `mask`: left, right, sinks, keep, len_k, scale."""
+    """`ops.attention` with a gradient; `mask`: left, right, sinks, keep, len_k, scale, and `err`, the error word of
+    both directions."""
     _refuse_capture(q, k, v)
     return _Attention.apply(q, k, v, cu_q, cu_k, mask)
 
@@ -167,6 +169,18 @@ class ContextHead(nn.Module):
         self.query = nn.Parameter(torch.randn(n_out, heads, d))
         self.out_weight = nn.Parameter(torch.randn(n_out, heads * d) * (heads * d) ** -0.5)
         self.out_bias = nn.Parameter(torch.zeros(n_out))
+        # the error word of the head's attention kernels, forward and backward (see check)
+        self.register_buffer("err", torch.zeros(1, dtype=torch.int32), persistent=False)
+
+    def check(self) -> None:
+        """Raises if a kernel of the head, forward or backward, gave up a bounded wait, or met offsets outside the
+        tensors, since the last check (synchronises; its outputs hold zeros or rows that were never written then)."""
+        if self.err.is_cuda:
+            torch.cuda.synchronize(self.err.device)
+        code = int(self.err)
+        if code:
+            self.err.zero_()
+            raise nat.Dn8Error(f"ContextHead: a kernel gave up a bounded wait or met offsets outside the tensors (code {code})")
 
     def _linear(self, x: torch.Tensor, m: nn.Linear) -> torch.Tensor:
         return F.linear(x, m.weight.to(self.dtype), m.bias.to(self.dtype))
@@ -213,11 +227,11 @@ class ContextHead(nn.Module):
             y, tok = (la.norm1(tok), tok) if branch is None else la.norm1(branch, None, tok)
             q, k, v = self._linear(y, la.qkv).view(at, H + 2 * K, d).split((H, K, K), 1)
             q, k = rope(q, k, posn, self.sections, self.base, True)
-            o = attention(q, k, v, cu_k, cu_k, left=self.window, right=self.window, sinks=f, keep=kept)
+            o = attention(q, k, v, cu_k, cu_k, left=self.window, right=self.window, sinks=f, keep=kept, err=self.err)
             y, tok = la.norm2(self._linear(o.view(at, H * d), la.proj), None, tok)
             branch = self._linear(F.gelu(self._linear(y, la.up)), la.down)
         y = self.norm_out(tok) if branch is None else self.norm_out(branch, None, tok)[0]
         k, v = self._linear(y, self.kv).view(at, 2 * K, d).split((K, K), 1)
         q = self.query.to(self.dtype).repeat(b, 1, 1)
-        o = attention(q, k, v, cu_q, cu_k, keep=kept)
+        o = attention(q, k, v, cu_q, cu_k, keep=kept, err=self.err)
         return (o.view(b, self.n_out, H * d).float() * self.out_weight).sum(2) + self.out_bias

@@ -218,6 +218,12 @@ class StudyRunner:
         torch.mean(torch.stack(self.views), 0, out=self.out)
         return self.out
 
+    def check(self) -> None:
+        """Raises if a kernel of the encoders or the context heads gave up a bounded wait since the last check
+        (synchronises)."""
+        for part in (*self.encoders, *(self.context or ())):
+            part.check()
+
 
 def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> torch.Tensor:
     """Study logits [n_local, n_out] (float32, host) of this rank's contiguous shard of the studies
@@ -226,11 +232,13 @@ def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> t
     copied to the device on a copy stream (two staging buffers, the next batch's copy overlapping
     this batch's encoders), run, and their logits read back into pinned host memory; the last batch
     is padded by repeating its last study. `runner` needs `studies`, `device`, `n_out` and
-    `run(volumes_on_device)` (on the current stream)."""
+    `run(volumes_on_device)` (on the current stream); where it has a `check()`, that is called before the logits
+    are given out."""
     vols = torch.as_tensor(volumes)
     order = list(range(vols.shape[1])) if studies is None else [int(k) for k in studies]
     start, end = shard(len(order), world, rank)
     B, dev = runner.studies, runner.device
+    check = getattr(runner, "check", lambda: None)
     starts = list(range(start, end, B))
     on_gpu = str(dev).startswith("cuda")
     out = torch.empty((end - start, runner.n_out), dtype=torch.float32, pin_memory=on_gpu)
@@ -257,6 +265,7 @@ def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> t
         for s0 in starts:
             k = fill(stages[0], s0)
             out[s0 - start:s0 - start + k].copy_(runner.run(stages[0])[:k])
+        check()
         return out
     cur = torch.cuda.current_stream(dev)
     copy = torch.cuda.Stream(dev)
@@ -283,6 +292,7 @@ def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> t
         k = min(B, end - s0)
         out[s0 - start:s0 - start + k].copy_(logits[:k], non_blocking=True)
     cur.synchronize()
+    check()
     return out
 
 
