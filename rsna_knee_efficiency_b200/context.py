@@ -29,11 +29,19 @@ from . import _native as nat
 from . import ops
 
 
+_NO_CAPTURE = "autograd through these operators cannot be captured: capture ops.*_backward, or use torch.no_grad()"
+
+
 def _refuse_capture(*tensors) -> None:
     if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing() and \
             any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("autograd through these operators cannot be captured: capture ops.*_backward, or use "
-                           "torch.no_grad()")
+        raise RuntimeError(_NO_CAPTURE)
+
+
+def _refuse_captured_backward() -> None:
+    """(of a forward pass that was not captured)"""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(_NO_CAPTURE)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -52,6 +60,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dsum=None):
+        _refuse_captured_backward()
         h, weight, mean, rstd = ctx.saved_tensors
         dx = torch.empty_like(h, memory_format=torch.contiguous_format)
         dw = None if weight is None else torch.empty_like(weight)
@@ -84,6 +93,7 @@ class _Rope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
+        _refuse_captured_backward()
         pos, = ctx.saved_tensors
         dq, dk = dq.contiguous(), dk.contiguous()
         out = [torch.empty_like(t) for t in (dq, dk)]
@@ -113,6 +123,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        _refuse_captured_backward()
         q, k, v, out, lse, cu_q, cu_k, keep, len_k = ctx.saved_tensors
         grads = [torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
         ops.attention_backward(dout.contiguous(), q, k, v, out, lse, *grads, cu_q, cu_k, keep=keep, len_k=len_k, **ctx.mask)
