@@ -207,7 +207,7 @@ int dn8_zoom(const dn8_zoom_args* a, dn8_stream stream);
 
 /* Layer norm of `rows` rows of C elements: h = x + res (rounded to x's type and written to sum; h = x
  * without res), mu = mean(h), r = 1 / sqrt(mean((h - mu)^2) + eps), y = (h - mu) r w + b. Statistics
- * in fp32. y may be x or res itself where types and strides agree, and so may sum. */
+ * in fp32. rows below 2^31, C below 2^29. y may be x or res itself where types and strides agree, and so may sum. */
 typedef struct dn8_layer_norm_args {
     const void* x;          /* [rows][C] x_type */
     const void* res;        /* x_type, or NULL */

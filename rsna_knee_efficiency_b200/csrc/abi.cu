@@ -227,11 +227,12 @@ int dn8_head_noalloc(const dn8_head_args* a, dn8_stream stream) {
 
 // ---- the context transformer's operators ----
 
+constexpr int LN_MOST_C = 1 << 29;      // (the kernels' column numbers, up to 2 C, stay in 32 bits)
 static bool float_type(int t) { return t == DN8_F32 || t == DN8_F16 || t == DN8_BF16; }
 
 int dn8_layer_norm(const dn8_layer_norm_args* a, dn8_stream stream) {
     if (a == nullptr) return fail(DN8_EINVAL, "dn8_layer_norm: null arguments");
-    if (a->rows < 0 || a->rows >= (1ll << 31) || a->C < 1 || !(a->eps >= 0.0f))
+    if (a->rows < 0 || a->rows >= (1ll << 31) || a->C < 1 || a->C >= LN_MOST_C || !(a->eps >= 0.0f))
         return fail(DN8_EINVAL, "dn8_layer_norm: bad geometry rows=%lld C=%d eps=%g", static_cast<long long>(a->rows), a->C,
                     a->eps);
     if (!float_type(a->x_type) || !float_type(a->y_type) || !float_type(a->w_type) ||
@@ -247,11 +248,13 @@ int dn8_layer_norm(const dn8_layer_norm_args* a, dn8_stream stream) {
     return e == cudaSuccess ? DN8_OK : cuda_fail(e, "dn8_layer_norm launch");
 }
 
-int64_t dn8_layer_norm_bwd_work(int32_t C) { return C < 1 ? -1 : static_cast<int64_t>(dn8::layer_norm_bwd_work(C)); }
+int64_t dn8_layer_norm_bwd_work(int32_t C) {
+    return C < 1 || C >= LN_MOST_C ? -1 : static_cast<int64_t>(dn8::layer_norm_bwd_work(C));
+}
 
 int dn8_layer_norm_bwd(const dn8_layer_norm_bwd_args* a, dn8_stream stream) {
     if (a == nullptr) return fail(DN8_EINVAL, "dn8_layer_norm_bwd: null arguments");
-    if (a->rows < 0 || a->rows >= (1ll << 31) || a->C < 1)
+    if (a->rows < 0 || a->rows >= (1ll << 31) || a->C < 1 || a->C >= LN_MOST_C)
         return fail(DN8_EINVAL, "dn8_layer_norm_bwd: bad geometry rows=%lld C=%d", static_cast<long long>(a->rows), a->C);
     if (!float_type(a->x_type) || !float_type(a->y_type) || !float_type(a->w_type) ||
         (a->x_type != a->y_type && a->x_type != DN8_F32))

@@ -93,6 +93,8 @@ def head_noalloc(in0: torch.Tensor, seg: torch.Tensor, fab: torch.Tensor, G0: in
 _TYPES = {torch.float32: nat.DN8_F32, torch.float16: nat.DN8_F16, torch.bfloat16: nat.DN8_BF16}
 _ANY = tuple(_TYPES)
 _HALF = (torch.float16, torch.bfloat16)
+# Sizes that the C structures hold in 32 bits are refused beyond these (ctypes would drop the upper bits)
+_MOST_C, _MOST_HEADS, _MOST_SEQUENCES = 1 << 29, 65535, 1 << 30
 _F32, _I32, _U8, _FLAG = (torch.float32,), (torch.int32,), (torch.uint8,), (torch.bool, torch.uint8)
 
 
@@ -204,6 +206,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
     shape = M, C = x.shape
     t = x.dtype
     same = (t,)
+    if C >= _MOST_C:
+        raise ValueError(f"{c}: rows of {C} elements (below 2^29)")
     if (res is None) != (sum is None):
         raise ValueError(f"{c}: res and sum come together")
     xs = _rows(c, "x", x, shape, same, dev)
@@ -238,6 +242,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     shape = M, C = x.shape
     t = x.dtype
     same = (t,)
+    if C >= _MOST_C:
+        raise ValueError(f"{c}: rows of {C} elements (below 2^29)")
     xs, gs = _rows(c, "x", x, shape, same, dev), _rows(c, "dy", dy, shape, _ANY if t is torch.float32 else same, dev)
     ds = 0 if dsum is None else _rows(c, "dsum", dsum, shape, same, dev)
     os = _rows(c, "dx", dx, shape, same, dev, True)
@@ -277,6 +283,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, q_out: torc
     axes = len(sections)
     if not 1 <= axes <= nat.DN8_ROPE_AXES:
         raise ValueError(f"{c}: 1 to {nat.DN8_ROPE_AXES} axes")
+    if min(sections) < 0 or 2 * sum(sections) > D or Hq > _MOST_HEADS or D > _MOST_HEADS:
+        raise ValueError(f"{c}: sections {tuple(sections)} of {Hq} heads of {D} elements")
     _flat(c, "pos", pos, (T, axes), _I32, dev)
     if pos is None or (k is None) != (k_out is None):
         raise ValueError(f"{c}: pos is needed, and k and k_out come together")
@@ -286,6 +294,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, q_out: torc
         if not isinstance(k, torch.Tensor) or k.dim() != 3:
             raise ValueError(f"{c}: k [T, H, D] expected")
         Hk = k.shape[1]
+        if Hk > _MOST_HEADS:
+            raise ValueError(f"{c}: {Hk} heads")
         ks, ko = _heads(c, "k", k, (T, Hk, D), t, dev), _heads(c, "k_out", k_out, (T, Hk, D), t, dev, True)
     a = nat.RopeArgs(q.data_ptr(), _ptr(k), pos.data_ptr(), q_out.data_ptr(), _ptr(k_out), T, *qs, *ks, *qo, *ko, Hq, Hk,
                      D, _TYPES[t[0]], axes, _SECTIONS(*sections), per_axis, interleaved, inverse, base)
@@ -303,8 +313,10 @@ def _packed(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, s
     sq, sk = q.shape, k.shape
     t = (q.dtype,)
     n = cu_q.shape[0]
-    if n < 1 or cu_k is None or sk[2] != sq[2]:
+    if n < 1 or n > _MOST_SEQUENCES or cu_k is None or sk[2] != sq[2]:
         raise ValueError(f"{c}: cu_q and cu_k int32 [B + 1], q and k of one head size expected")
+    if sq[1] > _MOST_HEADS or sk[1] > _MOST_HEADS or sq[2] > _MOST_HEADS or min(left, right, sinks) < -1:
+        raise ValueError(f"{c}: q {tuple(sq)}, k {tuple(sk)}, left={left}, right={right}, sinks={sinks}")
     _flat(c, "cu_q", cu_q, (n,), _I32, dev)
     _flat(c, "cu_k", cu_k, (n,), _I32, dev)
     _flat(c, "len_k", len_k, (n - 1,), _I32, dev)
