@@ -95,7 +95,7 @@ _ANY = tuple(_TYPES)
 _HALF = (torch.float16, torch.bfloat16)
 # Sizes that the C structures hold in 32 bits are refused beyond these (ctypes would drop the upper bits)
 _MOST_C, _MOST_HEADS, _MOST_SEQUENCES = 1 << 29, 65535, 1 << 30
-_F32, _I32, _U8, _FLAG = (torch.float32,), (torch.int32,), (torch.uint8,), (torch.bool, torch.uint8)
+_F32, _I32, _FLAG = (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
 
 
 def _refuse(call: str, name: str, t, shape, types, dev, what: str) -> None:
