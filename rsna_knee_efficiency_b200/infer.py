@@ -171,6 +171,7 @@ class StudyRunner:
 
     @property
     def launches_per_call(self) -> int:
+        """Kernel launches of the encoders (and of the zoom) in one `run`; those of context heads are not counted."""
         per_pass = 2 + 2 * sum(b["L"] for b in self.encoders[0].meta["blocks"]) + \
             sum(1 for b in self.encoders[0].meta["blocks"] if b["trans"])
         passes = sum(-(-n // e.nb) for n, e in zip(self.n_img, self.encoders))
@@ -225,15 +226,16 @@ class StudyRunner:
             part.check()
 
 
-def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> torch.Tensor:
+def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None, present=None) -> torch.Tensor:
     """Study logits [n_local, n_out] (float32, host) of this rank's contiguous shard of the studies
     (`studies`: indices into `volumes`, default all of them, in order; `volumes`: uint8 [windows,
     n_volumes, S, H, W] in host memory, pinned for overlap). Batches of `runner.studies` studies are
     copied to the device on a copy stream (two staging buffers, the next batch's copy overlapping
     this batch's encoders), run, and their logits read back into pinned host memory; the last batch
     is padded by repeating its last study. `runner` needs `studies`, `device`, `n_out` and
-    `run(volumes_on_device)` (on the current stream); where it has a `check()`, that is called before the logits
-    are given out."""
+    `run(volumes_on_device)` (on the current stream); where it has a `check()`, that is called before the
+    logits are given out. `present`: bool [n_volumes, windows], the crop windows that each study has, for a
+    runner with context heads (`run(volumes, present)`; default: all)."""
     vols = torch.as_tensor(volumes)
     order = list(range(vols.shape[1])) if studies is None else [int(k) for k in studies]
     start, end = shard(len(order), world, rank)
@@ -242,6 +244,18 @@ def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> t
     starts = list(range(start, end, B))
     on_gpu = str(dev).startswith("cuda")
     out = torch.empty((end - start, runner.n_out), dtype=torch.float32, pin_memory=on_gpu)
+    have = None
+    if present is not None:
+        present = torch.as_tensor(present)
+        if tuple(present.shape) != (vols.shape[1], vols.shape[0]) or present.dtype != torch.bool:
+            raise ValueError(f"present {tuple(present.shape)} {present.dtype}: bool [{vols.shape[1]}, {vols.shape[0]}] expected")
+        pad = -(end - start) % B if starts else 0
+        idx = order[start:end] + order[end - 1:end] * pad
+        have = present[torch.tensor(idx, dtype=torch.long, device=present.device)].to(dev)     # (once, not between batches)
+
+    def run(j, st):
+        return runner.run(st) if have is None else runner.run(st, have[j * B:(j + 1) * B])
+
     shape = (vols.shape[0], B) + tuple(vols.shape[2:])
     stages = [torch.empty(shape, dtype=torch.uint8, device=dev) for _ in range(2 if on_gpu else 1)]
 
@@ -262,9 +276,9 @@ def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> t
         return k
 
     if not on_gpu:
-        for s0 in starts:
+        for j, s0 in enumerate(starts):
             k = fill(stages[0], s0)
-            out[s0 - start:s0 - start + k].copy_(runner.run(stages[0])[:k])
+            out[s0 - start:s0 - start + k].copy_(run(j, stages[0])[:k])
         check()
         return out
     cur = torch.cuda.current_stream(dev)
@@ -286,7 +300,7 @@ def run_shard(runner, volumes, rank: int = 0, world: int = 1, studies=None) -> t
         if j + 1 < len(starts):
             load(j + 1)
         cur.wait_event(loaded[j & 1])
-        logits = runner.run(stages[j & 1])
+        logits = run(j, stages[j & 1])
         freed[j & 1] = torch.cuda.Event()
         freed[j & 1].record(cur)
         k = min(B, end - s0)
