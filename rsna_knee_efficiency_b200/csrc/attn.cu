@@ -13,8 +13,8 @@ namespace dn8 {
 // maximum, sum and output; the warps are joined in shared memory, the shares of the key axis by
 // attn_join_kernel. Loads by cp.async with an address and a mask test per 16 bytes took 767 instructions
 // per tile and left the memory half idle; a TMA tile takes one, and tests are made per tile.
-// One token of each of 8 streams over caches of 1 to 32768 (551 MB of keys and values), 32 heads on 8, D = 128: 103 us,
-// 5.3 TB/s, 0.82 of the copy rate; 4 queries over 16 x 12288 tokens, 8 heads, D = 64 (403 MB): 77 us, 5.2 TB/s.
+// One token of each of 8 streams over caches of 1 to 32768 (551 MB of keys and values), 32 heads on 8, D = 128: 105 us,
+// 5.2 TB/s, 0.81 of the copy rate; 4 queries over 16 x 12288 tokens, 8 heads, D = 64 (403 MB): 78 us, 5.1 TB/s.
 // Rows of values that no query of the sequence may see (behind its end, keep = 0, or before every window) are zeroed
 // in shared memory, since 0 * NaN is not 0; their scores are replaced, so keys may hold anything.
 constexpr int AR_WARPS = 4, AR_ROWS = 16, AR_STAGES = 3;

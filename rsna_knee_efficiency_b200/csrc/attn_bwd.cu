@@ -21,9 +21,11 @@
 // tile is seen by every query: its walk is cut into shares, whose sums attn_bwd_join_kernel adds (and where heads are
 // few, every long walk of dk and dv).
 //
-// 2 x 8192 tokens, 16 heads, no mask: D = 64 2045 us (671 TFLOP/s of the 10 D per pair), D = 128 3440 us (800). Bound by no
-// single unit: at views of 6160 with windows of 512 to each side, D = 64, 422 us; 403 without the exponentials, 378
-// without the product of dS, 401 with half of the value products.
+// 2 x 8192 tokens, 16 heads, no mask, in bursts at 1965 MHz: D = 64 2083 us (660 TFLOP/s of the 10 D per pair), D =
+// 128 3171 us (867). Bound by the latency of a step's chain: at views of 6160 with windows of 512 to each side, D = 64
+// (436 us), issue slots are busy for 0.50 of the time, special function units for 0.38, tensor cores for 0.33, and
+// taking work away gained little (from 422 us then: 403 without the exponentials, 378 without the product of dS, 401
+// with half of the value products).
 #include <type_traits>
 
 #include "attn_umma.cuh"

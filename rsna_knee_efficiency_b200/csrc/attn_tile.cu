@@ -14,11 +14,13 @@
 // A CTA takes one piece after the other (ask_for_block): the loads and first scores of the next piece run
 // while the threads still write the last one's output. A piece costs some 5 us beyond its tiles (1.4 us each at
 // D <= 64), so for short sequences the next one is asked for early and looked up in shared memory: 128 x 128
-// tokens, 16 heads, D = 64, 90 us with the question behind V and offsets from memory, 74.
+// tokens, 16 heads, D = 64, 66 us (with the question behind V and offsets from memory it was 90, not 74).
 //
-// 2 x 8192 tokens, 16 heads, no mask: D = 64 658 us (835 TFLOP/s, bound by the special function units: the
-// exponentials alone take 0.7 of it, then by the latency of a tile's steps), D = 128 945 us (1163 TFLOP/s, 0.68 of
-// the measured matrix rate). Four views of 6144, causal, 8 heads, D = 128: 326 us.
+// In bursts at 1965 MHz: 2 x 8192 tokens, 16 heads, no mask, D = 64 689 us (798 TFLOP/s; the exponentials alone take
+// 0.67 of it at the special function units' rate), D = 128 1006 us (1093 TFLOP/s, 0.64 of the measured matrix rate).
+// Four views of 6144, causal, 8 heads, D = 128: 340 us, and 370 in a loop, where the power cap holds the clock at
+// 1715 MHz. Bound by the latency of a tile's steps: issue slots, special function units and tensor cores are each
+// busy for 0.41 to 0.56, 0.48 and 0.24 to 0.48 of the time (windows at D = 64, causal at D = 128).
 //
 // Warps 0-7 and 8-15: softmax of tile 0 and 1, a warp per 16 rows and four threads per row, so that a row's
 // maximum takes two shuffles (32 scores of two rows a thread; one thread per row left the schedulers idle
@@ -37,7 +39,7 @@ constexpr int AF_THREADS = 640;
 constexpr int AF_REGS_SOFTMAX = 104, AF_REGS_OTHER = 64;
 // How many tiles before the end of a piece the next one is asked for: time enough to hide the question and the
 // first loads. Asked for at the start, a piece waits behind a long one while others run out of work: four
-// sequences of 6144, causal, took 364 us instead of 317.
+// sequences of 6144, causal, D = 128, take 360 us instead of 344 (in a loop under the power cap 383, not 371).
 constexpr int AF_AHEAD = 4;
 constexpr float AF_SHARE = 4.0f;                      // key tiles of a share, at least
 

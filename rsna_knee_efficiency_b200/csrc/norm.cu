@@ -8,7 +8,7 @@
 // Both passes are bound by memory: a row is read once into registers (a team of 8, 32, 128 or 512
 // threads per row, so that a thread holds at most 32 values), the variance is summed from the
 // registers as squares of differences (no cancellation of E[x^2] - mu^2), and written once.
-// Statistics and sums are fp32. 98304 rows of 512 bf16 with a residual (403 MB): 76 us, 5.3 TB/s of 6.5 for a copy.
+// Statistics and sums are fp32. 98304 rows of 512 bf16 with a residual (403 MB): 77 us, 5.2 TB/s of 6.5 for a copy.
 // Narrow rows share a warp: 67678 rows of 31 bf16 took 52 us with a warp each and
 // take 11 with eight threads each, 90000 of 64 (fp32 in, fp16 out) 40 and 17.
 #include "ctx_common.cuh"
@@ -221,7 +221,7 @@ DN8_DEV void wait_copies(int n) {
 // and dy over the block's rows stay in its registers. Rows of 16-byte vectors come through a ring of `stages` rows
 // per team in shared memory: every thread copies and reads its own vectors, so nobody waits for anybody. (One
 // row ahead in registers is too little in flight: 23664 rows of 2016, fp32 and fp16, took 117 us and take 88; 98304 of
-// 512 bf16 with dsum 77 and 73, 5.5 TB/s; 20427 of 1064 fp16, bound by instructions, 50 and 53.) The sums are added
+// 512 bf16 with dsum 77 and 74, 5.4 TB/s; 20427 of 1064 fp16, bound by instructions, 50 and 53.) The sums are added
 // over the teams in shared memory and written as one row of the workspace [gridDim.x][2][C]; ln_cols_kernel adds
 // the rows in a fixed order (no atomics: the same bits every call).
 template <typename TX, typename TY, int VEC, int NV, int TPR>

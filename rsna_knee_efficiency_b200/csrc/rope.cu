@@ -23,7 +23,8 @@ constexpr int RP_THREADS = 256;
 constexpr int RP_MAX_PAIRS = 128;
 constexpr int RP_BATCH = 2;                       // items a thread has in flight
 // Items of 16 bytes per thread that a block is cut for: 98304 tokens of 20 heads, D = 64, bf16 (503 MB): 99 us
-// with 4, 93 with 8 (5.4 TB/s), 95 with 16; single elements (10626 tokens, 10 heads, 31 pairs) 23, 29, 29.
+// with 4, 93 with 8 (93 to 97 from one B200 to the next: 5.2 to 5.4 TB/s), 95 with 16; single elements (10626
+// tokens, 10 heads, 31 pairs) 23, 29, 29.
 constexpr int RP_BLOCK_WIDE = 8, RP_BLOCK_NARROW = 4;
 
 struct RopeTable {
