@@ -180,14 +180,22 @@ class ContextHead(nn.Module):
         self.query = nn.Parameter(torch.randn(n_out, heads, d))
         self.out_weight = nn.Parameter(torch.randn(n_out, heads * d) * (heads * d) ** -0.5)
         self.out_bias = nn.Parameter(torch.zeros(n_out))
-        # the error word of the head's attention kernels, forward and backward (see check)
-        self.register_buffer("err", torch.zeros(1, dtype=torch.int32), persistent=False)
+        # The error word of the head's attention kernels, forward and backward (see check), made by the first call on
+        # a device. No buffer: wrappers that share buffers between ranks would overwrite one rank's by another's.
+        self.err: torch.Tensor | None = None
+
+    def _error_word(self, dev: torch.device) -> torch.Tensor:
+        if self.err is None or self.err.device != dev:
+            with torch.inference_mode(False):                # (check clears it, in whatever mode)
+                self.err = torch.zeros(1, dtype=torch.int32, device=dev)
+        return self.err
 
     def check(self) -> None:
         """Raises if a kernel of the head, forward or backward, gave up a bounded wait, or met offsets outside the
         tensors, since the last check (synchronises; its outputs hold zeros or rows that were never written then)."""
-        if self.err.is_cuda:
-            torch.cuda.synchronize(self.err.device)
+        if self.err is None:
+            return
+        torch.cuda.synchronize(self.err.device)
         code = int(self.err)
         if code:
             self.err.zero_()
@@ -223,7 +231,7 @@ class ContextHead(nn.Module):
             raise ValueError(f"features {tuple(feats.shape)}, expected {(n, self.c)}")
         if tuple(pos.shape) != (n, 2) or (keep is not None and tuple(keep.shape) != (n,)):
             raise ValueError(f"pos [{n}, 2] and keep [{n}] expected")
-        rows, cu_k, cu_q = lay["rows"], lay["cu_k"], lay["cu_q"]
+        rows, cu_k, cu_q, err = lay["rows"], lay["cu_k"], lay["cu_q"], self._error_word(dev)
         posn = torch.zeros(at, 2, dtype=torch.int32, device=dev).index_copy_(0, rows, pos)
         kept = None
         if keep is not None:
@@ -238,11 +246,11 @@ class ContextHead(nn.Module):
             y, tok = (la.norm1(tok), tok) if branch is None else la.norm1(branch, None, tok)
             q, k, v = self._linear(y, la.qkv).view(at, H + 2 * K, d).split((H, K, K), 1)
             q, k = rope(q, k, posn, self.sections, self.base, True)
-            o = attention(q, k, v, cu_k, cu_k, left=self.window, right=self.window, sinks=f, keep=kept, err=self.err)
+            o = attention(q, k, v, cu_k, cu_k, left=self.window, right=self.window, sinks=f, keep=kept, err=err)
             y, tok = la.norm2(self._linear(o.view(at, H * d), la.proj), None, tok)
             branch = self._linear(F.gelu(self._linear(y, la.up)), la.down)
         y = self.norm_out(tok) if branch is None else self.norm_out(branch, None, tok)[0]
         k, v = self._linear(y, self.kv).view(at, 2 * K, d).split((K, K), 1)
         q = self.query.to(self.dtype).repeat(b, 1, 1)
-        o = attention(q, k, v, cu_q, cu_k, keep=kept, err=self.err)
+        o = attention(q, k, v, cu_q, cu_k, keep=kept, err=err)
         return (o.view(b, self.n_out, H * d).float() * self.out_weight).sum(2) + self.out_bias

@@ -26,12 +26,13 @@ def beyond(lay):
 def test_head(grad):
     torch.manual_seed(1)
     m = ContextHead(c=64, n_out=3, width=64, heads=2, window=4).to(DEV)
-    assert "err" not in m.state_dict() and m.err.device == torch.device(DEV)
+    m.check()                                                # (no call yet: nothing to report)
     feats, pos = torch.randn(20, 64, device=DEV), torch.zeros(20, 2, dtype=torch.int32, device=DEV)
     lay = m.layout([12, 8], DEV)
     with torch.set_grad_enabled(grad):
         good = m(feats, lay, pos)
         m.check()
+        assert "err" not in m.state_dict() and not list(m.buffers()) and m.err.device == torch.device(DEV)
         bad = m(feats, beyond(lay), pos)
     with pytest.raises(nat.Dn8Error, match="code 4"):
         m.check()
@@ -59,3 +60,26 @@ def test_study_loop():
         infer.run_shard(runner, vols)
     runner.layouts[1] = good
     assert torch.equal(infer.run_shard(runner, vols), want)
+
+
+def test_first_call_in_inference_mode_or_in_a_capture():
+    torch.manual_seed(2)
+    feats, pos = torch.randn(20, 64, device=DEV), torch.zeros(20, 2, dtype=torch.int32, device=DEV)
+    m = ContextHead(c=64, n_out=3, width=64, heads=2).to(DEV)
+    bad = beyond(m.layout([12, 8], DEV))
+    with torch.inference_mode():
+        m(feats, bad, pos)
+    with pytest.raises(nat.Dn8Error):
+        m.check()
+    m.check()
+    n = ContextHead(c=64, n_out=3, width=64, heads=2).to(DEV)
+    m(feats, m.layout([20], DEV), pos)                       # (the libraries' own first calls)
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            n(feats, bad, pos)
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(nat.Dn8Error):
+            n.check()
+        n.check()
