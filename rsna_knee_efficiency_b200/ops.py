@@ -341,9 +341,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tens
     causal; a single new token per sequence over caches is nq = 1. out = softmax(scale q k) v; scale
     defaults to D^-1/2; lse [Tq, Hq] fp32 is kept for the backward pass. A query that sees nothing:
     0 and -inf. Keys that no query of their sequence sees (by keep, len_k or the window) may hold anything
-    (NaN included), the others must be finite. Rows of no sequence are left as they are. Offsets are read on the device: a sequence outside the tensors
-    counts as empty and sets `err` (int32 [1]). `work`: uint8 of `dn8_attention_work` bytes,
-    allocated if needed and not given."""
+    (NaN included), the others must be finite. Rows of no sequence are left as they are. Offsets are read
+    on the device: a sequence outside the tensors counts as empty and sets `err` (int32 [1]). `work`:
+    uint8 of `dn8_attention_work` bytes, allocated if needed and not given."""
     c = "attention"
     dev, sq, sk, t, strides, mask = _packed(c, q, k, v, cu_q, cu_k, len_k, keep, lse, err, left, right, sinks, scale)
     os = _heads(c, "out", out, sq, t, dev, True)
